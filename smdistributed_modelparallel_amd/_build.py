@@ -129,6 +129,12 @@ def build_kernels(jobs=8, verbose=False):
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
         "-munsafe-fp-atomics",
         "-Wno-unused-result",
+        # no packed fp32 arithmetic (v_pk_add/mul/fma_f32): hipcc -O3 forms it from plain float code,
+        # and some of its forms have given wrong results on this hardware now and then
+        "-Xclang",
+        "-target-feature",
+        "-Xclang",
+        "-packed-fp32-ops",
     ]
     tasks, objs = [], []
     for s in hip_srcs:
