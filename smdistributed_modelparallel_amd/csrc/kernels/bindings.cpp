@@ -6,6 +6,7 @@
 
 #include "kernels.h"
 #include "../torchrt/torchrt.h"
+#include "training_ops.h"
 
 namespace {
 
@@ -837,6 +838,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "smdistributed_modelparallel_amd CDNA4 (gfx950) kernels + torch-aware runtime";
   smprt_torch::register_bindings(m);
   m.def("fused_adam", &fused_adam);
+  register_training_ops(m);
   m.def("fused_sgd", &fused_sgd);
   m.def("fused_adagrad", &fused_adagrad);
   m.def("mt_adam", &mt_adam);

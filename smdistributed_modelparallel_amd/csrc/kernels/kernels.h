@@ -232,4 +232,22 @@ int strided_copy4(int elem_bytes, const void* src, void* dst, const int64_t* siz
 // kernel of the pull stream (no copy-engine queue shared with the process's other streams).
 int device_copy(void* dst, const void* src, int64_t nbytes, hipStream_t s);
 
+// ------------------------------------------------------------------ embedding (embedding.hip)
+// A list of row numbers of a table of `rows` rows whose first row has the id `start`: int32 or
+// int64 (`wide`) ids, or -- ids null -- the numbers t % period.
+struct IndexList {
+  const void* ids = nullptr;
+  int wide = 1;
+  int64_t start = 0, rows = 0, period = 1;
+};
+// y[t] = scale * w[row of ids[t]] (+ p[row of pos[t]]), p may be null.  An id that is none of the
+// table's rows gives zeros (foreign_zero: another shard holds it) or NaN; a position NaN.
+int embedding_fwd(int dt, const IndexList& ids, const void* w, int64_t w_stride, float scale, int foreign_zero,
+                  const IndexList& pos, const void* p, int64_t p_stride, void* y, int64_t n, int64_t d,
+                  hipStream_t s);
+// dw[v] = scale * sum of dy[t] over the tokens of row v, or added to dw (accumulate); row `skip`
+// (-1: none) gets no gradient.
+int embedding_bwd(int dt, const IndexList& ids, const void* dy, int64_t n, int64_t d, float scale, int64_t skip,
+                  void* dw, int accumulate, hipStream_t s);
+
 }  // namespace smpk

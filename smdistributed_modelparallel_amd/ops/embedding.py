@@ -1,0 +1,138 @@
+"""Token embedding with scale, position table and vocabulary shards; gradients by sorted tokens.
+
+``y[t] = scale * weight[ids[t]] + position_weight[position[t]]``, formed in fp32 and rounded once
+into the tables' dtype, in one kernel (`csrc/kernels/embedding.hip`).  The backward adds the
+gradient rows of each token's occurrences in token order and in fp32 -- the same bits on every
+run -- and writes the parameters' flat-buffer gradients in place where they are bound
+(`parallel/flat.py`): only the rows that occur are touched then, and no dense gradient exists.
+CPU tensors (and torch.autocast regions) use plain torch operations.
+"""
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ..backend.exceptions import SMPInvalidArgumentError
+from ._ext import ext, fused_ok
+from .linear import _fusable
+
+
+def _table_grad(weight, dy, ids, period, scale, start, skip):
+    """Gradient of one table; None when it went into the bound gradient in place."""
+    if _fusable(weight):
+        ext().embedding_bwd(dy, ids, period, scale, start, skip, weight.grad, True)
+        return None
+    dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
+    ext().embedding_bwd(dy, ids, period, scale, start, skip, dw, False)
+    return dw
+
+
+class _EmbeddingHIP(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, position_weight, ids, position_ids, padding_idx, scale, vocab_start):
+        flat = ids.reshape(-1).contiguous()
+        pos = position_ids.reshape(-1).contiguous() if position_ids is not None else None
+        period = ids.shape[-1] if position_weight is not None and pos is None else 1
+        start = vocab_start or 0
+        w = weight if weight.stride(1) == 1 else weight.contiguous()
+        pw = position_weight
+        if pw is not None and pw.stride(1) != 1:
+            pw = pw.contiguous()
+        y = ext().embedding_fwd(flat, w, scale, start, vocab_start is not None, pos, pw, period)
+        ctx.save_for_backward(flat, pos)
+        # the tables' values are not needed again: they may change before the backward
+        ctx.tables = (weight, position_weight)
+        ctx.args = (period, scale, start, -1 if padding_idx is None else padding_idx - start)
+        return y.view(*ids.shape, weight.shape[1])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        flat, pos = ctx.saved_tensors
+        weight, position_weight = ctx.tables
+        period, scale, start, skip = ctx.args
+        dy2 = dy.reshape(-1, weight.shape[1]).contiguous()
+        dw = dpw = None
+        if ctx.needs_input_grad[0]:
+            dw = _table_grad(weight, dy2, flat, 1, scale, start, skip)
+        if ctx.needs_input_grad[1]:
+            dpw = _table_grad(position_weight, dy2, pos, period, 1.0, 0, -1)
+        return dw, dpw, None, None, None, None, None
+
+
+def _embedding_torch(ids, weight, padding_idx, scale, vocab_start, position_ids, position_weight):
+    rows = weight.shape[0]
+    if vocab_start is None:
+        y = torch.nn.functional.embedding(ids, weight, padding_idx)
+    else:
+        local = ids - vocab_start
+        outside = (local < 0) | (local >= rows)
+        pad = None
+        if padding_idx is not None and vocab_start <= padding_idx < vocab_start + rows:
+            pad = padding_idx - vocab_start
+        y = torch.nn.functional.embedding(local.clamp(0, rows - 1), weight, pad)
+        y = y.masked_fill(outside.unsqueeze(-1), 0.0)
+    if position_weight is None:
+        return y if scale == 1.0 else (y.float() * scale).to(weight.dtype)
+    if position_ids is None:
+        position_ids = torch.arange(ids.shape[-1], device=ids.device).expand(ids.shape)
+    p = torch.nn.functional.embedding(position_ids, position_weight)
+    return (y.float() * scale + p.float()).to(weight.dtype)
+
+
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _check_ids(name, t, device):
+    if not torch.is_tensor(t) or t.dtype not in (torch.int32, torch.int64):
+        raise SMPInvalidArgumentError(f"{name} must be an int32 or int64 tensor")
+    if t.device != device:
+        raise SMPInvalidArgumentError(f"{name} is on {t.device}, the table on {device}")
+
+
+def embedding(ids, weight, padding_idx=None, scale=1.0, vocab_start=None, position_ids=None, position_weight=None):
+    """``scale * weight[ids] + position_weight[position_ids]`` -> ``[*ids.shape, dim]``.
+
+    ``weight`` [rows, dim] fp32 / fp16 / bf16; ``ids`` int32 or int64 of any shape.
+    ``padding_idx``: a token id that gets no gradient (negative: counted from the table's end).
+    ``vocab_start``: the table holds the ids ``vocab_start .. vocab_start + rows - 1`` of a larger
+    vocabulary; the other ids give zeros and take no gradient.  Without it an id outside the table
+    is an error: IndexError on the CPU, a row of NaN on the GPU (nothing waits for the ids there).
+    ``position_weight`` [positions, dim]: rows added unscaled, chosen by ``position_ids``
+    (broadcast to ``ids``) or, without them, by the place in the last dimension."""
+    if not torch.is_tensor(weight) or weight.dim() != 2 or weight.dtype not in _FLOATS or 0 in weight.shape:
+        raise SMPInvalidArgumentError("weight must be a [rows, dim] fp32 / fp16 / bf16 tensor")
+    _check_ids("ids", ids, weight.device)
+    rows = weight.shape[0]
+    scale = float(scale)
+    if not math.isfinite(scale):
+        raise SMPInvalidArgumentError(f"scale must be finite, got {scale}")
+    if vocab_start is not None:
+        vocab_start = int(vocab_start)
+        if vocab_start < 0 or (padding_idx is not None and padding_idx < 0):
+            raise SMPInvalidArgumentError("vocab_start, and padding_idx beside it, must not be negative")
+    elif padding_idx is not None:
+        if not -rows <= padding_idx < rows:
+            raise SMPInvalidArgumentError(f"padding_idx {padding_idx} is not a row of a table of {rows}")
+        padding_idx = padding_idx % rows
+    if position_weight is None:
+        if position_ids is not None:
+            raise SMPInvalidArgumentError("position_ids need a position_weight")
+    else:
+        if position_weight.dim() != 2 or position_weight.shape[1] != weight.shape[1] or 0 in position_weight.shape:
+            raise SMPInvalidArgumentError("position_weight must be [positions, dim] with weight's dim")
+        if position_weight.dtype != weight.dtype or position_weight.device != weight.device:
+            raise SMPInvalidArgumentError("position_weight must have weight's dtype and device")
+        if position_ids is not None:
+            _check_ids("position_ids", position_ids, weight.device)
+            try:
+                position_ids = position_ids.expand(ids.shape)
+            except RuntimeError:
+                raise SMPInvalidArgumentError(f"position_ids {tuple(position_ids.shape)} do not broadcast to "
+                                              f"{tuple(ids.shape)}") from None
+        elif ids.dim() == 0 or ids.shape[-1] > position_weight.shape[0]:
+            raise SMPInvalidArgumentError(f"ids {tuple(ids.shape)} need position_ids: the position table has "
+                                          f"{position_weight.shape[0]} rows")
+    if fused_ok(weight):
+        return _EmbeddingHIP.apply(weight, position_weight, ids, position_ids, padding_idx, scale, vocab_start)
+    return _embedding_torch(ids, weight, padding_idx, scale, vocab_start, position_ids, position_weight)

@@ -1,0 +1,252 @@
+"""The embedding kernels against plain 64-bit arithmetic.
+
+Bounds: the forward adds two fp32 products' roundings (2^-24 of each term, twice) and one
+rounding into the output type; a gradient that is the fp32 sum of k rows is off by at most
+k * 2^-24 of the sum of their magnitudes, and rounded once.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U32 = 2.0 ** -24
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def within(got, exact, slack):
+    """|got - exact| <= slack + half a step of the result; subnormals of the type round absolutely."""
+    dt = got.dtype
+    bound = slack + half_step(dt) * (exact.abs() + slack) + torch.finfo(dt).tiny * torch.finfo(dt).eps
+    err = (got.double() - exact).abs()
+    assert bool((err <= bound).all()), f"{int((err > bound).sum())} values off, worst {float((err - bound).max())}"
+
+
+def table_grad(ids, dy, rows, scale, skip=None):
+    """(gradient, slack) in 64 bits; ids outside the table and `skip` take none."""
+    ids, dy = ids.reshape(-1), dy.double().reshape(-1, dy.shape[-1])
+    keep = (ids >= 0) & (ids < rows)
+    if skip is not None:
+        keep &= ids != skip
+    ids, dy = ids[keep], dy[keep]
+    z = torch.zeros(rows, dy.shape[-1], dtype=torch.float64, device=dy.device)
+    count = torch.bincount(ids, minlength=rows).double().unsqueeze(1)
+    total, size = z.index_add(0, ids, dy) * scale, z.index_add(0, ids, dy.abs()) * abs(scale)
+    return total, (count + 2) * U32 * size
+
+
+def forward(ids, w, scale, start, pos, p):
+    rows = w.shape[0]
+    local = ids - (start or 0)
+    out = w.double()[local.clamp(0, rows - 1)] * scale
+    if start is not None:
+        out = out * ((local >= 0) & (local < rows)).unsqueeze(-1)
+    slack = out.abs()
+    if p is not None:
+        out, slack = out + p.double()[pos], slack + p.double()[pos].abs()
+    return out, 2 * U32 * slack
+
+
+def check(b, s, rows, dim, dtype, ids=None, scale=1.0, padding=None, start=None, positions="none", idt=torch.long,
+          seed=0, strided=False):
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    vocab = rows if start is None else rows + 2 * start + 1
+    if ids is None:
+        ids = torch.randint(0, vocab, (b, s), generator=g, device="cuda")
+    ids = ids.to(idt)
+    w = torch.randn(rows, dim + 8 if strided else dim, generator=g, device="cuda").to(dtype)[:, :dim].requires_grad_()
+    p = pos = None
+    if positions != "none":
+        p = torch.randn(s + 3, dim, generator=g, device="cuda").to(dtype).requires_grad_()
+        pos = torch.arange(s, device="cuda").expand(b, s)
+        if positions == "given":
+            pos = pos + torch.randint(0, 4, (b, 1), generator=g, device="cuda")
+    y = embedding(ids, w, padding_idx=padding, scale=scale, vocab_start=start,
+                  position_ids=pos if positions == "given" else None, position_weight=p)
+    assert y.shape == (b, s, dim) and y.dtype == dtype
+    within(y, *forward(ids.long(), w.detach(), scale, start, pos, None if p is None else p.detach()))
+    dy = torch.randn(b, s, dim, generator=g, device="cuda").to(dtype)
+    grads = torch.autograd.grad(y, [w] if p is None else [w, p], dy)
+    skip = None if padding is None else padding - (start or 0)
+    within(grads[0], *table_grad(ids.long() - (start or 0), dy, rows, scale, skip))
+    if p is not None:
+        within(grads[1], *table_grad(pos, dy, s + 3, 1.0))
+    return grads
+
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,s,rows,dim", [(1, 1, 1, 1), (1, 1, 7, 64), (2, 3, 5, 1601), (3, 77, 300, 8), (5, 100, 50, 40),
+                                          (4, 600, 1000, 264), (2, 1025, 70000, 24)])
+def test_sizes(b, s, rows, dim, dtype):
+    check(b, s, rows, dim, dtype)
+
+
+@pytest.mark.parametrize("positions", ["implicit", "given"])
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 36), (torch.bfloat16, 1600), (torch.float16, 37)])
+def test_positions_and_scale(positions, dtype, dim):
+    check(3, 65, 40, dim, dtype, positions=positions, scale=dim ** 0.5, padding=3)
+
+
+@pytest.mark.parametrize("start", [0, 13])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_vocabulary_shard(start, dtype):
+    check(3, 50, 20, 72, dtype, start=start, padding=start + 2, scale=0.25, idt=torch.int32)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,dim", [(40, 64), (5000, 200), (20000, 33)])
+def test_one_token_everywhere(dtype, n, dim):
+    """The longest segment: all positions hold the same token."""
+    check(1, n, 9, dim, dtype, ids=torch.full((1, n), 4, device="cuda"))
+
+
+def test_all_padding_and_all_foreign():
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    w = torch.randn(6, 16, device="cuda", requires_grad=True)
+    ids = torch.full((2, 9), 5, device="cuda")
+    (dw,) = torch.autograd.grad(embedding(ids, w, padding_idx=-1).sum(), w)  # an expanded gradient
+    assert torch.equal(dw, torch.zeros_like(dw))
+    y = embedding(ids, w, vocab_start=6)
+    assert torch.equal(y, torch.zeros_like(y))
+    (dw,) = torch.autograd.grad(y, w, torch.full_like(y, float("nan")))
+    assert torch.equal(dw, torch.zeros_like(dw))
+
+
+def test_ids_outside_the_table_are_nan_rows():
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    w = torch.randn(6, 16, device="cuda", requires_grad=True)
+    p = torch.randn(4, 16, device="cuda")
+    ids = torch.tensor([0, 6, -1, 2 ** 40, 5], device="cuda")
+    y = embedding(ids, w)
+    assert y.isnan().all(1).tolist() == [False, True, True, True, False]
+    (dw,) = torch.autograd.grad(y, w, torch.ones_like(y))
+    assert dw[:, 0].tolist() == [1, 0, 0, 0, 0, 1]
+    y = embedding(ids.clamp(0, 5), w, position_ids=torch.tensor([0, 4, -1, 3, 2], device="cuda"), position_weight=p)
+    assert y.isnan().all(1).tolist() == [False, True, True, False, False]
+
+
+def test_infinite_gradients_stay_in_their_row():
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    w = torch.randn(8, 8, device="cuda", requires_grad=True)
+    ids = torch.tensor([1, 2, 2, 3], device="cuda")
+    dy = torch.ones(4, 8, device="cuda")
+    dy[1] = float("inf")
+    dy[3] = float("nan")
+    (dw,) = torch.autograd.grad(embedding(ids, w), w, dy)
+    assert torch.isfinite(dw[[0, 1, 4, 5, 6, 7]]).all() and dw[2].isinf().all() and dw[3].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_layouts(dtype):
+    """Strided ids, rows and gradients, and a table whose rows start off 16 bytes."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    check(4, 30, 25, 48, dtype, strided=True)
+    check(4, 30, 25, 45, dtype, strided=True)
+    ids = torch.randint(0, 25, (30, 8), device="cuda")[::2, ::2].t()
+    w = torch.randn(25 * 48 + 1, device="cuda").to(dtype)[1:].view(25, 48).requires_grad_()
+    y = embedding(ids, w)
+    within(y, *forward(ids, w.detach(), 1.0, None, None, None))
+    dy = torch.randn(48, 4, 15, device="cuda").to(dtype).permute(1, 2, 0)
+    (dw,) = torch.autograd.grad(y, w, dy)
+    within(dw, *table_grad(ids, dy, 25, 1.0))
+    wt = torch.randn(48, 25, device="cuda").to(dtype).t().requires_grad_()  # columns dense instead of rows
+    y = embedding(ids, wt)
+    within(y, *forward(ids, wt.detach(), 1.0, None, None, None))
+    (dw,) = torch.autograd.grad(y, wt, dy)
+    within(dw, *table_grad(ids, dy, 25, 1.0))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [50, 3000, 40000])
+def test_bound_gradient_accumulates_in_place(dtype, n):
+    """A parameter bound to the flat gradient buffer: touched rows grow, the others keep their bits."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = torch.nn.Parameter(torch.randn(700, 40, generator=g, device="cuda").to(dtype))
+    p = torch.nn.Parameter(torch.randn(64, 40, generator=g, device="cuda").to(dtype))
+    n = n // 50 * 50
+    ids = torch.randint(0, 300, (n // 50, 50), generator=g, device="cuda")
+    before = {}
+    for t in (w, p):
+        t.grad = torch.randn(t.shape, generator=g, device="cuda").to(dtype)
+        t._smp_fused_grad = True
+        before[t] = t.grad.clone()
+    hooks = []
+    w.register_post_accumulate_grad_hook(lambda t: hooks.append(t))
+    dy = torch.randn(n // 50, 50, 40, generator=g, device="cuda").to(dtype)
+    embedding(ids, w, position_weight=p, scale=2.0).backward(dy)
+    assert len(hooks) == 1 and hooks[0] is w
+    for t, at, scale in ((w, ids, 2.0), (p, torch.arange(50, device="cuda").expand(n // 50, 50), 1.0)):
+        total, slack = table_grad(at, dy, t.shape[0], scale)
+        seen = torch.bincount(at.reshape(-1), minlength=t.shape[0]) > 0
+        within(t.grad[seen], (total + before[t].double())[seen], (slack + 2 * U32 * before[t].double().abs())[seen])
+        assert torch.equal(t.grad[~seen], before[t][~seen])
+
+
+def test_same_bits_on_every_run_and_stream():
+    g1 = check(8, 1000, 500, 200, torch.float32, seed=5)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        g2 = check(8, 1000, 500, 200, torch.float32, seed=5)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(g1[0], g2[0])
+
+
+def test_offsets_past_32_bits():
+    """A table and an output of more than 2^31 elements."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    rows, dim = 600_000, 4096
+    w = torch.zeros(rows, dim, device="cuda", dtype=torch.bfloat16)
+    w[-1], w[300_000] = 2.0, 3.0
+    ids = torch.zeros(550_000, device="cuda", dtype=torch.long)
+    ids[-1], ids[-2] = rows - 1, 300_000
+    w.requires_grad_()
+    y = embedding(ids, w)
+    assert y[-1].eq(2).all() and y[-2].eq(3).all() and y[-3].eq(0).all()
+    dy = torch.zeros_like(y)
+    dy[-1], dy[-2] = 1.0, 4.0
+    (dw,) = torch.autograd.grad(y, w, dy)
+    assert dw[-1].eq(1).all() and dw[300_000].eq(4).all() and float(dw.sum(dtype=torch.float64)) == 5 * dim
+
+
+def test_graph_replays():
+    """Forward and backward captured: every replay on new ids gives what the eager call gives."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    w = torch.randn(900, 64, device="cuda").requires_grad_()
+    p = torch.randn(130, 64, device="cuda").requires_grad_()
+    ids = torch.randint(0, 900, (50, 128), device="cuda")
+    dy = torch.randn(50, 128, 64, device="cuda")
+
+    def step():
+        y = embedding(ids, w, position_weight=p, scale=0.5, padding_idx=7)
+        return [y.detach(), *torch.autograd.grad(y, [w, p], dy)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(3):
+        ids.copy_(torch.randint(0, 900 >> (4 * k), (50, 128), device="cuda"))
+        dy.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, e in zip(out, step()):
+            assert torch.equal(a, e)
