@@ -250,4 +250,28 @@ int embedding_fwd(int dt, const IndexList& ids, const void* w, int64_t w_stride,
 int embedding_bwd(int dt, const IndexList& ids, const void* dy, int64_t n, int64_t d, float scale, int64_t skip,
                   void* dw, int accumulate, hipStream_t s);
 
+// ------------------------------------------------------------------ gradient norm (grad_norm.hip)
+// Up to kGradList tensors, each cut into chunks of one size: chunk b of a launch lies in tensor t
+// with first[t] <= b < first[t + 1]; its partial is number first_chunk + b.  Passed by value: the
+// kernel arguments hold at most 4096 bytes.
+constexpr int kGradList = 120;
+struct GradList {
+  const void* p[kGradList];
+  void* o[kGradList];
+  int64_t n[kGradList];
+  uint32_t first[kGradList + 1];
+  uint8_t dt[kGradList], odt[kGradList];
+  int count;
+  int64_t first_chunk;
+};
+int64_t grad_chunk_size(int64_t total);
+// part[chunk] = sum of squares (inf: largest |x|) of each chunk
+int grad_partials(const GradList& l, int64_t size, int inf, double* part, hipStream_t s);
+// power = scale^2 * sum (inf: scale * max) of n partials, norm = its root (inf: itself), factor (may be
+// null) = scale * min(1, max_norm / (norm + 1e-6))
+int grad_join(const double* part, int64_t n, int inf, double scale, double max_norm, double* power, float* norm,
+              float* factor, hipStream_t s);
+// o = p * factor
+int grad_scale(const GradList& l, int64_t size, const float* factor, hipStream_t s);
+
 }  // namespace smpk

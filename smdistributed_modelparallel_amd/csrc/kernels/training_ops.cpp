@@ -5,6 +5,9 @@
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
 
+#include <algorithm>
+#include <vector>
+
 #include "kernels.h"
 
 namespace {
@@ -86,9 +89,106 @@ void embedding_bwd(at::Tensor dy, c10::optional<at::Tensor> ids, int64_t period,
         "embedding_bwd");
 }
 
+// --------------------------------------------------------------- gradient norm
+// [start, end) of the memory of a dense tensor
+std::pair<uintptr_t, uintptr_t> extent(const at::Tensor& t) {
+  const auto p = reinterpret_cast<uintptr_t>(t.data_ptr());
+  return {p, p + static_cast<uintptr_t>(t.nbytes())};
+}
+
+// No element may be written twice, or written while another tensor's turn reads it.
+void check_disjoint(const std::vector<at::Tensor>& in, const std::vector<at::Tensor>& out) {
+  struct Range {
+    uintptr_t s, e;
+    bool write;
+  };
+  std::vector<Range> r;
+  r.reserve(in.size() * 2);
+  for (size_t i = 0; i < in.size(); ++i) {
+    if (in[i].numel() == 0) continue;
+    const auto a = extent(in[i]), b = extent(out[i]);
+    r.push_back({b.first, b.second, true});
+    if (a != b) r.push_back({a.first, a.second, false});
+  }
+  std::sort(r.begin(), r.end(), [](const Range& x, const Range& y) { return x.s < y.s; });
+  uintptr_t end = 0, write_end = 0;
+  for (const Range& x : r) {
+    TORCH_CHECK_VALUE(x.s >= write_end && (!x.write || x.s >= end),
+                      "clip_grad_norm_: two tensors of the list share memory");
+    end = std::max(end, x.e);
+    if (x.write) write_end = std::max(write_end, x.e);
+  }
+}
+
+// {power fp64 [1], norm fp32 []}; with `out`, also out[i] = grads[i] * scale * min(1, max_norm / (norm + 1e-6))
+std::vector<at::Tensor> grad_norm(std::vector<at::Tensor> grads, bool inf, double scale,
+                                  c10::optional<std::vector<at::Tensor>> out, double max_norm) {
+  TORCH_CHECK(!grads.empty(), "grad_norm: no tensors");
+  const c10::DeviceGuard guard(grads[0].device());
+  int64_t total = 0;
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const at::Tensor& t = grads[i];
+    TORCH_CHECK(t.is_cuda() && t.device() == grads[0].device() && t.is_non_overlapping_and_dense(),
+                "grad_norm: dense tensors of one GPU expected");
+    dt_code(t, "grad_norm");
+    total += t.numel();
+  }
+  if (out.has_value()) {
+    TORCH_CHECK(out->size() == grads.size(), "grad_norm: lists of different lengths");
+    for (size_t i = 0; i < grads.size(); ++i) {
+      const at::Tensor& o = (*out)[i];
+      TORCH_CHECK(o.device() == grads[0].device() && o.sizes() == grads[i].sizes() &&
+                      (o.numel() == 0 || o.strides() == grads[i].strides()),
+                  "grad_norm: out differs from its gradient");
+      dt_code(o, "grad_norm");
+    }
+    check_disjoint(grads, *out);
+  }
+  const int64_t size = smpk::grad_chunk_size(total);
+  std::vector<smpk::GradList> lists(1);
+  lists[0].count = 0;
+  lists[0].first[0] = 0;
+  lists[0].first_chunk = 0;
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const int64_t n = grads[i].numel();
+    if (n == 0) continue;
+    if (lists.back().count == smpk::kGradList) {
+      const int64_t next = lists.back().first_chunk + lists.back().first[lists.back().count];
+      lists.emplace_back();
+      lists.back().count = 0;
+      lists.back().first[0] = 0;
+      lists.back().first_chunk = next;
+    }
+    smpk::GradList& l = lists.back();
+    const int k = l.count++;
+    l.p[k] = grads[i].data_ptr();
+    l.o[k] = out.has_value() ? (*out)[i].data_ptr() : nullptr;
+    l.n[k] = n;
+    l.dt[k] = static_cast<uint8_t>(dt_code(grads[i], "grad_norm"));
+    l.odt[k] = out.has_value() ? static_cast<uint8_t>(dt_code((*out)[i], "grad_norm")) : 0;
+    l.first[k + 1] = l.first[k] + static_cast<uint32_t>((n + size - 1) / size);
+  }
+  const int64_t chunks = lists.back().first_chunk + lists.back().first[lists.back().count];
+  const auto opts = grads[0].options();
+  auto part = at::empty({chunks < 1 ? 1 : chunks}, opts.dtype(at::kDouble));
+  auto power = at::empty({1}, opts.dtype(at::kDouble));
+  auto norm = at::empty({}, opts.dtype(at::kFloat));
+  auto factor = at::empty({1}, opts.dtype(at::kFloat));
+  for (const auto& l : lists)
+    check(smpk::grad_partials(l, size, inf ? 1 : 0, part.data_ptr<double>(), stream()), "grad_partials");
+  check(smpk::grad_join(part.data_ptr<double>(), chunks, inf ? 1 : 0, scale, max_norm, power.data_ptr<double>(),
+                        norm.data_ptr<float>(), out.has_value() ? factor.data_ptr<float>() : nullptr, stream()),
+        "grad_join");
+  if (out.has_value())
+    for (const auto& l : lists) check(smpk::grad_scale(l, size, factor.data_ptr<float>(), stream()), "grad_scale");
+  return {power, norm};
+}
+
 }  // namespace
 
 void register_training_ops(py::module_& m) {
+  m.def("grad_norm", &grad_norm, py::arg("grads"), py::arg("inf"), py::arg("scale"), py::arg("out") = py::none(),
+        py::arg("max_norm") = 0.0);
   m.def("embedding_fwd", &embedding_fwd, py::arg("ids"), py::arg("weight"), py::arg("scale"), py::arg("start"),
         py::arg("foreign_zero"), py::arg("pos"), py::arg("pos_weight"), py::arg("period"));
   m.def("embedding_bwd", &embedding_bwd, py::arg("dy"), py::arg("ids"), py::arg("period"), py::arg("scale"),

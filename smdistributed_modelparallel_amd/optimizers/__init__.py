@@ -273,4 +273,13 @@ class FusedNovoGrad(torch.optim.Optimizer):
         return loss
 
 
-__all__ = ["DistributedOptimizer", "FusedAdam", "FusedLAMB", "FusedNovoGrad"]
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
+    """``torch.nn.utils.clip_grad_norm_`` for the standalone optimizers above: one norm over the
+    ``.grad`` of all parameters (any mix of fp32 / fp16 / bf16), clipped in place, returned as a
+    fp32 scalar tensor without a host synchronisation (`ops/multi_tensor.py`).  It sees this
+    rank's gradients only: under ``smp.DistributedOptimizer`` use ``clip_master_grads``."""
+    parameters = [parameters] if torch.is_tensor(parameters) else list(parameters)
+    return mt.clip_grad_norm_([p.grad for p in parameters if p.grad is not None], max_norm, norm_type)
+
+
+__all__ = ["DistributedOptimizer", "FusedAdam", "FusedLAMB", "FusedNovoGrad", "clip_grad_norm_"]

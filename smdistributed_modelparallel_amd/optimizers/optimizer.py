@@ -301,29 +301,28 @@ class DistributedOptimizer(torch.optim.Optimizer):
                 fill()
 
     def clip_master_grads(self, max_norm, norm_type=2):
-        """Global L2 norm of the (unscaled) gradients across all ranks holding distinct
-        gradients; records the clip coefficient applied inside the next step."""
-        if norm_type != 2:
-            raise SMPInvalidArgumentError("only L2 norm clipping is supported")
+        """Global L2 (``norm_type=inf``: largest-value) norm of the (unscaled) gradients across all
+        ranks holding distinct gradients; records the clip coefficient applied inside the next step."""
+        if norm_type not in (2, float("inf")):
+            raise SMPInvalidArgumentError("only L2 and inf norm clipping is supported")
         self._materialize_grads()
         dev = state.device
-        acc = torch.zeros(1, dtype=torch.float32, device=dev)
         core = state.core
-        inv = 1.0 / self.loss_scale
-        for d in self.domains:
-            # replicated (non-TP) params are identical on every tp_rank: count them once
-            if d.key == "default" and core.tp_size() > 1 and core.tp_rank() != 0 and not state.cfg.shard_optimizer_state:
-                continue
-            mt.sumsq(self._grad_range(d), acc, scale=inv)
+        # replicated (non-TP) params are identical on every tp_rank: count them once
+        once = core.tp_size() > 1 and core.tp_rank() != 0 and not state.cfg.shard_optimizer_state
+        ranges = [self._grad_range(d) for d in self.domains if not (once and d.key == "default")]
+        # fp64 over the ranks too: no finite gradient overflows the sum of squares
+        acc = mt.grad_power(ranges, norm_type, scale=1.0 / self.loss_scale).to(dev)
+        op = dist.ReduceOp.SUM if norm_type == 2 else dist.ReduceOp.MAX
         if state.sdp is not None:
             # every replica holds identical reduced shards: the norm spans one shard group
             if state.pgs.shard is not None:
-                dist.all_reduce(acc, group=state.pgs.shard)
+                dist.all_reduce(acc, op=op, group=state.pgs.shard)
         elif state.cfg.shard_optimizer_state and core.dp_size() > 1:
-            dist.all_reduce(acc, group=state.pgs.world)
+            dist.all_reduce(acc, op=op, group=state.pgs.world)
         elif core.mp_size() > 1:
-            dist.all_reduce(acc, group=state.pgs.mp)
-        norm = acc.sqrt()
+            dist.all_reduce(acc, op=op, group=state.pgs.mp)
+        norm = (acc.sqrt() if norm_type == 2 else acc).float()
         coef = torch.clamp(max_norm / (norm + 1e-6), max=1.0)
         self._clip_coef = coef
         return norm
