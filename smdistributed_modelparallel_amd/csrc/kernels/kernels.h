@@ -274,4 +274,42 @@ int grad_join(const double* part, int64_t n, int inf, double scale, double max_n
 // o = p * factor
 int grad_scale(const GradList& l, int64_t size, const float* factor, hipStream_t s);
 
+// ------------------------------------------------------------------ block norm (block_norm.hip)
+// Rows [rows, d] dense; w, b, pw, pb [d] of the rows' type or all fp32 (w_f32); gate [rows / gate_rows,
+// d], of the rows' type or fp32 (gate_f32).  x null: s = residual, y = N1(residual) alone.
+struct BlockNormArgs {
+  const void *x = nullptr, *res = nullptr, *w = nullptr, *b = nullptr, *pw = nullptr, *pb = nullptr, *gate = nullptr;
+  int w_f32 = 0, gate_f32 = 0, rms = 0;
+  int64_t rows = 0, gate_rows = 1;
+  int d = 0;
+  float alpha = 1.f, eps = 0.f;
+  float* stats = nullptr;  // [rows][4]: mean, 1 / deviation of s, then of x
+  void *y = nullptr, *s = nullptr;
+  // backward
+  const void *dy = nullptr, *ds = nullptr;  // either may be null: no gradient
+  void *dx = nullptr, *dres = nullptr, *dgate = nullptr;
+  int64_t split = 1;
+  int gate_direct = 0;          // a unit has whole gate rows: it writes dgate itself
+  float* gate_part = nullptr;   // else [units][d]
+  float* part[5] = {};          // [blocks][d] of dw1, db1, dw2, db2, dgate (one gate row for all)
+};
+struct BlockNormPlan {
+  int team, threads, lds;
+  int64_t blocks, units, split, iterations;
+};
+// out[g] = or += the sum of the partial rows g * split .. (g + 1) * split - 1
+struct BlockNormJoin {
+  struct Item {
+    const float* part;
+    void* out;
+    int64_t split, groups;
+    int dt, accumulate;
+  } item[6];
+  int count = 0;
+};
+int block_norm_fwd(int dt, const BlockNormArgs& a, hipStream_t s);
+int block_norm_bwd_plan(int64_t rows, int64_t d, int64_t gate_rows, BlockNormPlan& p);
+int block_norm_bwd(int dt, const BlockNormArgs& a, const BlockNormPlan& p, hipStream_t s);
+int block_norm_join(const BlockNormJoin& l, int d, hipStream_t s);
+
 }  // namespace smpk

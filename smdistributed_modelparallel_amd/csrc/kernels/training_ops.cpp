@@ -89,6 +89,156 @@ void embedding_bwd(at::Tensor dy, c10::optional<at::Tensor> ids, int64_t period,
         "embedding_bwd");
 }
 
+// ------------------------------------------------------------------ block norm
+typedef c10::optional<at::Tensor> Opt;
+
+const void* ptr(const Opt& t) { return t.has_value() ? t->data_ptr() : nullptr; }
+
+// Arguments that the forward and the backward share, checked.
+smpk::BlockNormArgs block_args(const Opt& x, const at::Tensor& res, const at::Tensor& w, const Opt& b, const Opt& pw,
+                               const Opt& pb, const Opt& gate, int64_t gate_rows, double alpha, double eps, bool rms) {
+  TORCH_CHECK(res.is_cuda() && res.dim() == 2 && res.is_contiguous(), "block_norm: rows must be a dense matrix");
+  const int64_t d = res.size(1);
+  TORCH_CHECK(d >= 1 && d <= 16384, "block_norm: width ", d, " is not within 1 .. 16384");
+  dt_code(res, "block_norm");
+  auto like = [&](const Opt& t) {
+    return !t.has_value() || (t->device() == res.device() && t->is_contiguous() && t->sizes() == res.sizes() &&
+                              t->scalar_type() == res.scalar_type());
+  };
+  TORCH_CHECK(like(x), "block_norm: x differs from the residual");
+  auto vec = [&](const Opt& t) {
+    return !t.has_value() || (t->device() == res.device() && t->is_contiguous() && t->numel() == d &&
+                              t->scalar_type() == w.scalar_type());
+  };
+  TORCH_CHECK(w.scalar_type() == res.scalar_type() || w.scalar_type() == at::kFloat, "block_norm: weight dtype");
+  TORCH_CHECK(vec(w) && vec(b) && vec(pw) && vec(pb), "block_norm: weights and biases must be alike");
+  if (gate.has_value()) {
+    TORCH_CHECK(gate->device() == res.device() && gate->is_contiguous() && gate_rows >= 1 &&
+                    gate->numel() == (res.size(0) + gate_rows - 1) / gate_rows * d && res.size(0) % gate_rows == 0 &&
+                    (gate->scalar_type() == res.scalar_type() || gate->scalar_type() == at::kFloat),
+                "block_norm: bad gate");
+  }
+  smpk::BlockNormArgs a;
+  a.x = ptr(x);
+  a.res = res.data_ptr();
+  a.w = w.data_ptr();
+  a.b = ptr(b);
+  a.pw = ptr(pw);
+  a.pb = ptr(pb);
+  a.gate = ptr(gate);
+  a.w_f32 = w.scalar_type() == at::kFloat;
+  a.gate_f32 = gate.has_value() && gate->scalar_type() == at::kFloat;
+  a.rms = rms;
+  a.rows = res.size(0);
+  a.gate_rows = gate.has_value() ? gate_rows : (a.rows < 1 ? 1 : a.rows);
+  a.d = static_cast<int>(d);
+  a.alpha = static_cast<float>(alpha);
+  a.eps = static_cast<float>(eps);
+  return a;
+}
+
+// {y, s, stats}; s is empty without x, stats without need_stats
+std::vector<at::Tensor> block_norm_fwd(Opt x, at::Tensor res, at::Tensor w, Opt b, Opt pw, Opt pb, Opt gate,
+                                       int64_t gate_rows, double alpha, double eps, bool rms, bool need_stats) {
+  const c10::DeviceGuard guard(res.device());
+  auto a = block_args(x, res, w, b, pw, pb, gate, gate_rows, alpha, eps, rms);
+  auto y = at::empty_like(res);
+  auto s = x.has_value() ? at::empty_like(res) : at::empty({0}, res.options());
+  auto stats = at::empty({need_stats ? a.rows : 0, 4}, res.options().dtype(at::kFloat));
+  a.y = y.data_ptr();
+  a.s = x.has_value() ? s.data_ptr() : nullptr;
+  a.stats = need_stats ? stats.data_ptr<float>() : nullptr;
+  check(smpk::block_norm_fwd(dt_code(res, "block_norm"), a, stream()), "block_norm_fwd");
+  return {y, s, stats};
+}
+
+// Gradients of x, residual, w, b, pw, pb, gate: those of `need` (undefined otherwise).  into[i]: the
+// bound gradient of w, b, pw, pb, gate, added to in place (and returned undefined).
+std::vector<Opt> block_norm_bwd(Opt dy, Opt ds, Opt x, at::Tensor res, at::Tensor w, Opt b, Opt pw, Opt pb, Opt gate,
+                                int64_t gate_rows, double alpha, double eps, bool rms, at::Tensor stats,
+                                std::vector<bool> need, std::vector<Opt> into) {
+  const c10::DeviceGuard guard(res.device());
+  auto a = block_args(x, res, w, b, pw, pb, gate, gate_rows, alpha, eps, rms);
+  TORCH_CHECK(need.size() == 7 && into.size() == 5, "block_norm: bad lists");
+  TORCH_CHECK(stats.is_contiguous() && stats.scalar_type() == at::kFloat && stats.numel() == 4 * a.rows,
+              "block_norm: bad statistics");
+  for (const Opt* t : {&dy, &ds})
+    TORCH_CHECK(!t->has_value() || ((*t)->is_contiguous() && (*t)->sizes() == res.sizes() &&
+                                    (*t)->scalar_type() == res.scalar_type() && (*t)->device() == res.device()),
+                "block_norm: bad gradient");
+  const Opt vectors[5] = {Opt(w), b, pw, pb, gate};
+  std::vector<Opt> out(7);
+  at::Tensor target[5];
+  for (int i = 0; i < 5; ++i) {
+    if (!need[2 + i]) continue;
+    TORCH_CHECK(vectors[i].has_value(), "block_norm: gradient of an absent vector");
+    if (into[i].has_value()) {
+      TORCH_CHECK(into[i]->is_contiguous() && into[i]->numel() == vectors[i]->numel() &&
+                      into[i]->scalar_type() == vectors[i]->scalar_type() && into[i]->device() == res.device(),
+                  "block_norm: bad bound gradient");
+      target[i] = *into[i];
+    } else {
+      target[i] = a.rows > 0 ? at::empty_like(*vectors[i]) : at::zeros_like(*vectors[i]);
+      out[2 + i] = target[i];
+    }
+  }
+  at::Tensor dx, dres;
+  if (need[0]) {
+    TORCH_CHECK(x.has_value(), "block_norm: gradient of an absent x");
+    out[0] = dx = at::empty_like(res);
+    a.dx = dx.data_ptr();
+  }
+  if (need[1]) {
+    out[1] = dres = at::empty_like(res);
+    a.dres = dres.data_ptr();
+  }
+  if (a.rows == 0) return out;  // (bound gradients stay as they are)
+  a.dy = ptr(dy);
+  a.ds = ptr(ds);
+  a.stats = stats.data_ptr<float>();
+  smpk::BlockNormPlan p;
+  check(smpk::block_norm_bwd_plan(a.rows, a.d, a.gate_rows, p), "block_norm_bwd_plan");
+  a.split = p.split;
+  const auto f32 = res.options().dtype(at::kFloat);
+  const int64_t groups = a.rows / a.gate_rows;
+  const bool gate_rows_own = need[6] && groups > 1;  // one sum for each gate row, not one for all rows
+  at::Tensor parts, gate_part;
+  int sums = 0;
+  for (int i = 0; i < 5; ++i) sums += target[i].defined() && !(i == 4 && gate_rows_own);
+  if (sums) parts = at::empty({sums, p.blocks, a.d}, f32);
+  smpk::BlockNormJoin join;
+  int used = 0;
+  for (int i = 0; i < 5; ++i) {
+    if (!target[i].defined()) continue;
+    auto& it = join.item[join.count];
+    it.dt = dt_code(target[i], "block_norm");
+    it.out = target[i].data_ptr();
+    it.accumulate = into[i].has_value();
+    if (i == 4 && gate_rows_own) {
+      if (p.split == 1 && !it.accumulate) {  // written by the units
+        a.gate_direct = 1;
+        a.dgate = it.out;
+        continue;
+      }
+      TORCH_CHECK(p.split > 1, "block_norm: a bound gradient of a gate with many rows");
+      gate_part = at::empty({p.units, a.d}, f32);
+      a.gate_part = gate_part.data_ptr<float>();
+      it.part = a.gate_part;
+      it.split = p.split;
+      it.groups = groups;
+    } else {
+      a.part[i] = parts.data_ptr<float>() + used++ * p.blocks * a.d;
+      it.part = a.part[i];
+      it.split = p.blocks;
+      it.groups = 1;
+    }
+    ++join.count;
+  }
+  check(smpk::block_norm_bwd(dt_code(res, "block_norm"), a, p, stream()), "block_norm_bwd");
+  check(smpk::block_norm_join(join, a.d, stream()), "block_norm_join");
+  return out;
+}
+
 // --------------------------------------------------------------- gradient norm
 // [start, end) of the memory of a dense tensor
 std::pair<uintptr_t, uintptr_t> extent(const at::Tensor& t) {
@@ -187,6 +337,12 @@ std::vector<at::Tensor> grad_norm(std::vector<at::Tensor> grads, bool inf, doubl
 }  // namespace
 
 void register_training_ops(py::module_& m) {
+  m.def("block_norm_fwd", &block_norm_fwd, py::arg("x"), py::arg("res"), py::arg("w"), py::arg("b"), py::arg("pw"),
+        py::arg("pb"), py::arg("gate"), py::arg("gate_rows"), py::arg("alpha"), py::arg("eps"), py::arg("rms"),
+        py::arg("need_stats"));
+  m.def("block_norm_bwd", &block_norm_bwd, py::arg("dy"), py::arg("ds"), py::arg("x"), py::arg("res"), py::arg("w"),
+        py::arg("b"), py::arg("pw"), py::arg("pb"), py::arg("gate"), py::arg("gate_rows"), py::arg("alpha"),
+        py::arg("eps"), py::arg("rms"), py::arg("stats"), py::arg("need"), py::arg("into"));
   m.def("grad_norm", &grad_norm, py::arg("grads"), py::arg("inf"), py::arg("scale"), py::arg("out") = py::none(),
         py::arg("max_norm") = 0.0);
   m.def("embedding_fwd", &embedding_fwd, py::arg("ids"), py::arg("weight"), py::arg("scale"), py::arg("start"),

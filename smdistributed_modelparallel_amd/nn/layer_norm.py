@@ -2,6 +2,8 @@
 
 * ``FusedLayerNorm`` / ``MixedFusedLayerNorm``: the HIP fused LayerNorm (apex replacement,
   reference `smp/torch/nn/layer_norm.py:140-152`).
+* ``FusedBlockNorm``: the norm after a block, its gate and residual scale, and the norm before the
+  next block in one kernel (ops/layernorm.py ``block_norm``).
 * ``DistributedLayerNorm``: LayerNorm over a hidden dimension sharded across the TP group
   (``optimize="memory"`` layout; reference `layer_norm.py:24-135`): forward all-reduces the
   per-row mean and variance (fp32), backward all-reduces the two per-row partial sums.
@@ -11,7 +13,7 @@ import numbers
 import torch
 import torch.nn as nn
 
-from ..ops.layernorm import add_layer_norm, layer_norm, layer_norm_passthrough
+from ..ops.layernorm import add_layer_norm, block_norm, layer_norm, layer_norm_passthrough
 from ..parallel.throttle import throttler
 from .utils import get_local_channels, get_start_pos_for_slicing, tp_group, tp_size
 from ..parallel import oneshot
@@ -75,6 +77,41 @@ class MixedFusedLayerNorm(FusedLayerNorm):
         from ..ops.layernorm import mixed_layer_norm
 
         return mixed_layer_norm(x, self.weight, self.bias, self.eps)
+
+
+class FusedBlockNorm(nn.Module):
+    """``forward(x, residual) -> (norm(s), s)`` with ``s = residual + residual_scale * gate *
+    post_norm(x)``: stands between a block (output ``x``, input taken from ``residual``) and the
+    next one.  ``rms``: root-mean-square norms without biases; ``post_norm`` False: no norm after
+    the block; ``gate``: the initial value of a learned per-channel gate (None: none), over which
+    ``forward``'s own ``gate`` -- for each sample or element -- takes precedence."""
+
+    def __init__(self, hidden_size, eps=1e-5, rms=False, post_norm=True, gate=None, residual_scale=1.0, device=None,
+                 dtype=None):
+        super().__init__()
+        self.eps, self.rms, self.residual_scale = eps, rms, residual_scale
+        kw = dict(device=device, dtype=dtype)
+        self.gate_init = gate
+        self.weight = nn.Parameter(torch.empty(hidden_size, **kw))
+        for name, present in (("bias", not rms), ("post_weight", post_norm), ("post_bias", post_norm and not rms),
+                              ("gate", gate is not None)):
+            self.register_parameter(name, nn.Parameter(torch.empty(hidden_size, **kw)) if present else None)
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        with torch.no_grad():
+            for p, v in ((self.weight, 1.0), (self.bias, 0.0), (self.post_weight, 1.0), (self.post_bias, 0.0),
+                         (self.gate, self.gate_init)):
+                if p is not None:
+                    p.fill_(v)
+
+    def forward(self, x, residual, gate=None):
+        return block_norm(x, residual, self.weight, self.bias, self.post_weight, self.post_bias,
+                          self.gate if gate is None else gate, self.residual_scale, self.eps, self.rms)
+
+    def extra_repr(self):
+        return (f"{self.weight.numel()}, eps={self.eps}, rms={self.rms}, post_norm={self.post_weight is not None}, "
+                f"residual_scale={self.residual_scale}")
 
 
 class _DistLNStats(torch.autograd.Function):

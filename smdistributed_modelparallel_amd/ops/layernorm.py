@@ -5,8 +5,12 @@ Replaces apex ``fused_layer_norm_cuda`` (K9-K11, reference
 semantics (fp32 input, low-precision affine) are covered by the kernel's independent
 input / weight dtypes.
 """
-import torch
+import math
 
+import torch
+from torch.autograd.function import once_differentiable
+
+from ..backend.exceptions import SMPInvalidArgumentError
 from ._ext import ext, fused_ok
 from .dropout import dropout_seed_offset
 from .linear import _fusable
@@ -168,3 +172,145 @@ def add_layer_norm(x, residual, weight, bias, eps=1e-5, dropout_p=0.0, drawn=Non
         x = torch.nn.functional.dropout(x, dropout_p, True)
     s = x + residual
     return torch.nn.functional.layer_norm(s, (s.shape[-1],), weight, bias, eps), s
+
+
+# ------------------------------------------------- the norms before and after a block, fused
+MAX_BLOCK_NORM_WIDTH = 16384
+
+
+class _BlockNorm(torch.autograd.Function):
+    """(y, s) of ``block_norm`` on [rows, d] matrices; ``x`` None: y alone, the norm of residual."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, post_weight, post_bias, gate, gate_rows, alpha, eps, rms):
+        need = any(ctx.needs_input_grad)
+        y, s, stats = ext().block_norm_fwd(x, residual, weight, bias, post_weight, post_bias, gate, gate_rows, alpha,
+                                           eps, rms, need)
+        if need:
+            # s is not kept: the backward forms it again from x and the residual (block_norm.hip)
+            ctx.save_for_backward(x, residual, weight, bias, post_weight, post_bias, gate, stats)
+            ctx.args = (gate_rows, alpha, eps, rms)
+            ctx.set_materialize_grads(False)
+        return (y, s) if x is not None else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, ds=None):
+        *inputs, stats = ctx.saved_tensors
+        need = list(ctx.needs_input_grad[:7])
+        none = (None,) * 11
+        if dy is None and ds is None:
+            return none
+        into, bound = [], set()
+        for t, n in zip(inputs[2:], need[2:]):
+            # in place into the flat gradient buffer; a parameter used twice only once so
+            bind = n and t is not None and t.is_leaf and _fusable(t) and id(t) not in bound
+            # (the gradient of a gate with many rows may be written without a partial sum)
+            bind = bind and not (t is inputs[6] and t.numel() != t.shape[-1])
+            into.append(t.grad if bind else None)
+            if bind:
+                bound.add(id(t))
+        dy, ds = (t.contiguous() if t is not None else None for t in (dy, ds))
+        return (*ext().block_norm_bwd(dy, ds, *inputs, *ctx.args, stats, need, into), None, None, None, None)
+
+
+def _gate_matrix(gate, shape):
+    """The gate as [groups, d] where each row serves a run of consecutive rows of the input, and
+    the length of that run.  Gates that broadcast otherwise are expanded, in fp32: autograd sums
+    their gradient back, and its terms must not be rounded before they are added."""
+    d = shape[-1]
+    if gate.shape == (d,):
+        return gate, math.prod(shape[:-1])
+    if gate.shape[-1:] != (d,):
+        gate = gate.float().expand(*gate.shape[:-1], d)
+    lead = (1,) * (len(shape) - gate.dim()) + tuple(gate.shape[:-1])
+    k = 0  # the leading dimensions in which the gate has its own rows; in all others it has one
+    while k < len(lead) and lead[k] == shape[k]:
+        k += 1
+    if any(n != 1 for n in lead[k:]):
+        gate, k = gate.float().expand(*shape), len(shape) - 1
+    groups = math.prod(shape[:k])
+    return gate.reshape(groups, d), math.prod(shape[:-1]) // max(groups, 1)
+
+
+def _norm_torch(v, weight, bias, eps, rms):
+    if not rms:
+        v = v - v.mean(-1, keepdim=True)
+    v = v * torch.rsqrt((v * v).mean(-1, keepdim=True) + eps) * weight.float()
+    return v if bias is None else v + bias.float()
+
+
+def _check_norm(name, rows, weight, bias, dtype):
+    if not torch.is_tensor(weight) or weight.shape != rows.shape[-1:] or weight.device != rows.device:
+        raise SMPInvalidArgumentError(f"{name} must be a [{rows.shape[-1]}] tensor on {rows.device}")
+    if weight.dtype not in (rows.dtype, torch.float32) or weight.dtype != dtype:
+        raise SMPInvalidArgumentError("weights and biases must all have the input's dtype, or all be fp32")
+    if bias is not None and (bias.shape != weight.shape or bias.dtype != weight.dtype or bias.device != weight.device):
+        raise SMPInvalidArgumentError(f"the bias beside {name} must have its shape, dtype and device")
+
+
+def _check_rows(t, name):
+    if not torch.is_tensor(t) or t.dim() == 0 or t.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise SMPInvalidArgumentError(f"{name} must be a fp32 / fp16 / bf16 tensor [..., dim]")
+    if not 1 <= t.shape[-1] <= MAX_BLOCK_NORM_WIDTH:
+        raise SMPInvalidArgumentError(f"{name}: widths of 1 to {MAX_BLOCK_NORM_WIDTH} are supported, got {t.shape[-1]}")
+
+
+def block_norm(x, residual, weight, bias=None, post_weight=None, post_bias=None, gate=None, residual_scale=1.0,
+               eps=1e-5, rms=False):
+    """The norms after one block and before the next, with the gated residual add between them:
+
+        h = norm(x; post_weight, post_bias)        (h = x without post_weight)
+        s = residual + residual_scale * gate * h
+        y = norm(s; weight, bias)
+
+    -> ``(y, s)``, in one kernel each way.  ``norm`` is LayerNorm or, with ``rms``, the
+    root-mean-square norm.  ``x`` and ``residual`` [..., dim] are alike; the weights and biases
+    [dim] have their dtype or are fp32.  ``gate`` (that dtype or fp32) broadcasts to ``x``: one
+    vector, one for each sample ([batch, 1, dim]), or one value for each element; None is 1.
+    All arithmetic is fp32, and the second norm is taken of ``s`` before it is rounded."""
+    _check_rows(x, "x")
+    if not torch.is_tensor(residual) or residual.shape != x.shape or residual.dtype != x.dtype \
+            or residual.device != x.device:
+        raise SMPInvalidArgumentError("residual must have x's shape, dtype and device")
+    _check_norm("weight", x, weight, bias, weight.dtype if torch.is_tensor(weight) else None)
+    if post_weight is not None:
+        _check_norm("post_weight", x, post_weight, post_bias, weight.dtype)
+    elif post_bias is not None:
+        raise SMPInvalidArgumentError("post_bias needs a post_weight")
+    residual_scale, eps = float(residual_scale), float(eps)
+    if not math.isfinite(residual_scale) or not (math.isfinite(eps) and eps >= 0.0):
+        raise SMPInvalidArgumentError(f"bad residual_scale {residual_scale} or eps {eps}")
+    if gate is not None:
+        if not torch.is_tensor(gate) or gate.dtype not in (x.dtype, torch.float32) or gate.device != x.device:
+            raise SMPInvalidArgumentError("gate must be a tensor of x's dtype or fp32, on its device")
+        lead = x.dim() - gate.dim()
+        if lead < 0 or any(n not in (1, m) for n, m in zip(gate.shape, x.shape[lead:])):
+            raise SMPInvalidArgumentError(f"gate {tuple(gate.shape)} does not broadcast to {tuple(x.shape)}")
+    if not fused_ok(x):
+        h = x.float() if post_weight is None else _norm_torch(x.float(), post_weight, post_bias, eps, rms)
+        s = residual.float() + residual_scale * (h if gate is None else gate.float() * h)
+        return _norm_torch(s, weight, bias, eps, rms).to(x.dtype), s.to(x.dtype)
+    d, run = x.shape[-1], 1
+    if gate is not None:
+        gate, run = _gate_matrix(gate if gate.dim() else gate.reshape(1), x.shape)
+        gate = gate.contiguous()
+    vectors = [t.contiguous() if t is not None else None for t in (weight, bias, post_weight, post_bias)]
+    y, s = _BlockNorm.apply(x.reshape(-1, d).contiguous(), residual.reshape(-1, d).contiguous(), *vectors, gate, run,
+                            residual_scale, eps, bool(rms))
+    return y.view(x.shape), s.view(x.shape)
+
+
+def rms_norm(x, weight, eps=1e-5):
+    """``x / sqrt(mean(x^2) + eps) * weight``: the norm before the first block of a model whose
+    blocks are joined by ``block_norm(..., rms=True)``.  ``weight`` [dim] of x's dtype or fp32."""
+    _check_rows(x, "x")
+    _check_norm("weight", x, weight, None, weight.dtype if torch.is_tensor(weight) else None)
+    eps = float(eps)
+    if not (math.isfinite(eps) and eps >= 0.0):
+        raise SMPInvalidArgumentError(f"bad eps {eps}")
+    if not fused_ok(x):
+        return _norm_torch(x.float(), weight, None, eps, True).to(x.dtype)
+    y = _BlockNorm.apply(None, x.reshape(-1, x.shape[-1]).contiguous(), weight.contiguous(), None, None, None, None, 1,
+                         1.0, eps, True)
+    return y.view(x.shape)

@@ -1,0 +1,231 @@
+"""The block-norm kernels against 64-bit arithmetic, held to the bounds of block_norm_ref.slack
+and one rounding (half a step) into each output's type."""
+import pytest
+import torch
+
+from tests import block_norm_ref as ref
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def within(name, got, exact, slack):
+    dt = torch.finfo(got.dtype)
+    bound = slack + dt.eps / 2 * (exact.abs() + slack) + dt.tiny * dt.eps
+    err = (got.double() - exact).abs()
+    assert bool((err <= bound).all()), (
+        f"{name}: {int((~(err <= bound)).sum())} of {err.numel()} values off, worst {float((err / bound).max())} bounds")
+
+
+def inputs(shape, dtype, wdtype, rms, post, gate, seed=0, mean=0.3, gdtype=None):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    b, s, d = shape
+
+    def r(*n, dt=dtype, m=0.0, std=1.0):
+        return (torch.randn(n, generator=g, device="cuda") * std + m).to(dt)
+
+    gshape = {"none": None, "scalar": (), "channel": (d,), "sample": (b, 1, d), "places": (1, s, d),
+              "rows": (b, s, 1), "full": (b, s, d)}[gate]
+    return {"x": r(b, s, d, m=mean), "residual": r(b, s, d, m=-mean, std=2.0), "weight": r(d, dt=wdtype, m=1.0, std=0.2),
+            "bias": None if rms else r(d, dt=wdtype), "post_weight": r(d, dt=wdtype, m=1.0, std=0.2) if post else None,
+            "post_bias": r(d, dt=wdtype) if post and not rms else None,
+            "gate": None if gshape is None else r(*gshape, dt=gdtype or dtype, m=0.5)}
+
+
+def call(t, alpha, eps, rms):
+    from smdistributed_modelparallel_amd.ops.layernorm import block_norm
+
+    return block_norm(t["x"], t["residual"], t["weight"], t["bias"], t["post_weight"], t["post_bias"], t["gate"], alpha,
+                      eps, rms)
+
+
+def check(shape, dtype, wdtype=None, rms=False, post=True, gate="none", alpha=0.5, eps=1e-5, use=("y", "s"), **kw):
+    t = inputs(shape, dtype, wdtype or dtype, rms, post, gate, **kw)
+    leaf = {k: None if v is None else v.clone().requires_grad_() for k, v in t.items()}
+    y, s = call(leaf, alpha, eps, rms)
+    assert y.shape == s.shape == torch.Size(shape) and y.dtype == s.dtype == dtype
+    g = torch.Generator(device="cuda").manual_seed(11)
+    dy, ds = ((torch.randn(shape, generator=g, device="cuda") * 0.5).to(dtype) if n in use else None for n in ("y", "s"))
+    outs = [(o, d) for o, d in ((y, dy), (s, ds)) if d is not None]
+    names = [k for k, v in leaf.items() if v is not None and (dy is not None or k not in ("weight", "bias"))]
+    grads = torch.autograd.grad([o for o, _ in outs], [leaf[k] for k in names], [d for _, d in outs])
+    want, slack = ref.exact(t, alpha, eps, rms, dy, ds), ref.slack(t, alpha, eps, rms, dy, ds)
+    within("y", y, want["y"], slack["y"])
+    within("s", s, want["s"], slack["s"])
+    for k, got in zip(names, grads):
+        within("d" + k, got, want["d" + k], slack["d" + k])
+    return [y, s, *grads]
+
+
+SHAPES = [(1, 1, 1), (1, 1, 64), (2, 3, 7), (3, 5, 8), (1, 700, 40), (5, 41, 512), (2, 129, 1600), (7, 33, 1601),
+          (3, 50, 2056), (2, 20, 4096), (2, 9, 6144), (1, 7, 8192), (1, 5, 8193), (2, 3, 12288), (1, 3, 16384)]
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sizes(shape, dtype):
+    check(shape, dtype, gate="channel")
+    check(shape, dtype, torch.float32, rms=True, gate="sample")
+
+
+@pytest.mark.parametrize("rms", [False, True])
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("gate", ["none", "scalar", "channel", "sample", "places", "rows", "full"])
+@pytest.mark.parametrize("dtype,wdtype", [(torch.float32, torch.float32), (torch.float16, torch.float16),
+                                          (torch.bfloat16, torch.float32)])
+def test_forms(dtype, wdtype, rms, post, gate):
+    check((6, 37, 200), dtype, wdtype, rms, post, gate, alpha=-0.75)
+
+
+@pytest.mark.parametrize("use", [("y",), ("s",)])
+@pytest.mark.parametrize("post", [False, True])
+def test_one_output_used(use, post):
+    check((3, 40, 136), torch.bfloat16, post=post, gate="channel", use=use)
+
+
+@pytest.mark.parametrize("shape,gate", [((3000, 3, 24), "sample"), ((30, 300, 24), "full"), ((600, 40, 72), "sample"),
+                                        ((2, 9000, 48), "sample"), ((1, 20000, 96), "channel"), ((9000, 2, 16), "none")])
+def test_many_rows(shape, gate):
+    """More gate rows than units, fewer, and one for all rows; fp32 gate beside 16-bit rows."""
+    check(shape, torch.bfloat16, torch.float32, gate=gate, gdtype=torch.float32)
+
+
+def test_only_some_gradients():
+    t = inputs((4, 9, 80), torch.float32, torch.float32, False, True, "channel")
+    want = ref.exact(t, 1.0, 1e-5, False, torch.ones(4, 9, 80, device="cuda"), None)
+    slack = ref.slack(t, 1.0, 1e-5, False, torch.ones(4, 9, 80, device="cuda"), None)
+    for k in ("x", "residual", "gate", "post_bias", "weight"):
+        leaf = dict(t, **{k: t[k].clone().requires_grad_()})
+        y, _ = call(leaf, 1.0, 1e-5, False)
+        (got,) = torch.autograd.grad(y.sum(), leaf[k])  # an expanded gradient
+        within("d" + k, got, want["d" + k], slack["d" + k])
+
+
+def test_layouts():
+    """Transposed and sliced rows, gates and gradients, off 16 bytes and not."""
+    t = inputs((5, 12, 104), torch.bfloat16, torch.bfloat16, False, True, "sample")
+    u = dict(t)
+    u["x"] = t["x"].transpose(0, 1).contiguous().transpose(0, 1)
+    u["residual"] = torch.cat([t["residual"], t["residual"]], -1)[..., :104]
+    u["gate"] = torch.cat([t["gate"], t["gate"]], 1)[:, :1]
+    u["weight"] = torch.stack([t["weight"], t["weight"]], -1)[:, 0]
+    big = torch.empty(104 * 60 + 1, device="cuda", dtype=torch.bfloat16)
+    v = dict(t, x=big[1:].view(5, 12, 104).copy_(t["x"]))
+    base = call(t, 0.5, 1e-5, False)
+    for other in (u, v):
+        assert all(torch.equal(a, b) for a, b in zip(base, call(other, 0.5, 1e-5, False)))
+    leaf = {k: None if x is None else x.detach().requires_grad_() for k, x in u.items()}
+    y, s = call(leaf, 0.5, 1e-5, False)
+    dy = torch.randn(12, 104, 5, device="cuda").bfloat16().permute(2, 0, 1)
+    names = [k for k, x in leaf.items() if x is not None]
+    want, slack = ref.exact(t, 0.5, 1e-5, False, dy), ref.slack(t, 0.5, 1e-5, False, dy)
+    for k, got in zip(names, torch.autograd.grad(y, [leaf[k] for k in names], dy)):
+        within("d" + k, got, want["d" + k], slack["d" + k])
+
+
+@pytest.mark.parametrize("rms", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_constant_zero_and_infinite_rows(dtype, rms):
+    """Rows without deviation are finite; infinities and NaN stay in their rows."""
+    t = inputs((1, 6, 48), dtype, dtype, rms, True, "none")
+    for k in ("x", "residual"):
+        t[k][0, 0] = 0.0
+        t[k][0, 1] = 3.0
+    t["x"][0, 2, 5] = float("inf")
+    t["x"][0, 3, 47] = float("nan")
+    leaf = {k: None if v is None else v.clone().requires_grad_() for k, v in t.items()}
+    y, s = call(leaf, 1.0, 1e-5, rms)
+    dx, = torch.autograd.grad(y, leaf["x"], torch.ones_like(y))
+    # a zero row of x and residual: both norms multiply the gradient by 1e-5 ** -0.5 = 316, together
+    # 1e5, which fp16 (65504 at most) cannot hold: infinite exactly where the definition is too large
+    want = ref.exact({k: v if v is None else v[:, [0, 1, 4, 5]] for k, v in t.items() if v is None or v.dim() == 3}
+                     | {k: v for k, v in t.items() if v is not None and v.dim() == 1}, 1.0, 1e-5, rms,
+                     torch.ones_like(y[:, [0, 1, 4, 5]]))["dx"]
+    over = want.abs() > torch.finfo(dtype).max * (1 + 2.0 ** -12)
+    assert torch.equal(dx[:, [0, 1, 4, 5]].isinf(), over) and not dx[0, [2, 3]].isfinite().all(-1).any()
+    for o in (y, s):
+        assert o[0, [0, 1, 4, 5]].isfinite().all() and not o[0, [2, 3]].isfinite().all(-1).any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [40, 1601, 4096])
+def test_rms_norm(dtype, d):
+    from smdistributed_modelparallel_amd.ops.layernorm import rms_norm
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(3, 50, d, generator=g, device="cuda").to(dtype).requires_grad_()
+    w = torch.randn(d, generator=g, device="cuda").requires_grad_()
+    dy = torch.randn(3, 50, d, generator=g, device="cuda").to(dtype)
+    y = rms_norm(x, w, 1e-6)
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    # the definition with nothing added: block_norm of a zero block
+    t = {"x": torch.zeros_like(x), "residual": x, "weight": w}
+    want, slack = ref.exact(t, 1.0, 1e-6, True, dy), ref.slack(t, 1.0, 1e-6, True, dy)
+    within("y", y, want["y"], slack["y"])
+    within("dx", dx, want["dresidual"], slack["dresidual"])
+    within("dw", dw, want["dweight"], slack["dweight"])
+
+
+def test_bound_gradients_and_a_shared_parameter():
+    """Parameters bound to the flat gradient buffer are added to in place; one that serves as both
+    weights gets the sum."""
+    t = inputs((3, 70, 160), torch.bfloat16, torch.bfloat16, False, True, "channel")
+    names = ("weight", "bias", "post_bias", "gate")
+    p = {k: torch.nn.Parameter(t[k].clone()) for k in names}
+    start = {}
+    for k, q in p.items():
+        q.grad = torch.randn_like(q)
+        q._smp_fused_grad = True
+        start[k] = q.grad.clone()
+    x, r = t["x"].requires_grad_(), t["residual"].requires_grad_()
+    u = {"x": x, "residual": r, "post_weight": p["weight"], **p}
+    y, s = call(u, 0.5, 1e-5, False)
+    dy, ds = torch.randn_like(y), torch.randn_like(s)
+    torch.autograd.backward([y, s], [dy, ds])
+    want, slack = ref.exact(u, 0.5, 1e-5, False, dy, ds), ref.slack(u, 0.5, 1e-5, False, dy, ds)
+    eps = torch.finfo(torch.bfloat16).eps
+    for k in names:
+        exact, room = want["d" + k], slack["d" + k]
+        if k == "weight":  # two contributions, the second rounded by itself and added to the bound gradient
+            other = want["dpost_weight"]
+            room = room + slack["dpost_weight"] + eps / 2 * (exact.abs() + other.abs() + start[k].double().abs() + room)
+            exact = exact + other
+        within(k, p[k].grad, exact + start[k].double(), room + ref.FEW * start[k].double().abs())
+
+
+def test_no_rows_on_the_gpu():
+    w = torch.ones(8, device="cuda", requires_grad=True)
+    x = torch.empty(0, 8, device="cuda", requires_grad=True)
+    y, s = call({"x": x, "residual": x, "weight": w, "bias": None, "post_weight": w, "post_bias": None, "gate": None},
+                1.0, 1e-5, True)
+    dx, dw = torch.autograd.grad((y + s).sum(), [x, w])
+    assert y.shape == dx.shape == (0, 8) and torch.equal(dw, torch.zeros_like(w))
+
+
+def test_same_bits_and_graph_replays():
+    t = inputs((4, 300, 328), torch.bfloat16, torch.float32, False, True, "sample")
+    leaf = {k: None if v is None else v.requires_grad_() for k, v in t.items()}
+    dy, ds = (torch.randn(4, 300, 328, device="cuda").bfloat16() for _ in range(2))
+    names = [k for k, v in leaf.items() if v is not None]
+
+    def step():
+        y, s = call(leaf, 0.5, 1e-5, False)
+        return [y.detach(), s.detach(), *torch.autograd.grad([y, s], [leaf[k] for k in names], [dy, ds])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(3):
+        with torch.no_grad():
+            leaf["x"].normal_()
+            leaf["gate"].normal_()
+        dy.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, e in zip(out, step()):
+            assert torch.equal(a, e)
