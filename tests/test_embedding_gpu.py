@@ -87,6 +87,13 @@ def test_sizes(b, s, rows, dim, dtype):
     check(b, s, rows, dim, dtype)
 
 
+@pytest.mark.parametrize("b,s,rows,dim", [(8, 5000, 60000, 16), (3, 16384, 1023, 9), (3, 16384, 1024, 8), (1, 700001, 3000, 8),
+                                          (1, 600000, 1200000, 2), (2, 9000, 2, 3000), (64, 17, 40, 9000)])
+def test_long_lists(b, s, rows, dim):
+    """Lists that many blocks sort, one to three passes, rows of several column slabs."""
+    check(b, s, rows, dim, torch.bfloat16, positions="implicit")
+
+
 @pytest.mark.parametrize("positions", ["implicit", "given"])
 @pytest.mark.parametrize("dtype,dim", [(torch.float32, 36), (torch.bfloat16, 1600), (torch.float16, 37)])
 def test_positions_and_scale(positions, dtype, dim):
