@@ -12,7 +12,7 @@ namespace smpk {
 namespace {
 
 constexpr int kT = 256;
-constexpr int64_t kShortSort = 16384;
+constexpr int64_t kShortSort = 16384;  // tokens that one block sorts alone
 
 // Row of a table for one token, or -1 where the id is not one of its rows.
 __device__ __forceinline__ int64_t row_of(const IndexList& l, int64_t t) {
@@ -26,65 +26,132 @@ __device__ __forceinline__ int64_t row_of(const IndexList& l, int64_t t) {
   return id >= 0 && id < l.rows ? id : -1;
 }
 
-template <typename T, int N>
-struct Pack {
-  T v[N];
+// A thread handles 8 consecutive columns of a row.  Rows of odd widths start off 16 bytes: the
+// hardware loads and stores 16 bytes at any address, so only a row's last, partial vector goes
+// element by element.
+constexpr int kCols = 8;
+
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Any16 {
+  T v[16 / sizeof(T)];
+};
+template <typename T>
+struct Raw8 {
+  Any16<T> a[kCols * sizeof(T) / 16];
 };
 
-template <typename T, int N>
-__device__ __forceinline__ void load_pack(const T* p, float (&o)[N]) {
-  if constexpr (N > 1) {
-    const Vec16<T> a = load16(p);
+// FULL: rows are whole vectors; then no thread branches on `left`, and a batch of loads is issued
+// without a wait between them.
+template <bool FULL, typename T>
+__device__ __forceinline__ void read8(const T* p, int left, Raw8<T>& r) {
+  constexpr int M = 16 / sizeof(T);
+  if (FULL || left >= kCols) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) o[j] = to_f32(a.v[j]);
+    for (int k = 0; k < kCols / M; ++k) __builtin_memcpy(&r.a[k], p + k * M, 16);
   } else {
-    o[0] = to_f32(*p);
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) r.a[j / M].v[j % M] = j < left ? p[j] : from_f32<T>(0.f);
   }
 }
-template <typename T, int N>
-__device__ __forceinline__ void store_pack(T* p, const float (&o)[N]) {
-  if constexpr (N > 1) {
-    Vec16<T> a;
+template <typename T>
+__device__ __forceinline__ float at8(const Raw8<T>& r, int j) {
+  constexpr int M = 16 / sizeof(T);
+  return to_f32(r.a[j / M].v[j % M]);
+}
+template <bool FULL, typename T>
+__device__ __forceinline__ void write8(T* p, int left, const float (&o)[kCols]) {
+  constexpr int M = 16 / sizeof(T);
+  if (FULL || left >= kCols) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) a.v[j] = from_f32<T>(o[j]);
-    store16(p, a);
+    for (int k = 0; k < kCols / M; ++k) {
+      Any16<T> a;
+#pragma unroll
+      for (int j = 0; j < M; ++j) a.v[j] = from_f32<T>(o[k * M + j]);
+      __builtin_memcpy(p + k * M, &a, 16);
+    }
   } else {
-    *p = from_f32<T>(o[0]);
+#pragma unroll
+    for (int j = 0; j < kCols; ++j)
+      if (j < left) p[j] = from_f32<T>(o[j]);
   }
 }
 
-template <typename T, int N>
+constexpr int kPerThread = 4;  // vectors of a thread, all loads in flight together
+
+// Vectors of the output in order, kT * kPerThread of them a block: all lanes are busy at any width.
+// Threads past the end and tokens without a row load row 0 and drop it: no branch separates the
+// loads.
+template <typename T, bool FULL>
 __global__ void __launch_bounds__(kT) emb_fwd(IndexList ids, const T* __restrict__ w, int64_t w_stride, float scale,
                                               int foreign_zero, IndexList pos, const T* __restrict__ p,
-                                              int64_t p_stride, T* __restrict__ y, int64_t n, int d) {
-  const int per_row = d / N;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kT + threadIdx.x;
-  if (i >= n * per_row) return;
-  const int64_t t = i / per_row;
-  const int c = static_cast<int>(i - t * per_row) * N;
-  const int64_t r = row_of(ids, t);
-  float o[N];
-  if (r >= 0) {
-    load_pack<T, N>(w + r * w_stride + c, o);
+                                              int64_t p_stride, T* __restrict__ y, int n, int d, uint32_t per_row,
+                                              uint32_t reciprocal) {
+  const int64_t v0 = static_cast<int64_t>(blockIdx.x) * (kT * kPerThread);
+  const int t0 = static_cast<int>(v0 / per_row);
+  const uint32_t r0 = static_cast<uint32_t>(v0 - static_cast<int64_t>(t0) * per_row);
+  int t[kPerThread], c[kPerThread];
+  int64_t id[kPerThread], at[kPerThread];
 #pragma unroll
-    for (int j = 0; j < N; ++j) o[j] *= scale;
+  for (int u = 0; u < kPerThread; ++u) {
+    const uint32_t off = r0 + u * kT + threadIdx.x;
+    uint32_t q = __umulhi(off, reciprocal), r = off - q * per_row;  // reciprocal rounded down: q may be one short
+    q += r >= per_row ? 1 : 0;
+    r -= r >= per_row ? per_row : 0;
+    t[u] = t0 + static_cast<int>(q);
+    c[u] = static_cast<int>(r) * kCols;
+  }
+  if (ids.wide) {
+#pragma unroll
+    for (int u = 0; u < kPerThread; ++u) id[u] = static_cast<const int64_t*>(ids.ids)[t[u] < n ? t[u] : 0];
   } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j) o[j] = foreign_zero ? 0.f : NAN;
+    for (int u = 0; u < kPerThread; ++u) id[u] = static_cast<const int32_t*>(ids.ids)[t[u] < n ? t[u] : 0];
   }
   if (p != nullptr) {
-    const int64_t q = row_of(pos, t);
-    float a[N];
-    if (q >= 0) {
-      load_pack<T, N>(p + q * p_stride + c, a);
+    if (pos.ids == nullptr) {
+      const uint32_t period = static_cast<uint32_t>(pos.period), first = static_cast<uint32_t>(t0) % period;
+#pragma unroll
+      for (int u = 0; u < kPerThread; ++u) {
+        uint32_t k = first + static_cast<uint32_t>(t[u] - t0);
+        if (k >= period) k -= period;
+        at[u] = k < period ? k : k % period;  // (a block spans several periods)
+      }
+    } else if (pos.wide) {
+#pragma unroll
+      for (int u = 0; u < kPerThread; ++u) at[u] = static_cast<const int64_t*>(pos.ids)[t[u] < n ? t[u] : 0];
     } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j) a[j] = NAN;
+      for (int u = 0; u < kPerThread; ++u) at[u] = static_cast<const int32_t*>(pos.ids)[t[u] < n ? t[u] : 0];
     }
-#pragma unroll
-    for (int j = 0; j < N; ++j) o[j] += a[j];
   }
-  store_pack<T, N>(y + t * d + c, o);
+  Raw8<T> a[kPerThread], b[kPerThread];
+  bool held[kPerThread];
+#pragma unroll
+  for (int u = 0; u < kPerThread; ++u) {
+    const int64_t row = id[u] - ids.start;
+    held[u] = row >= 0 && row < ids.rows;
+    read8<FULL>(w + (held[u] ? row : 0) * w_stride + c[u], d - c[u], a[u]);
+  }
+  if (p != nullptr) {
+#pragma unroll
+    for (int u = 0; u < kPerThread; ++u) {
+      const bool ok = at[u] >= 0 && at[u] < pos.rows;
+      read8<FULL>(p + (ok ? at[u] : 0) * p_stride + c[u], d - c[u], b[u]);
+      at[u] = ok;
+    }
+  }
+  const float none = foreign_zero ? 0.f : NAN;
+#pragma unroll
+  for (int u = 0; u < kPerThread; ++u) {
+    float o[kCols];
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) o[j] = held[u] ? at8(a[u], j) * scale : none;
+    if (p != nullptr) {
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) o[j] += at[u] ? at8(b[u], j) : NAN;
+    }
+    if (t[u] < n) write8<FULL>(y + static_cast<int64_t>(t[u]) * d + c[u], d - c[u], o);
+  }
 }
 
 // ----------------------------------------------------------------------- sorting the tokens
@@ -106,6 +173,7 @@ struct SortItems {
   int32_t* tokens_out;
   int64_t n, per_block;  // per_block: a multiple of kSortThreads
   int shift, bits;
+  uint8_t* marks;  // null, or [rows rounded up to 16]: 1 for every row that has a token
 };
 
 // Rows' keys are their numbers; tokens without a row come last, with the key `rows`.
@@ -121,40 +189,68 @@ __device__ __forceinline__ void wave_run(const SortItems& a, int block, int64_t&
   e = s + part < a.n ? s + part : a.n;
 }
 
+constexpr int kRounds = 8;  // 64-item rounds of a wave whose keys are loaded together
+
+__device__ __forceinline__ void load_keys(const SortItems& a, int64_t i0, int64_t e, uint32_t (&key)[kRounds]) {
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int64_t i = i0 + r * 64 + (threadIdx.x & 63);
+    key[r] = i < e ? key_of(a, i) : 0u;
+  }
+}
+
+__device__ __forceinline__ void count_digits(const SortItems& a, int64_t s, int64_t e, int32_t* cnt) {
+  for (int64_t i0 = s; i0 < e; i0 += 64 * kRounds) {
+    uint32_t key[kRounds];
+    load_keys(a, i0, e, key);
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r)
+      if (i0 + r * 64 + (threadIdx.x & 63) < e) atomicAdd(&cnt[(key[r] >> a.shift) & ((1 << a.bits) - 1)], 1);
+  }
+}
+
+// The first pass also clears the marks that its second launch sets for every row with a token.
+__device__ __forceinline__ void clear_marks(const SortItems& a, int block, int blocks) {
+  if (a.marks == nullptr || a.keys != nullptr) return;
+  const int64_t words = (a.ids.rows + 15) / 16;  // (the workspace is a multiple of 16 bytes)
+  for (int64_t i = static_cast<int64_t>(block) * kSortThreads + threadIdx.x; i < words;
+       i += static_cast<int64_t>(blocks) * kSortThreads)
+    reinterpret_cast<uint4*>(a.marks)[i] = make_uint4(0, 0, 0, 0);
+}
+
 __global__ void __launch_bounds__(kSortThreads) emb_sort_count(SortItems a, int32_t* __restrict__ counts) {
   __shared__ int32_t cnt[1 << kMaxBits];
   const int bins = 1 << a.bits;
   for (int d = threadIdx.x; d < bins; d += kSortThreads) cnt[d] = 0;
+  clear_marks(a, blockIdx.x, gridDim.x);
   __syncthreads();
   int64_t s, e;
   wave_run(a, blockIdx.x, s, e);
-  for (int64_t i = s + (threadIdx.x & 63); i < e; i += 64) atomicAdd(&cnt[(key_of(a, i) >> a.shift) & (bins - 1)], 1);
+  count_digits(a, s, e, cnt);
   __syncthreads();
   for (int d = threadIdx.x; d < bins; d += kSortThreads) counts[static_cast<int64_t>(blockIdx.x) * bins + d] = cnt[d];
 }
 
-// One pass of one block.  counts [blocks][bins]: of all blocks (a single block needs none).
-__device__ __forceinline__ void sort_pass(const SortItems& a, const int32_t* counts, int blocks, int block,
-                                          int32_t (*cnt)[1 << kMaxBits], int32_t* wave_total) {
-  const int bins = 1 << a.bits, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  for (int d = lane; d < bins; d += 64) cnt[wid][d] = 0;
-  __syncthreads();
-  int64_t s, e;
-  wave_run(a, block, s, e);
-  for (int64_t i = s + lane; i < e; i += 64) atomicAdd(&cnt[wid][(key_of(a, i) >> a.shift) & (bins - 1)], 1);
-  __syncthreads();
-  // thread d owns digit d: items with smaller digits anywhere, then of this digit in earlier blocks
-  int total = 0, before = 0;
+template <int BITS>
+struct SortLds {
+  int32_t cnt[kWaves][1 << BITS];
+  int32_t total[1 << BITS], before[1 << BITS];
+  int32_t wave_total[kWaves];
+};
+
+// cnt[w][d], the items of digit d in wave w, becomes the place of the first of them: after all items
+// of smaller digits (anywhere), and of digit d in earlier blocks (`before`) and waves.
+template <int BITS>
+__device__ __forceinline__ void counts_to_places(SortLds<BITS>& lds, int bins, bool one_block) {
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  int c[kWaves], total = 0;
   if (tid < bins) {
-    if (blocks == 1) {
-      for (int w = 0; w < kWaves; ++w) total += cnt[w][tid];
-    } else {
-      for (int b = 0; b < blocks; ++b) {
-        const int c = counts[static_cast<int64_t>(b) * bins + tid];
-        total += c;
-        before += b < block ? c : 0;
-      }
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      c[w] = lds.cnt[w][tid];
+      total += c[w];
     }
+    if (!one_block) total = lds.total[tid];
   }
   int incl = total;
 #pragma unroll
@@ -162,62 +258,136 @@ __device__ __forceinline__ void sort_pass(const SortItems& a, const int32_t* cou
     const int v = __shfl_up(incl, o, 64);
     if (lane >= o) incl += v;
   }
-  if (lane == 63) wave_total[wid] = incl;
+  if (lane == 63) lds.wave_total[wid] = incl;
   __syncthreads();
-  int base = incl - total + before;
-  for (int w = 0; w < wid; ++w) base += wave_total[w];
   if (tid < bins) {
+    int base = incl - total + (one_block ? 0 : lds.before[tid]);
+    for (int w = 0; w < wid; ++w) base += lds.wave_total[w];
+#pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const int c = cnt[w][tid];
-      cnt[w][tid] = base;
-      base += c;
+      lds.cnt[w][tid] = base;
+      base += c[w];
     }
   }
   __syncthreads();
-  for (int64_t i0 = s; i0 < e; i0 += 64) {
-    const int64_t i = i0 + lane;
-    const bool valid = i < e;
-    const uint32_t key = valid ? key_of(a, i) : 0u;
-    const int digit = (key >> a.shift) & (bins - 1);
-    uint64_t same = __ballot(valid);  // the lanes with this lane's digit
-    for (int b = 0; b < a.bits; ++b) {
-      const bool one = (digit >> b) & 1;
-      const uint64_t m = __ballot(one);
-      same &= one ? m : ~m;
+}
+
+// Places of a wave's next 64 items, in lane order for equal digits; cnt moves on.
+__device__ __forceinline__ int place_of(int digit, bool valid, int bits, int32_t* cnt) {
+  const int lane = threadIdx.x & 63;
+  uint64_t same = __ballot(valid);  // the lanes with this lane's digit
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (digit >> b) & 1;
+    const uint64_t m = __ballot(one);
+    same &= one ? m : ~m;
+  }
+  const int first = valid ? __ffsll(static_cast<unsigned long long>(same)) - 1 : lane;
+  int at = 0;
+  if (valid && lane == first) at = atomicAdd(&cnt[digit], __popcll(same));
+  return __shfl(at, first, 64) + __popcll(same & ((1ull << lane) - 1));
+}
+
+// One pass over the items of one block; counts [blocks][bins] of all blocks.
+__global__ void __launch_bounds__(kSortThreads) emb_sort_place(SortItems a, const int32_t* __restrict__ counts) {
+  __shared__ SortLds<kMaxBits> lds;
+  const int bins = 1 << a.bits, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int blocks = gridDim.x, block = blockIdx.x;
+  for (int d = lane; d < bins; d += 64) lds.cnt[wid][d] = 0;
+  if (tid < bins) lds.total[tid] = lds.before[tid] = 0;
+  __syncthreads();
+  int64_t s, e;
+  wave_run(a, block, s, e);
+  count_digits(a, s, e, lds.cnt[wid]);
+  {  // every thread adds up one digit of some blocks
+    int total = 0, before = 0;
+    const int digit = tid & (bins - 1), step = kSortThreads >> a.bits;
+#pragma unroll 8
+    for (int b = tid >> a.bits; b < blocks; b += step) {
+      const int c = counts[(static_cast<int64_t>(b) << a.bits) + digit];
+      total += c;
+      before += b < block ? c : 0;
     }
-    const int first = valid ? __ffsll(static_cast<unsigned long long>(same)) - 1 : lane;
-    int at = 0;
-    if (valid && lane == first) at = atomicAdd(&cnt[wid][digit], __popcll(same));
-    at = __shfl(at, first, 64) + __popcll(same & ((1ull << lane) - 1));
-    if (valid) {
-      a.keys_out[at] = key;
-      a.tokens_out[at] = a.tokens != nullptr ? a.tokens[i] : static_cast<int32_t>(i);
+    atomicAdd(&lds.total[digit], total);
+    atomicAdd(&lds.before[digit], before);
+  }
+  __syncthreads();
+  counts_to_places(lds, bins, false);
+  for (int64_t i0 = s; i0 < e; i0 += 64 * kRounds) {
+    uint32_t keys[kRounds];
+    int32_t token[kRounds];
+    load_keys(a, i0, e, keys);
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      const int64_t i = i0 + r * 64 + lane;
+      token[r] = a.tokens != nullptr && i < e ? a.tokens[i] : static_cast<int32_t>(i);
+    }
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      if (i0 + r * 64 >= e) break;
+      const bool valid = i0 + r * 64 + lane < e;
+      const int at = place_of((keys[r] >> a.shift) & (bins - 1), valid, a.bits, lds.cnt[wid]);
+      if (valid) {
+        a.keys_out[at] = keys[r];
+        a.tokens_out[at] = token[r];
+        if (a.marks != nullptr && a.keys == nullptr && keys[r] < a.ids.rows) a.marks[keys[r]] = 1;
+      }
     }
   }
 }
 
-__global__ void __launch_bounds__(kSortThreads) emb_sort_place(SortItems a, const int32_t* __restrict__ counts) {
-  __shared__ int32_t cnt[kWaves][1 << kMaxBits];
-  __shared__ int32_t wave_total[kWaves];
-  sort_pass(a, counts, gridDim.x, blockIdx.x, cnt, wave_total);
-}
+// All passes over a list of at most R * 1024 items in one block: the items stay in registers and
+// change places through LDS (one CU stores only one scattered 4-byte word a clock to memory).
+constexpr int kShortBits = 8;  // of a pass: the counters and 16384 items fit the 160 KB of LDS
 
-// All passes of a short list in one block; the result lies in keys_out / tokens_out.
-__global__ void __launch_bounds__(kSortThreads) emb_sort_short(SortItems a, uint32_t* keys2, int32_t* tokens2,
-                                                               int passes) {
-  __shared__ int32_t cnt[kWaves][1 << kMaxBits];
-  __shared__ int32_t wave_total[kWaves];
-  uint32_t* k[2] = {a.keys_out, keys2};
-  int32_t* t[2] = {a.tokens_out, tokens2};
-  for (int p = 0; p < passes; ++p) {
-    const int to = (passes - 1 - p) & 1;
-    a.keys_out = k[to];
-    a.tokens_out = t[to];
-    sort_pass(a, nullptr, 1, 0, cnt, wave_total);
+template <int R>
+__global__ void __launch_bounds__(kSortThreads) emb_sort_short(SortItems a, int passes) {
+  __shared__ SortLds<kShortBits> lds;
+  __shared__ uint32_t keys[R * kSortThreads];
+  __shared__ int32_t tokens[R * kSortThreads];
+  const int bins = 1 << a.bits, lane = threadIdx.x & 63, wid = threadIdx.x >> 6, n = static_cast<int>(a.n);
+  const int s = wid * (64 * R) + lane;  // this thread's items are 64 apart
+  uint32_t key[R];
+  int32_t token[R];
+  clear_marks(a, 0, 1);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = s + r * 64;
+    key[r] = i < n ? key_of(a, i) : 0u;
+    token[r] = i;
+  }
+  for (int p = 0; p < passes; ++p, a.shift += a.bits) {
+    for (int d = lane; d < bins; d += 64) lds.cnt[wid][d] = 0;  // (its own wave's: no barrier)
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (s + r * 64 < n) atomicAdd(&lds.cnt[wid][(key[r] >> a.shift) & (bins - 1)], 1);
     __syncthreads();
-    a.keys = k[to];
-    a.tokens = t[to];
-    a.shift += a.bits;
+    counts_to_places(lds, bins, true);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool valid = s + r * 64 < n;
+      const int at = place_of((key[r] >> a.shift) & (bins - 1), valid, a.bits, lds.cnt[wid]);
+      if (valid) {
+        keys[at] = key[r];
+        tokens[at] = token[r];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (s + r * 64 < n) {
+        key[r] = keys[s + r * 64];
+        token[r] = tokens[s + r * 64];
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = s + r * 64;
+    if (i >= n) continue;
+    a.keys_out[i] = key[r];
+    a.tokens_out[i] = token[r];
+    if (a.marks != nullptr && key[r] < a.ids.rows && (i == 0 || keys[i - 1] != key[r])) a.marks[key[r]] = 1;
   }
 }
 
@@ -238,77 +408,138 @@ struct Sorted {
   }
 };
 
-constexpr int kCols = 8;    // columns of a thread
-constexpr int kAhead = 8;  // rows whose loads are in flight together
-
-template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Any16 {
-  T v[16 / sizeof(T)];
-};
-template <typename T>
-struct Raw8 {
-  Any16<T> a[kCols * sizeof(T) / 16];
-};
-
-template <typename T>
-__device__ __forceinline__ void read8(const T* p, int left, Raw8<T>& r) {
-  constexpr int M = 16 / sizeof(T);
-  if (left >= kCols) {
-#pragma unroll
-    for (int k = 0; k < kCols / M; ++k) __builtin_memcpy(&r.a[k], p + k * M, 16);
-  } else {
-#pragma unroll
-    for (int j = 0; j < kCols; ++j) r.a[j / M].v[j % M] = j < left ? p[j] : from_f32<T>(0.f);
-  }
-}
-template <typename T>
-__device__ __forceinline__ float at8(const Raw8<T>& r, int j) {
-  constexpr int M = 16 / sizeof(T);
-  return to_f32(r.a[j / M].v[j % M]);
-}
-template <typename T>
-__device__ __forceinline__ void write8(T* p, int left, const float (&o)[kCols]) {
-  constexpr int M = 16 / sizeof(T);
-  if (left >= kCols) {
-#pragma unroll
-    for (int k = 0; k < kCols / M; ++k) {
-      Any16<T> a;
-#pragma unroll
-      for (int j = 0; j < M; ++j) a.v[j] = from_f32<T>(o[k * M + j]);
-      __builtin_memcpy(p + k * M, &a, 16);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < kCols; ++j)
-      if (j < left) p[j] = from_f32<T>(o[j]);
-  }
-}
-
 // dw row = scale * sum, or that added to the row
-template <typename T>
+template <bool FULL, typename T>
 __device__ __forceinline__ void write_row(T* p, int left, float (&sum)[kCols], float scale, int accumulate) {
   if (accumulate) {
     Raw8<T> r;
-    read8(p, left, r);
+    read8<FULL>(p, left, r);
 #pragma unroll
     for (int j = 0; j < kCols; ++j) sum[j] = fmaf(sum[j], scale, at8(r, j));
   } else {
 #pragma unroll
     for (int j = 0; j < kCols; ++j) sum[j] *= scale;
   }
-  write8(p, left, sum);
+  write8<FULL>(p, left, sum);
 }
 
-// `lanes` threads (a power of two) hold a chunk's columns, kT / lanes chunks a block
-template <typename T>
-__global__ void __launch_bounds__(kT) emb_bwd_chunks(Sorted l, const T* __restrict__ dy, int d, int chunk, int lanes,
-                                                     float scale, T* __restrict__ dw, int accumulate,
-                                                     float* __restrict__ part) {
+constexpr int kZeroRows = 64;
+
+// A dense gradient: 64 rows x 512 columns a block, of which the rows without a token are cleared
+// (marks null: the rows from `period` on).
+template <bool FULL, typename T>
+__device__ __forceinline__ void clear_rows(const Sorted& l, const uint8_t* marks, int64_t block, int slabs, T* dw,
+                                           int d) {
+  const int lane = threadIdx.x & 63;
+  const int64_t window = block / slabs, r0 = window * kZeroRows, mine = r0 + lane;
+  const int c = (static_cast<int>(block - window * slabs) * 64 + lane) * kCols;
+  const bool empty = mine < l.rows && (l.n == 0 || (marks != nullptr ? marks[mine] == 0 : mine >= l.period));
+  uint64_t rows = __ballot(empty);  // the same in all waves, which take every fourth of them
+  const float zero[kCols] = {};
+  for (int k = 0; rows != 0; ++k, rows &= rows - 1) {
+    if (k % (kT / 64) != static_cast<int>(threadIdx.x >> 6)) continue;
+    const int64_t r = r0 + __ffsll(static_cast<unsigned long long>(rows)) - 1;
+    if (c < d) write8<FULL>(dw + r * d + c, d - c, zero);
+  }
+}
+
+// A wave takes a chunk of at most 64 tokens and 512 columns.  Lane i knows the i-th token; a run is
+// followed with scalar registers, so the branches cost nothing, and the gradient rows of one
+// batch are loaded while those of the batch before are added.
+template <typename T, bool FULL>
+__global__ void __launch_bounds__(kT) emb_bwd_wide(Sorted l, const T* __restrict__ dy, int d, int chunk, int slabs,
+                                                   int64_t blocks, float scale, T* __restrict__ dw, int accumulate,
+                                                   float* __restrict__ part, const uint8_t* __restrict__ marks) {
+  constexpr int kAhead = sizeof(T) == 4 ? 4 : 8;
+  if (static_cast<int64_t>(blockIdx.x) >= blocks) {
+    clear_rows<FULL>(l, marks, blockIdx.x - blocks, slabs, dw, d);
+    return;
+  }
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kT / 64) +
+                       __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int64_t ch = unit / slabs;
+  const int c = (static_cast<int>(unit - ch * slabs) * 64 + lane) * kCols, left = d - c;
+  const int64_t j0 = ch * chunk, j1 = j0 + chunk < l.n ? j0 + chunk : l.n;
+  const int from = left > 0 ? c : 0;  // lanes past the row's end load its first vector and drop it
+  if (j0 >= l.n) return;
+  const int m = static_cast<int>(j1 - j0);
+  const uint32_t none = static_cast<uint32_t>(l.rows);
+  const uint32_t my_key = lane < m ? l.key(j0 + lane) : none;
+  const int my_token = lane < m ? static_cast<int>(l.token(j0 + lane, my_key)) : 0;
+  const uint32_t before = j0 > 0 ? l.key(j0 - 1) : none, after = j1 < l.n ? l.key(j1) : none;
+  auto key_at = [&](int i) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(my_key), i)); };
+  // tokens with a row: those without come last
+  const int live = __popcll(__ballot(lane < m && my_key != none));
+  if (live == 0) return;
+  Raw8<T> buf[2][kAhead];
+  auto fetch = [&](int i, Raw8<T> (&r)[kAhead]) {  // (past the last token: that token again, dropped)
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t t = __builtin_amdgcn_readlane(my_token, i + u < live ? i + u : live - 1);
+      read8<FULL>(dy + t * d + from, left, r[u]);
+    }
+  };
+  uint32_t cur = key_at(0);
+  bool head = before == cur;
+  float sum[kCols];
+#pragma unroll
+  for (int q = 0; q < kCols; ++q) sum[q] = 0.f;
+  auto add = [&](int i, const Raw8<T> (&r)[kAhead]) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (i + u >= live) break;
+      const uint32_t k = key_at(i + u);
+      if (k != cur) {
+        if (left > 0) {
+          if (head) {
+            write8<FULL>(part + (2 * ch) * d + c, left, sum);
+          } else {
+            write_row<FULL>(dw + static_cast<int64_t>(cur) * d + c, left, sum, scale, accumulate);
+          }
+        }
+        head = false;
+        cur = k;
+#pragma unroll
+        for (int q = 0; q < kCols; ++q) sum[q] = 0.f;
+      }
+#pragma unroll
+      for (int q = 0; q < kCols; ++q) sum[q] += at8(r[u], q);
+    }
+  };
+  fetch(0, buf[0]);
+  for (int i = 0; i < live; i += 2 * kAhead) {
+    fetch(i + kAhead, buf[1]);
+    add(i, buf[0]);
+    fetch(i + 2 * kAhead, buf[0]);
+    add(i + kAhead, buf[1]);
+  }
+  if (left <= 0) return;
+  const bool tail = live == m && after == cur;
+  if (head || tail) {
+    write8<FULL>(part + (2 * ch + (head ? 0 : 1)) * d + c, left, sum);
+  } else {
+    write_row<FULL>(dw + static_cast<int64_t>(cur) * d + c, left, sum, scale, accumulate);
+  }
+}
+
+// The same for rows of at most 256 columns: `lanes` threads (a power of two) hold a chunk's
+// columns, kT / lanes chunks a block.
+template <typename T, bool FULL>
+__global__ void __launch_bounds__(kT) emb_bwd_narrow(Sorted l, const T* __restrict__ dy, int d, int chunk, int lanes,
+                                                     int64_t blocks, float scale, T* __restrict__ dw, int accumulate,
+                                                     float* __restrict__ part, const uint8_t* __restrict__ marks) {
+  constexpr int kAhead = 8;
+  if (static_cast<int64_t>(blockIdx.x) >= blocks) {
+    clear_rows<FULL>(l, marks, blockIdx.x - blocks, 1, dw, d);
+    return;
+  }
   const int64_t ch = static_cast<int64_t>(blockIdx.x) * (kT / lanes) + threadIdx.x / lanes;
-  const int c = (blockIdx.y * lanes + threadIdx.x % lanes) * kCols;
+  const int c = threadIdx.x % lanes * kCols;
   const int left = d - c;
   const int64_t j0 = ch * chunk, j1 = j0 + chunk < l.n ? j0 + chunk : l.n;
   if (j0 >= l.n || left <= 0) return;
+  const uint32_t none = static_cast<uint32_t>(l.rows);
   uint32_t cur = l.key(j0);
   bool head = j0 > 0 && l.key(j0 - 1) == cur;
   float sum[kCols];
@@ -318,35 +549,35 @@ __global__ void __launch_bounds__(kT) emb_bwd_chunks(Sorted l, const T* __restri
     uint32_t key[kAhead];
     Raw8<T> row[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) key[u] = j + u < j1 ? l.key(j + u) : static_cast<uint32_t>(l.rows);
+    for (int u = 0; u < kAhead; ++u) key[u] = j + u < j1 ? l.key(j + u) : none;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      if (key[u] < l.rows) read8(dy + l.token(j + u, key[u]) * d + c, left, row[u]);
+      if (key[u] != none) read8<FULL>(dy + l.token(j + u, key[u]) * d + c, left, row[u]);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       if (key[u] != cur && j + u < j1) {
         if (head) {
-          write8(part + (2 * ch) * d + c, left, sum);
+          write8<FULL>(part + (2 * ch) * d + c, left, sum);
         } else {
-          write_row(dw + static_cast<int64_t>(cur) * d + c, left, sum, scale, accumulate);
+          write_row<FULL>(dw + static_cast<int64_t>(cur) * d + c, left, sum, scale, accumulate);
         }
         head = false;
         cur = key[u];
 #pragma unroll
         for (int q = 0; q < kCols; ++q) sum[q] = 0.f;
       }
-      if (key[u] < l.rows) {
+      if (key[u] != none) {
 #pragma unroll
         for (int q = 0; q < kCols; ++q) sum[q] += at8(row[u], q);
       }
     }
-    if (cur >= l.rows) return;  // only tokens without a row follow
+    if (cur == none) return;  // only tokens without a row follow
   }
   const bool tail = j1 < l.n && l.key(j1) == cur;
   if (head || tail) {
-    write8(part + (2 * ch + (head ? 0 : 1)) * d + c, left, sum);
+    write8<FULL>(part + (2 * ch + (head ? 0 : 1)) * d + c, left, sum);
   } else {
-    write_row(dw + static_cast<int64_t>(cur) * d + c, left, sum, scale, accumulate);
+    write_row<FULL>(dw + static_cast<int64_t>(cur) * d + c, left, sum, scale, accumulate);
   }
 }
 
@@ -368,31 +599,13 @@ __device__ __forceinline__ int64_t lower_bound(const Sorted& l, uint32_t k) {
   return lo;
 }
 
-constexpr int kZeroRows = 64;  // rows of a block that clears what no token touched
-
-// Blocks 0 .. chunks - 1 join the run that begins in that chunk and goes on behind it; further
-// blocks (a dense gradient) write zeros to the rows that no token has.
-template <typename T>
-__global__ void __launch_bounds__(kT) emb_bwd_join(Sorted l, const float* __restrict__ part, int d, int chunk,
-                                                   int64_t chunks, int lanes, float scale, T* __restrict__ dw,
-                                                   int accumulate) {
+// Block b joins the run that begins in chunk b and goes on behind it.
+template <typename T, bool FULL>
+__global__ void __launch_bounds__(kT) emb_bwd_join(Sorted l, const float* __restrict__ part, int d, int chunk, int lanes,
+                                                   float scale, T* __restrict__ dw, int accumulate) {
   __shared__ float buf[kT][kCols];
   const int tid = threadIdx.x, lane = tid % lanes, g = tid / lanes, groups = kT / lanes;
   const int c = (blockIdx.y * lanes + lane) * kCols, left = d - c;
-  if (blockIdx.x >= chunks) {
-    const int64_t r0 = (blockIdx.x - chunks) * kZeroRows;
-    const int64_t mine = r0 + (tid & 63);
-    bool empty = false;
-    if (mine < l.rows) {
-      const int64_t j = lower_bound(l, static_cast<uint32_t>(mine));
-      empty = j >= l.n || l.key(j) != mine;
-    }
-    const uint64_t rows = __ballot(empty);  // the same in all waves
-    const float zero[kCols] = {};
-    for (int r = g; r < kZeroRows; r += groups)
-      if (((rows >> r) & 1) && left > 0) write8(dw + (r0 + r) * d + c, left, zero);
-    return;
-  }
   const int64_t ch = blockIdx.x, j0 = ch * chunk, j1 = j0 + chunk;
   if (j1 >= l.n) return;
   const uint32_t k = l.key(j1);
@@ -404,7 +617,7 @@ __global__ void __launch_bounds__(kT) emb_bwd_join(Sorted l, const float* __rest
   if (left > 0) {
     for (int64_t m = ch + g; m <= last; m += groups) {
       Raw8<float> r;
-      read8(part + (2 * m + (m == ch ? 1 : 0)) * d + c, left, r);
+      read8<FULL>(part + (2 * m + (m == ch ? 1 : 0)) * d + c, left, r);
 #pragma unroll
       for (int q = 0; q < kCols; ++q) sum[q] += at8(r, q);
     }
@@ -417,11 +630,7 @@ __global__ void __launch_bounds__(kT) emb_bwd_join(Sorted l, const float* __rest
 #pragma unroll
     for (int q = 0; q < kCols; ++q) sum[q] += buf[m * lanes + lane][q];
   }
-  write_row(dw + static_cast<int64_t>(k) * d + c, left, sum, scale, accumulate);
-}
-
-bool packs(int64_t d, int64_t stride, const void* p, int es) {
-  return (d * es) % 16 == 0 && (stride * es) % 16 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+  write_row<FULL>(dw + static_cast<int64_t>(k) * d + c, left, sum, scale, accumulate);
 }
 
 }  // namespace
@@ -430,30 +639,27 @@ int embedding_fwd(int dt, const IndexList& ids, const void* w, int64_t w_stride,
                   const IndexList& pos, const void* p, int64_t p_stride, void* y, int64_t n, int64_t d,
                   hipStream_t s) {
   if (n <= 0 || d <= 0) return 0;
+  const int64_t per_row = (d + kCols - 1) / kCols;
+  const int64_t blocks = (n * per_row + kT * kPerThread - 1) / (kT * kPerThread);
+  if (blocks > 0x7fffffff || n > 0x7fffffff - kT * kPerThread) return -3;
+  const uint32_t reciprocal = per_row == 1 ? 0xffffffffu : static_cast<uint32_t>((1ull << 32) / per_row);
   SMPK_DISPATCH(dt, T, {
-    const int es = sizeof(T);
-    const bool vec = packs(d, w_stride, w, es) && packs(d, d, y, es) && (p == nullptr || packs(d, p_stride, p, es));
-    const int64_t items = n * (vec ? d / Vec16<T>::N : d);
-    const int64_t blocks = (items + kT - 1) / kT;
-    if (blocks > 0x7fffffff) return -3;
-    if (vec) {
-      emb_fwd<T, Vec16<T>::N><<<static_cast<unsigned>(blocks), kT, 0, s>>>(
-          ids, static_cast<const T*>(w), w_stride, scale, foreign_zero, pos, static_cast<const T*>(p), p_stride,
-          static_cast<T*>(y), n, static_cast<int>(d));
-    } else {
-      emb_fwd<T, 1><<<static_cast<unsigned>(blocks), kT, 0, s>>>(
-          ids, static_cast<const T*>(w), w_stride, scale, foreign_zero, pos, static_cast<const T*>(p), p_stride,
-          static_cast<T*>(y), n, static_cast<int>(d));
-    }
+    const auto kernel = d % kCols == 0 ? emb_fwd<T, true> : emb_fwd<T, false>;
+    kernel<<<static_cast<unsigned>(blocks), kT, 0, s>>>(ids, static_cast<const T*>(w), w_stride, scale, foreign_zero, pos,
+                                                       static_cast<const T*>(p), p_stride, static_cast<T*>(y),
+                                                       static_cast<int>(n), static_cast<int>(d),
+                                                       static_cast<uint32_t>(per_row), reciprocal);
   });
   return static_cast<int>(hipGetLastError());
 }
 
-EmbeddingPlan embedding_bwd_plan(int64_t n, int64_t d, int64_t rows, bool sorted) {
+EmbeddingPlan embedding_bwd_plan(int64_t n, int64_t d, int64_t rows, int64_t batch) {
+  const bool sorted = batch > 0;
   EmbeddingPlan p;
   int bits = 1;
   while ((rows >> bits) != 0) ++bits;  // the keys 0 .. rows
-  p.passes = sorted ? 0 : (bits + kMaxBits - 1) / kMaxBits;
+  const int most = n <= kShortSort ? kShortBits : kMaxBits;
+  p.passes = sorted ? 0 : (bits + most - 1) / most;
   p.bits = sorted ? 0 : (bits + p.passes - 1) / p.passes;
   // one block sorts a short list alone, in one launch; longer ones go in runs of 2048 tokens or,
   // above 256 blocks, whose counts every block reads, in longer runs
@@ -462,6 +668,9 @@ EmbeddingPlan embedding_bwd_plan(int64_t n, int64_t d, int64_t rows, bool sorted
   p.sort_blocks = n > 0 ? (n + p.per_block - 1) / p.per_block : 0;
   int64_t c = 16;  // tokens of a chunk: long ones leave fewer partial sums, short ones more to run at once
   while (c < 64 && n / (c * 2) >= 1024) c *= 2;
+  // positions of up to 64 sequences: whole runs in a chunk, which leave nothing to join
+  p.join = !(sorted && batch <= 64);
+  if (!p.join) c = c < batch ? batch : c / batch * batch;
   p.chunk = static_cast<int>(c);
   p.chunks = (n + c - 1) / c;
   return p;
@@ -469,7 +678,7 @@ EmbeddingPlan embedding_bwd_plan(int64_t n, int64_t d, int64_t rows, bool sorted
 
 int embedding_bwd(int dt, const IndexList& ids, const void* dy, int64_t n, int64_t d, float scale, int64_t skip,
                   void* dw, int accumulate, const EmbeddingPlan& p, uint32_t* keys, int32_t* tokens, int32_t* counts,
-                  float* part, hipStream_t s) {
+                  float* part, uint8_t* marks, hipStream_t s) {
   if (ids.rows <= 0 || d <= 0 || (n <= 0 && accumulate)) return 0;
   Sorted l{nullptr, nullptr, n, ids.rows, ids.period > 0 ? n / ids.period : 1, ids.period};
   if (ids.ids != nullptr && n > 0) {
@@ -484,8 +693,13 @@ int embedding_bwd(int dt, const IndexList& ids, const void* dy, int64_t n, int64
     a.bits = p.bits;
     a.keys_out = keys;
     a.tokens_out = tokens;
+    a.marks = accumulate ? nullptr : marks;
     if (p.sort_blocks == 1) {
-      emb_sort_short<<<1, kSortThreads, 0, s>>>(a, keys + n, tokens + n, p.passes);
+      const auto kernel = n <= 2 * kSortThreads   ? emb_sort_short<2>
+                          : n <= 4 * kSortThreads ? emb_sort_short<4>
+                          : n <= 8 * kSortThreads ? emb_sort_short<8>
+                                                  : emb_sort_short<16>;
+      kernel<<<1, kSortThreads, 0, s>>>(a, p.passes);
     } else {
       for (int q = 0; q < p.passes; ++q) {
         const int to = (p.passes - 1 - q) & 1;
@@ -503,19 +717,33 @@ int embedding_bwd(int dt, const IndexList& ids, const void* dy, int64_t n, int64
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return static_cast<int>(e);
   }
-  int lanes = 1;
+  int lanes = 1;  // of a narrow chunk, and of a joining block's column slab
   while (lanes < kT && lanes * kCols < d) lanes *= 2;
-  const unsigned slabs = static_cast<unsigned>((d + lanes * kCols - 1) / (lanes * kCols));
-  const int64_t per = kT / lanes, zero = accumulate ? 0 : (ids.rows + kZeroRows - 1) / kZeroRows;
-  if (slabs > 65535 || p.chunks + zero > 0x7fffffff) return -3;
+  const int64_t slabs = (d + 64 * kCols - 1) / (64 * kCols), join_slabs = (d + lanes * kCols - 1) / (lanes * kCols);
+  const int64_t zero = accumulate ? 0 : (ids.rows + kZeroRows - 1) / kZeroRows * slabs;
+  const bool wide = lanes >= 64, full = d % kCols == 0;
+  const int64_t units = wide ? kT / 64 : kT / lanes;
+  const int64_t blocks = ((wide ? p.chunks * slabs : p.chunks) + units - 1) / units;
+  if (blocks + zero > 0x7fffffff || join_slabs > 65535) return -3;
+  const uint8_t* flags = l.keys != nullptr ? marks : nullptr;
   SMPK_DISPATCH(dt, T, {
-    if (p.chunks > 0)
-      emb_bwd_chunks<T><<<dim3(static_cast<unsigned>((p.chunks + per - 1) / per), slabs), kT, 0, s>>>(
-          l, static_cast<const T*>(dy), static_cast<int>(d), p.chunk, lanes, scale, static_cast<T*>(dw), accumulate,
-          part);
-    if (p.chunks + zero > 0)
-      emb_bwd_join<T><<<dim3(static_cast<unsigned>(p.chunks + zero), slabs), kT, 0, s>>>(
-          l, part, static_cast<int>(d), p.chunk, p.chunks, lanes, scale, static_cast<T*>(dw), accumulate);
+    if (blocks + zero > 0) {
+      const unsigned grid = static_cast<unsigned>(blocks + zero);
+      if (wide) {
+        const auto kernel = full ? emb_bwd_wide<T, true> : emb_bwd_wide<T, false>;
+        kernel<<<grid, kT, 0, s>>>(l, static_cast<const T*>(dy), static_cast<int>(d), p.chunk, static_cast<int>(slabs),
+                                   blocks, scale, static_cast<T*>(dw), accumulate, part, flags);
+      } else {
+        const auto kernel = full ? emb_bwd_narrow<T, true> : emb_bwd_narrow<T, false>;
+        kernel<<<grid, kT, 0, s>>>(l, static_cast<const T*>(dy), static_cast<int>(d), p.chunk, lanes, blocks, scale,
+                                   static_cast<T*>(dw), accumulate, part, flags);
+      }
+    }
+    if (p.join && p.chunks > 1) {
+      const auto kernel = full ? emb_bwd_join<T, true> : emb_bwd_join<T, false>;
+      kernel<<<dim3(static_cast<unsigned>(p.chunks), static_cast<unsigned>(join_slabs)), kT, 0, s>>>(
+          l, part, static_cast<int>(d), p.chunk, lanes, scale, static_cast<T*>(dw), accumulate);
+    }
   });
   return static_cast<int>(hipGetLastError());
 }

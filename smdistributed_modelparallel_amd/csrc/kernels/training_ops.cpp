@@ -86,16 +86,18 @@ void embedding_bwd(at::Tensor dy, c10::optional<at::Tensor> ids, int64_t period,
   const auto li = index_list(ids, n, start, dw.size(0), period, dw);
   TORCH_CHECK(ids.has_value() || (period >= 1 && n % period == 0 && period <= dw.size(0)),
               "embedding: the tokens are no whole sequences of positions");
-  const auto p = smpk::embedding_bwd_plan(n, d, dw.size(0), !ids.has_value());
+  const auto p = smpk::embedding_bwd_plan(n, d, dw.size(0), ids.has_value() ? 0 : std::max<int64_t>(n / period, 1));
   const auto i32 = dw.options().dtype(at::kInt);
   const bool sort = ids.has_value() && n > 0;
   auto order = at::empty({sort ? 4 * n : 0}, i32);
   auto counts = at::empty({sort && p.sort_blocks > 1 ? p.sort_blocks << p.bits : 0}, i32);
-  auto part = at::empty({p.chunks * 2 * d}, dw.options().dtype(at::kFloat));
+  auto part = at::empty({p.join ? p.chunks * 2 * d : 0}, dw.options().dtype(at::kFloat));
+  auto marks = at::empty({sort && !accumulate ? (dw.size(0) + 15) / 16 * 16 : 0}, dw.options().dtype(at::kByte));
   int32_t* const o = order.data_ptr<int32_t>();
   check(smpk::embedding_bwd(dt_code(dw, "weight"), li, dy.data_ptr(), n, d, static_cast<float>(scale), skip,
                             dw.data_ptr(), accumulate ? 1 : 0, p, reinterpret_cast<uint32_t*>(o),
-                            sort ? o + 2 * n : o, counts.data_ptr<int32_t>(), part.data_ptr<float>(), stream()),
+                            sort ? o + 2 * n : o, counts.data_ptr<int32_t>(), part.data_ptr<float>(),
+                            marks.data_ptr<uint8_t>(), stream()),
         "embedding_bwd");
 }
 
