@@ -16,78 +16,40 @@
 // it has to read x in any case, and s in 16 bits would cost the fp32 weight gradients 1e-3 of
 // their value.
 //
-// A thread holds kN = 8 consecutive elements of a row (times V for the widest rows); a team of
-// threads, a multiple of 64, holds the row.  Rows of odd widths start off 16 bytes: the hardware
-// loads and stores 16 bytes at any address, so only the last, partial vector of a row goes
-// element by element.
-#include "common.h"
+// A thread holds 8 consecutive elements of a row (V times that for wide rows).  Forward, rows of up
+// to 2048 elements belong to one wave each: no barrier, and the rows of a CU's waves overlap freely.
+// Wider rows, and all rows of the backward, belong to a team of waves.
 #include "kernels.h"
+#include "vec8.h"
 
 namespace smpk {
 namespace {
 
-constexpr int kN = 8;
-
-template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Unaligned16 {
-  T v[16 / sizeof(T)];
-};
-
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int left, float (&o)[kN]) {
-  if (left >= kN) {
-    constexpr int M = 16 / sizeof(T);
-#pragma unroll
-    for (int k = 0; k < kN; k += M) {
-      Unaligned16<T> a;
-      __builtin_memcpy(&a, p + k, 16);
-#pragma unroll
-      for (int j = 0; j < M; ++j) o[k + j] = to_f32(a.v[j]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < kN; ++j) o[j] = j < left ? to_f32(p[j]) : 0.f;
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void store8(T* p, int left, const float (&o)[kN]) {
-  if (left >= kN) {
-    constexpr int M = 16 / sizeof(T);
-#pragma unroll
-    for (int k = 0; k < kN; k += M) {
-      Unaligned16<T> a;
-#pragma unroll
-      for (int j = 0; j < M; ++j) a.v[j] = from_f32<T>(o[k + j]);
-      __builtin_memcpy(p + k, &a, 16);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < kN; ++j)
-      if (j < left) p[j] = from_f32<T>(o[j]);
-  }
+template <bool FULL>
+__device__ __forceinline__ bool in_row(int j, int left) {
+  return FULL || j < left;
 }
 
 // A vector that may be absent (`other` then) and of either T or fp32.
-template <typename T>
-__device__ __forceinline__ void load_opt(const void* p, bool f32, int64_t at, int left, float other, float (&o)[kN]) {
+template <bool FULL, typename T>
+__device__ __forceinline__ void read_opt(const void* p, bool f32, int64_t at, int left, float other, float (&o)[kCols]) {
   if (p == nullptr) {
 #pragma unroll
-    for (int j = 0; j < kN; ++j) o[j] = other;
+    for (int j = 0; j < kCols; ++j) o[j] = other;
   } else if (f32) {
-    load8(static_cast<const float*>(p) + at, left, o);
+    read8<FULL>(static_cast<const float*>(p) + at, left, o);
   } else {
-    load8(static_cast<const T*>(p) + at, left, o);
+    read8<FULL>(static_cast<const T*>(p) + at, left, o);
   }
 }
 
-// Sums of two values over a team of `waves` waves; `slot` alternates so that one barrier suffices.
+// Sums over a team of `waves` waves; `slot` alternates so that one barrier suffices.
 struct Team {
   float* smem;  // [2][2][16]
   int first, waves, slot;
   __device__ __forceinline__ void sum2(float& a, float& b) {
-    a = wave_sum(a);
-    b = wave_sum(b);
+    a = wave_sum_fixed(a);
+    b = wave_sum_fixed(b);
     if (waves == 1) return;
     float* s = smem + slot * 32;
     slot ^= 1;
@@ -102,87 +64,107 @@ struct Team {
       b += s[16 + first + k];
     }
   }
+  __device__ __forceinline__ void sum1(float& a) {
+    a = wave_sum_fixed(a);
+    if (waves == 1) return;
+    float* s = smem + slot * 32;
+    slot ^= 1;
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = a;
+    __syncthreads();
+    a = 0.f;
+    for (int k = 0; k < waves; ++k) a += s[first + k];
+  }
 };
 
-template <int V>
-__device__ __forceinline__ void moments(const float (&v)[V][kN], const int (&left)[V], int d, float eps, bool rms,
+// Mean, then the mean square of the differences: values of any offset keep their deviation.
+template <int V, bool FULL>
+__device__ __forceinline__ void moments(const float (&v)[V][kCols], const int (&left)[V], int d, float eps, bool rms,
                                         Team& team, float& mean, float& rstd) {
   mean = 0.f;
-  float unused = 0.f;
   if (!rms) {
     float a = 0.f;
 #pragma unroll
     for (int k = 0; k < V; ++k)
 #pragma unroll
-      for (int j = 0; j < kN; ++j) a += v[k][j];  // (zero past the row's end)
-    team.sum2(a, unused);
+      for (int j = 0; j < kCols; ++j) a += v[k][j];  // (zero past the row's end)
+    team.sum1(a);
     mean = a / d;
   }
   float q = 0.f;
 #pragma unroll
-  for (int k = 0; k < V; ++k)
+  for (int k = 0; k < V; ++k) {
+    if (left[k] <= 0) continue;
 #pragma unroll
-    for (int j = 0; j < kN; ++j) {
-      const float c = j < left[k] ? v[k][j] - mean : 0.f;
+    for (int j = 0; j < kCols; ++j) {
+      const float c = in_row<FULL>(j, left[k]) ? v[k][j] - mean : 0.f;
       q = fmaf(c, c, q);
     }
-  team.sum2(q, unused);
+  }
+  team.sum1(q);
   rstd = rsqrtf(q / d + eps);
 }
 
-template <typename T, int V>
+// team_size threads for a row: 64 (and blockDim.x / 64 rows a block), or all of the block
+template <typename T, int V, bool FULL>
 __global__ void __launch_bounds__(1024) block_norm_fwd(BlockNormArgs a, int team_size) {
   __shared__ float smem[64];
-  const int tid = threadIdx.x, teams = blockDim.x / team_size, lane = tid % team_size, tm = tid / team_size;
-  Team team{smem, tm * (team_size / 64), team_size / 64, 0};
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * teams + tm;
-  const bool live = row < a.rows;  // a team past the end only joins the barriers
+  const int tid = threadIdx.x, lane = team_size == 64 ? tid & 63 : tid;
+  Team team{smem, 0, team_size / 64, 0};
+  const int64_t row = team_size == 64
+                          ? static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 6) + __builtin_amdgcn_readfirstlane(tid >> 6)
+                          : blockIdx.x;
+  if (row >= a.rows) return;  // (whole waves of their own rows: no barrier follows for them)
   int left[V];
-  float s[V][kN], h[V][kN];
+  float s[V][kCols], h[V][kCols];
+  Raw8<T> rs[V], rh[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    const int c = (k * team_size + lane) * kN;
-    left[k] = live ? a.d - c : 0;
-#pragma unroll
-    for (int j = 0; j < kN; ++j) s[k][j] = h[k][j] = 0.f;
-    if (left[k] > 0) {
-      load8(static_cast<const T*>(a.res) + row * a.d + c, left[k], s[k]);
-      if (a.x != nullptr) load8(static_cast<const T*>(a.x) + row * a.d + c, left[k], h[k]);
-    }
+    const int c = (k * team_size + lane) * kCols;
+    left[k] = a.d - c;
+    if (left[k] <= 0) continue;
+    if (a.x != nullptr) read8<FULL>(static_cast<const T*>(a.x) + row * a.d + c, left[k], rh[k]);
+    read8<FULL>(static_cast<const T*>(a.res) + row * a.d + c, left[k], rs[k]);
   }
+#pragma unroll
+  for (int k = 0; k < V; ++k)
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) {
+      h[k][j] = left[k] > 0 && a.x != nullptr ? at8(rh[k], j) : 0.f;
+      s[k][j] = left[k] > 0 ? at8(rs[k], j) : 0.f;
+    }
   float mean2 = 0.f, rstd2 = 1.f, mean1, rstd1;
   if (a.x != nullptr) {
-    if (a.pw != nullptr) moments(h, left, a.d, a.eps, a.rms, team, mean2, rstd2);
-    const int64_t gate_row = a.gate != nullptr && live ? row / a.gate_rows * a.d : 0;
+    if (a.pw != nullptr) moments<V, FULL>(h, left, a.d, a.eps, a.rms, team, mean2, rstd2);
+    const int64_t gate_row = a.gate != nullptr ? row / a.gate_rows * a.d : 0;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const int c = (k * team_size + lane) * kN;
+      const int c = (k * team_size + lane) * kCols;
       if (left[k] <= 0) continue;
-      float w[kN], b[kN], g[kN];
-      load_opt<T>(a.pw, a.w_f32, c, left[k], 1.f, w);
-      load_opt<T>(a.pb, a.w_f32, c, left[k], 0.f, b);
-      load_opt<T>(a.gate, a.gate_f32, gate_row + c, left[k], 1.f, g);
+      float w[kCols], b[kCols], g[kCols];
+      read_opt<FULL, T>(a.pw, a.w_f32, c, left[k], 1.f, w);
+      read_opt<FULL, T>(a.pb, a.w_f32, c, left[k], 0.f, b);
+      read_opt<FULL, T>(a.gate, a.gate_f32, gate_row + c, left[k], 1.f, g);
 #pragma unroll
-      for (int j = 0; j < kN; ++j) {
+      for (int j = 0; j < kCols; ++j) {
         const float v = fmaf((h[k][j] - mean2) * rstd2, w[j], b[j]);
-        s[k][j] = j < left[k] ? fmaf(a.alpha * g[j], v, s[k][j]) : 0.f;
+        s[k][j] = in_row<FULL>(j, left[k]) ? fmaf(a.alpha * g[j], v, s[k][j]) : 0.f;
       }
-      store8(static_cast<T*>(a.s) + row * a.d + c, left[k], s[k]);
+      write8<FULL, true>(static_cast<T*>(a.s) + row * a.d + c, left[k], s[k]);
     }
   }
-  moments(s, left, a.d, a.eps, a.rms, team, mean1, rstd1);
-  if (live && lane == 0 && a.stats != nullptr)
+  moments<V, FULL>(s, left, a.d, a.eps, a.rms, team, mean1, rstd1);
+  if (lane == 0 && a.stats != nullptr)
     reinterpret_cast<float4*>(a.stats)[row] = make_float4(mean1, rstd1, mean2, rstd2);
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    const int c = (k * team_size + lane) * kN;
+    const int c = (k * team_size + lane) * kCols;
     if (left[k] <= 0) continue;
-    float w[kN], b[kN];
-    load_opt<T>(a.w, a.w_f32, c, left[k], 1.f, w);
-    load_opt<T>(a.b, a.w_f32, c, left[k], 0.f, b);
+    float w[kCols], b[kCols];
+    read_opt<FULL, T>(a.w, a.w_f32, c, left[k], 1.f, w);
+    read_opt<FULL, T>(a.b, a.w_f32, c, left[k], 0.f, b);
 #pragma unroll
-    for (int j = 0; j < kN; ++j) w[j] = fmaf((s[k][j] - mean1) * rstd1, w[j], b[j]);
-    store8(static_cast<T*>(a.y) + row * a.d + c, left[k], w);
+    for (int j = 0; j < kCols; ++j) w[j] = fmaf((s[k][j] - mean1) * rstd1, w[j], b[j]);
+    write8<FULL, true>(static_cast<T*>(a.y) + row * a.d + c, left[k], w);
   }
 }
 
@@ -214,62 +196,113 @@ __device__ __forceinline__ Turn turn_of(const BlockNormArgs& a, int64_t unit, in
 
 enum { kW1, kB1, kW2, kB2, kG, kSums };
 
+// A row's loads, issued while the row before is worked on.
 template <typename T, int V>
-__global__ void __launch_bounds__(1024) block_norm_bwd(BlockNormArgs a, int team_size, int64_t iterations) {
-  extern __shared__ float lds[];  // [64] reductions, then [team_size * kN * V] to join the teams' sums
+struct RowData {
+  Raw8<T> x[V], res[V], dy[V], ds[V];
+  float4 st;
+};
+
+template <typename T, int V, bool FULL>
+__device__ __forceinline__ void fetch(const BlockNormArgs& a, const Turn& t, int team_size, int lane, RowData<T, V>& r) {
+  if (!t.live) return;
+  r.st = reinterpret_cast<const float4*>(a.stats)[t.row];
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const int c = (k * team_size + lane) * kCols, left = a.d - c;
+    if (left <= 0) continue;
+    const int64_t at = t.row * a.d + c;
+    read8<FULL>(static_cast<const T*>(a.res) + at, left, r.res[k]);
+    if (a.x != nullptr) read8<FULL>(static_cast<const T*>(a.x) + at, left, r.x[k]);
+    if (a.dy != nullptr) read8<FULL>(static_cast<const T*>(a.dy) + at, left, r.dy[k]);
+    if (a.ds != nullptr) read8<FULL>(static_cast<const T*>(a.ds) + at, left, r.ds[k]);
+  }
+}
+
+// The weights stay in registers, in their own type W (T or fp32): a unit works on many rows.
+template <typename T, typename W, int V, bool FULL, int THREADS>
+__global__ void __launch_bounds__(THREADS) block_norm_bwd(BlockNormArgs a, int team_size, int64_t iterations) {
+  extern __shared__ float lds[];  // [64] reductions, then [team_size * kCols * V] to join the teams' sums
   const int tid = threadIdx.x, teams = blockDim.x / team_size, lane = tid % team_size, tm = tid / team_size;
   Team team{lds, tm * (team_size / 64), team_size / 64, 0};
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * teams + tm, units = static_cast<int64_t>(gridDim.x) * teams;
-  float sum[kSums][V][kN];
+  float sum[kSums][V][kCols];
+  Raw8<W> w[V], pw[V], pb[V];
+  float ag[V][kCols];  // alpha * gate
+  int left[V];
 #pragma unroll
-  for (int q = 0; q < kSums; ++q)
+  for (int k = 0; k < V; ++k) {
+    const int c = (k * team_size + lane) * kCols;
+    left[k] = a.d - c;
 #pragma unroll
-    for (int k = 0; k < V; ++k)
+    for (int j = 0; j < kCols; ++j) {
+      w[k].v[j] = pw[k].v[j] = from_f32<W>(1.f);
+      pb[k].v[j] = from_f32<W>(0.f);
+      ag[k][j] = a.alpha;
+    }
+    if (left[k] > 0) {
+      read8<FULL>(static_cast<const W*>(a.w) + c, left[k], w[k]);
+      if (a.pw != nullptr) read8<FULL>(static_cast<const W*>(a.pw) + c, left[k], pw[k]);
+      if (a.pb != nullptr) read8<FULL>(static_cast<const W*>(a.pb) + c, left[k], pb[k]);
+    }
 #pragma unroll
-      for (int j = 0; j < kN; ++j) sum[q][k][j] = 0.f;
+    for (int q = 0; q < kSums; ++q)
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) sum[q][k][j] = 0.f;
+  }
+  int64_t gate_now = -1;
+  RowData<T, V> r;
+  Turn t = turn_of(a, unit, units, 0);
+  fetch<T, V, FULL>(a, t, team_size, lane, r);
 
   for (int64_t i = 0; i < iterations; ++i) {
-    const Turn t = turn_of(a, unit, units, i);
-    float n1[V][kN], n2[V][kN], dy[V][kN], ds[V][kN];
-    int left[V];
-    float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (t.live) st = reinterpret_cast<const float4*>(a.stats)[t.row];
+    if (a.gate != nullptr && t.live && t.gate != gate_now) {
+      gate_now = t.gate;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const int c = (k * team_size + lane) * kCols;
+        if (left[k] <= 0) continue;
+        read_opt<FULL, T>(a.gate, a.gate_f32, t.gate * a.d + c, left[k], 1.f, ag[k]);
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) ag[k][j] *= a.alpha;
+      }
+    }
+    float n1[V][kCols], n2[V][kCols], dy[V][kCols], ds[V][kCols];
+    const float4 st = r.st;
     float p = 0.f, q = 0.f;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const int c = (k * team_size + lane) * kN;
-      left[k] = t.live ? a.d - c : 0;
+      if (left[k] <= 0 || !t.live) continue;
 #pragma unroll
-      for (int j = 0; j < kN; ++j) n1[k][j] = n2[k][j] = dy[k][j] = ds[k][j] = 0.f;
-      if (left[k] <= 0) continue;
-      const int64_t at = t.row * a.d + c;
-      float w[kN], b[kN], g[kN], pw[kN];
-      load8(static_cast<const T*>(a.res) + at, left[k], n1[k]);
-      if (a.ds != nullptr) load8(static_cast<const T*>(a.ds) + at, left[k], ds[k]);
+      for (int j = 0; j < kCols; ++j) {
+        n1[k][j] = at8(r.res[k], j);
+        n2[k][j] = 0.f;
+        ds[k][j] = a.ds != nullptr ? at8(r.ds[k], j) : 0.f;
+      }
       if (a.x != nullptr) {
-        load8(static_cast<const T*>(a.x) + at, left[k], n2[k]);
-        load_opt<T>(a.pw, a.w_f32, c, left[k], 1.f, pw);
-        load_opt<T>(a.pb, a.w_f32, c, left[k], 0.f, b);
-        load_opt<T>(a.gate, a.gate_f32, t.gate * a.d + c, left[k], 1.f, g);
 #pragma unroll
-        for (int j = 0; j < kN; ++j) {
-          n2[k][j] = j < left[k] ? (n2[k][j] - st.z) * st.w : 0.f;
-          n1[k][j] = fmaf(a.alpha * g[j], fmaf(n2[k][j], pw[j], b[j]), n1[k][j]);
+        for (int j = 0; j < kCols; ++j) {
+          n2[k][j] = in_row<FULL>(j, left[k]) ? (at8(r.x[k], j) - st.z) * st.w : 0.f;
+          n1[k][j] = fmaf(ag[k][j], fmaf(n2[k][j], at8(pw[k], j), at8(pb[k], j)), n1[k][j]);
         }
       }
       if (a.dy != nullptr) {
-        load8(static_cast<const T*>(a.dy) + at, left[k], dy[k]);
-        load_opt<T>(a.w, a.w_f32, c, left[k], 1.f, w);
 #pragma unroll
-        for (int j = 0; j < kN; ++j) {
-          n1[k][j] = j < left[k] ? (n1[k][j] - st.x) * st.y : 0.f;
-          sum[kW1][k][j] = fmaf(dy[k][j], n1[k][j], sum[kW1][k][j]);
-          sum[kB1][k][j] += dy[k][j];
-          dy[k][j] *= w[j];
+        for (int j = 0; j < kCols; ++j) {
+          const float g = at8(r.dy[k], j);
+          n1[k][j] = in_row<FULL>(j, left[k]) ? (n1[k][j] - st.x) * st.y : 0.f;
+          sum[kW1][k][j] = fmaf(g, n1[k][j], sum[kW1][k][j]);
+          sum[kB1][k][j] += g;
+          dy[k][j] = g * at8(w[k], j);
           p += dy[k][j];
           q = fmaf(dy[k][j], n1[k][j], q);
         }
       }
+    }
+    const Turn now = t;
+    if (i + 1 < iterations) {
+      t = turn_of(a, unit, units, i + 1);
+      fetch<T, V, FULL>(a, t, team_size, lane, r);
     }
     if (a.dy != nullptr) {
       team.sum2(p, q);
@@ -279,28 +312,22 @@ __global__ void __launch_bounds__(1024) block_norm_bwd(BlockNormArgs a, int team
     float u = 0.f, v = 0.f;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const int c = (k * team_size + lane) * kN;
-      if (left[k] <= 0) continue;
-      const int64_t at = t.row * a.d + c;
+      if (left[k] <= 0 || !now.live) continue;
+      const int64_t at = now.row * a.d + (k * team_size + lane) * kCols;
       if (a.dy != nullptr) {
 #pragma unroll
-        for (int j = 0; j < kN; ++j)
-          ds[k][j] = fmaf(st.y, dy[k][j] - p - n1[k][j] * q, ds[k][j]);
+        for (int j = 0; j < kCols; ++j) ds[k][j] = fmaf(st.y, dy[k][j] - p - n1[k][j] * q, ds[k][j]);
       }
-      if (a.dres != nullptr) store8(static_cast<T*>(a.dres) + at, left[k], ds[k]);
+      if (a.dres != nullptr) write8<FULL, true>(static_cast<T*>(a.dres) + at, left[k], ds[k]);
       if (a.x == nullptr) continue;
-      float b[kN], g[kN], pw[kN];
-      load_opt<T>(a.pw, a.w_f32, c, left[k], 1.f, pw);
-      load_opt<T>(a.pb, a.w_f32, c, left[k], 0.f, b);
-      load_opt<T>(a.gate, a.gate_f32, t.gate * a.d + c, left[k], 1.f, g);
 #pragma unroll
-      for (int j = 0; j < kN; ++j) {
-        const float as = j < left[k] ? a.alpha * ds[k][j] : 0.f;
-        sum[kG][k][j] = fmaf(as, fmaf(n2[k][j], pw[j], b[j]), sum[kG][k][j]);
-        const float dh = as * g[j];
+      for (int j = 0; j < kCols; ++j) {
+        const float s = in_row<FULL>(j, left[k]) ? ds[k][j] : 0.f;
+        sum[kG][k][j] = fmaf(s, fmaf(n2[k][j], at8(pw[k], j), at8(pb[k], j)), sum[kG][k][j]);
+        const float dh = s * ag[k][j];
         sum[kW2][k][j] = fmaf(dh, n2[k][j], sum[kW2][k][j]);
         sum[kB2][k][j] += dh;
-        ds[k][j] = dh * pw[j];  // the gradient of n2; of x itself without a norm
+        ds[k][j] = dh * at8(pw[k], j);  // the gradient of n2; of x itself without a norm
         u += ds[k][j];
         v = fmaf(ds[k][j], n2[k][j], v);
       }
@@ -314,21 +341,23 @@ __global__ void __launch_bounds__(1024) block_norm_bwd(BlockNormArgs a, int team
     }
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const int c = (k * team_size + lane) * kN;
-      if (left[k] <= 0 || a.x == nullptr) continue;
+      const int c = (k * team_size + lane) * kCols;
+      if (left[k] <= 0 || !now.live || a.x == nullptr) continue;
       if (a.dx != nullptr) {
 #pragma unroll
-        for (int j = 0; j < kN; ++j) ds[k][j] = st.w * (ds[k][j] - u - n2[k][j] * v);
-        store8(static_cast<T*>(a.dx) + t.row * a.d + c, left[k], ds[k]);
+        for (int j = 0; j < kCols; ++j) ds[k][j] = st.w * (ds[k][j] - u - n2[k][j] * v);
+        write8<FULL, true>(static_cast<T*>(a.dx) + now.row * a.d + c, left[k], ds[k]);
       }
-      if (a.gate_direct && t.last) {  // a whole gate row's sum is complete
+      if (a.gate_direct && now.last) {  // a whole gate row's sum is complete
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) sum[kG][k][j] *= a.alpha;
         if (a.gate_f32) {
-          store8(static_cast<float*>(a.dgate) + t.gate * a.d + c, left[k], sum[kG][k]);
+          write8<FULL, true>(static_cast<float*>(a.dgate) + now.gate * a.d + c, left[k], sum[kG][k]);
         } else {
-          store8(static_cast<T*>(a.dgate) + t.gate * a.d + c, left[k], sum[kG][k]);
+          write8<FULL, true>(static_cast<T*>(a.dgate) + now.gate * a.d + c, left[k], sum[kG][k]);
         }
 #pragma unroll
-        for (int j = 0; j < kN; ++j) sum[kG][k][j] = 0.f;
+        for (int j = 0; j < kCols; ++j) sum[kG][k][j] = 0.f;
       }
     }
   }
@@ -336,8 +365,10 @@ __global__ void __launch_bounds__(1024) block_norm_bwd(BlockNormArgs a, int team
   // partial sums: of the teams together for the vectors, of each unit for its gate row
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    const int c = (k * team_size + lane) * kN;
-    if (a.gate_part != nullptr && c < a.d) store8(a.gate_part + unit * a.d + c, a.d - c, sum[kG][k]);
+    const int c = (k * team_size + lane) * kCols;
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) sum[kG][k][j] *= a.alpha;
+    if (a.gate_part != nullptr && c < a.d) write8<FULL, false>(a.gate_part + unit * a.d + c, a.d - c, sum[kG][k]);
   }
 #pragma unroll
   for (int q = 0; q < kSums; ++q) {
@@ -349,38 +380,42 @@ __global__ void __launch_bounds__(1024) block_norm_bwd(BlockNormArgs a, int team
 #pragma unroll
         for (int k = 0; k < V; ++k)
 #pragma unroll
-          for (int j = 0; j < kN; ++j) buf[(k * kN + j) * team_size + lane] = sum[q][k][j];
+          for (int j = 0; j < kCols; ++j) buf[(k * kCols + j) * team_size + lane] = sum[q][k][j];
       }
       __syncthreads();
       if (tm == 0) {
 #pragma unroll
         for (int k = 0; k < V; ++k)
 #pragma unroll
-          for (int j = 0; j < kN; ++j) sum[q][k][j] += buf[(k * kN + j) * team_size + lane];
+          for (int j = 0; j < kCols; ++j) sum[q][k][j] += buf[(k * kCols + j) * team_size + lane];
       }
     }
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const int c = (k * team_size + lane) * kN;
-      if (tm == 0 && c < a.d) store8(a.part[q] + static_cast<int64_t>(blockIdx.x) * a.d + c, a.d - c, sum[q][k]);
+      const int c = (k * team_size + lane) * kCols;
+      if (tm == 0 && c < a.d)
+        write8<FULL, false>(a.part[q] + static_cast<int64_t>(blockIdx.x) * a.d + c, a.d - c, sum[q][k]);
     }
   }
 }
 
-// out[g][c] = (or +=) the sum over `split` partial rows; 64 columns x 16 row groups a block
+// out[g][c] = (or +=) the sum over `split` partial rows; 32 columns x 32 row groups a block
 __global__ void __launch_bounds__(1024) block_norm_join(BlockNormJoin l, int d) {
-  __shared__ float buf[16][64];
+  __shared__ float buf[32][33];
   const BlockNormJoin::Item& it = l.item[blockIdx.y];
   const int64_t g = blockIdx.z;
   if (g >= it.groups) return;
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), r = threadIdx.x >> 6;
+  const int x = threadIdx.x & 31, r = threadIdx.x >> 5, c = blockIdx.x * 32 + x;
   float v = 0.f;
-  if (c < d)
-    for (int64_t k = r; k < it.split; k += 16) v += it.part[(g * it.split + k) * d + c];
-  buf[r][threadIdx.x & 63] = v;
+  if (c < d) {
+#pragma unroll 4
+    for (int64_t k = r; k < it.split; k += 32) v += it.part[(g * it.split + k) * d + c];
+  }
+  buf[r][x] = v;
   __syncthreads();
   if (r != 0 || c >= d) return;
-  for (int k = 1; k < 16; ++k) v += buf[k][threadIdx.x];
+#pragma unroll
+  for (int k = 1; k < 32; ++k) v += buf[k][x];
   const int64_t at = g * d + c;
   switch (it.dt) {
     case F32: {
@@ -400,40 +435,43 @@ __global__ void __launch_bounds__(1024) block_norm_join(BlockNormJoin l, int d) 
   }
 }
 
-// threads of a team and vectors a thread holds; false: the row is too wide
-bool team_for(int64_t d, int& team, int& v) {
-  const int64_t vectors = (d + kN - 1) / kN;
-  v = vectors <= 1024 ? 1 : 2;
-  const int64_t t = ((vectors + v - 1) / v + 63) / 64 * 64;
-  team = static_cast<int>(t);
-  return t <= 1024;
+// Teams of the backward: one vector a thread up to 4096 elements, two beyond.
+int team_of(int64_t d, int& v) {
+  const int64_t vectors = (d + kCols - 1) / kCols;
+  v = vectors <= 512 ? 1 : 2;
+  return static_cast<int>(((vectors + v - 1) / v + 63) / 64 * 64);
 }
+
+constexpr int64_t kMaxWidth = 16384;
 
 }  // namespace
 
 int block_norm_fwd(int dt, const BlockNormArgs& a, hipStream_t s) {
-  int team, v;
-  if (!team_for(a.d, team, v)) return -4;
+  if (a.d < 1 || a.d > kMaxWidth) return -4;
   if (a.rows <= 0) return 0;
-  const int teams = team >= 256 ? 1 : 256 / team;
-  const int64_t blocks = (a.rows + teams - 1) / teams;
+  const int64_t vectors = (a.d + kCols - 1) / kCols;
+  const bool wave = vectors <= 256;
+  const int v = vectors <= 64 ? 1 : vectors <= 128 ? 2 : wave ? 4 : vectors <= 1024 ? 1 : 2;
+  const int team = wave ? 64 : static_cast<int>(((vectors + v - 1) / v + 63) / 64 * 64);
+  const int64_t blocks = wave ? (a.rows + 3) / 4 : a.rows;
   if (blocks > 0x7fffffff) return -3;
   SMPK_DISPATCH(dt, T, {
-    if (v == 1) {
-      block_norm_fwd<T, 1><<<static_cast<unsigned>(blocks), team * teams, 0, s>>>(a, team);
-    } else {
-      block_norm_fwd<T, 2><<<static_cast<unsigned>(blocks), team * teams, 0, s>>>(a, team);
-    }
+    const bool full = a.d % kCols == 0;
+    const auto kernel = v == 1   ? (full ? block_norm_fwd<T, 1, true> : block_norm_fwd<T, 1, false>)
+                        : v == 2 ? (full ? block_norm_fwd<T, 2, true> : block_norm_fwd<T, 2, false>)
+                                 : (full ? block_norm_fwd<T, 4, true> : block_norm_fwd<T, 4, false>);
+    kernel<<<static_cast<unsigned>(blocks), wave ? 256 : team, 0, s>>>(a, team);
   });
   return static_cast<int>(hipGetLastError());
 }
 
 int block_norm_bwd_plan(int64_t rows, int64_t d, int64_t gate_rows, BlockNormPlan& p) {
+  if (d < 1 || d > kMaxWidth || rows < 1) return -4;
   int v;
-  if (!team_for(d, p.team, v)) return -4;
-  const int teams = 1024 / p.team;  // LDS joins their sums: fewer partial rows than units
+  p.team = team_of(d, v);
+  const int teams = p.team >= 512 ? 1 : 512 / p.team;  // LDS joins their sums: fewer partial rows than units
   p.threads = p.team * teams;
-  int64_t units = 512 * teams;
+  int64_t units = 512 * teams;  // two blocks for each CU
   if (units > rows) units = rows;
   const int64_t groups = rows / gate_rows;
   p.split = units / groups;
@@ -443,17 +481,31 @@ int block_norm_bwd_plan(int64_t rows, int64_t d, int64_t gate_rows, BlockNormPla
   p.blocks = (used + teams - 1) / teams;
   p.units = p.blocks * teams;
   p.iterations = p.split > 1 ? (gate_rows + p.split - 1) / p.split : (groups + p.units - 1) / p.units * gate_rows;
-  p.lds = static_cast<int>((64 + (teams > 1 ? p.team * kN * v : 0)) * sizeof(float));
+  p.lds = static_cast<int>((64 + (teams > 1 ? p.team * kCols * v : 0)) * sizeof(float));
   return 0;
 }
+
+namespace {
+template <typename T, typename W>
+void launch_bwd(const BlockNormArgs& a, const BlockNormPlan& p, hipStream_t s) {
+  const bool full = a.d % kCols == 0;
+  int v;
+  team_of(a.d, v);
+  const auto kernel = v == 1 ? (full ? block_norm_bwd<T, W, 1, true, 512> : block_norm_bwd<T, W, 1, false, 512>)
+                      : p.threads <= 512
+                          ? (full ? block_norm_bwd<T, W, 2, true, 512> : block_norm_bwd<T, W, 2, false, 512>)
+                          : (full ? block_norm_bwd<T, W, 2, true, 1024> : block_norm_bwd<T, W, 2, false, 1024>);
+  kernel<<<static_cast<unsigned>(p.blocks), p.threads, p.lds, s>>>(a, p.team, p.iterations);
+}
+}  // namespace
 
 int block_norm_bwd(int dt, const BlockNormArgs& a, const BlockNormPlan& p, hipStream_t s) {
   if (a.rows <= 0) return 0;
   SMPK_DISPATCH(dt, T, {
-    if ((a.d + kN - 1) / kN <= 1024) {
-      block_norm_bwd<T, 1><<<static_cast<unsigned>(p.blocks), p.threads, p.lds, s>>>(a, p.team, p.iterations);
+    if (a.w_f32) {
+      launch_bwd<T, float>(a, p, s);
     } else {
-      block_norm_bwd<T, 2><<<static_cast<unsigned>(p.blocks), p.threads, p.lds, s>>>(a, p.team, p.iterations);
+      launch_bwd<T, T>(a, p, s);
     }
   });
   return static_cast<int>(hipGetLastError());
@@ -464,7 +516,7 @@ int block_norm_join(const BlockNormJoin& l, int d, hipStream_t s) {
   int64_t groups = 1;
   for (int i = 0; i < l.count; ++i) groups = l.item[i].groups > groups ? l.item[i].groups : groups;
   if (groups > 65535) return -3;
-  block_norm_join<<<dim3((d + 63) / 64, l.count, static_cast<unsigned>(groups)), 1024, 0, s>>>(l, d);
+  block_norm_join<<<dim3((d + 31) / 32, l.count, static_cast<unsigned>(groups)), 1024, 0, s>>>(l, d);
   return static_cast<int>(hipGetLastError());
 }
 

@@ -5,8 +5,8 @@
 //
 // Backward: dW[v] = scale * sum of dy[t] over the tokens with id_t = v, in token order and in
 // fp32, so that the result does not depend on the order in which blocks run.
-#include "common.h"
 #include "kernels.h"
+#include "vec8.h"
 
 namespace smpk {
 namespace {
@@ -24,56 +24,6 @@ __device__ __forceinline__ int64_t row_of(const IndexList& l, int64_t t) {
   }
   id -= l.start;
   return id >= 0 && id < l.rows ? id : -1;
-}
-
-// A thread handles 8 consecutive columns of a row.  Rows of odd widths start off 16 bytes: the
-// hardware loads and stores 16 bytes at any address, so only a row's last, partial vector goes
-// element by element.
-constexpr int kCols = 8;
-
-template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Any16 {
-  T v[16 / sizeof(T)];
-};
-template <typename T>
-struct Raw8 {
-  Any16<T> a[kCols * sizeof(T) / 16];
-};
-
-// FULL: rows are whole vectors; then no thread branches on `left`, and a batch of loads is issued
-// without a wait between them.
-template <bool FULL, typename T>
-__device__ __forceinline__ void read8(const T* p, int left, Raw8<T>& r) {
-  constexpr int M = 16 / sizeof(T);
-  if (FULL || left >= kCols) {
-#pragma unroll
-    for (int k = 0; k < kCols / M; ++k) __builtin_memcpy(&r.a[k], p + k * M, 16);
-  } else {
-#pragma unroll
-    for (int j = 0; j < kCols; ++j) r.a[j / M].v[j % M] = j < left ? p[j] : from_f32<T>(0.f);
-  }
-}
-template <typename T>
-__device__ __forceinline__ float at8(const Raw8<T>& r, int j) {
-  constexpr int M = 16 / sizeof(T);
-  return to_f32(r.a[j / M].v[j % M]);
-}
-template <bool FULL, typename T>
-__device__ __forceinline__ void write8(T* p, int left, const float (&o)[kCols]) {
-  constexpr int M = 16 / sizeof(T);
-  if (FULL || left >= kCols) {
-#pragma unroll
-    for (int k = 0; k < kCols / M; ++k) {
-      Any16<T> a;
-#pragma unroll
-      for (int j = 0; j < M; ++j) a.v[j] = from_f32<T>(o[k * M + j]);
-      __builtin_memcpy(p + k * M, &a, 16);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < kCols; ++j)
-      if (j < left) p[j] = from_f32<T>(o[j]);
-  }
 }
 
 constexpr int kPerThread = 4;  // vectors of a thread, all loads in flight together
@@ -150,7 +100,7 @@ __global__ void __launch_bounds__(kT) emb_fwd(IndexList ids, const T* __restrict
 #pragma unroll
       for (int j = 0; j < kCols; ++j) o[j] += at[u] ? at8(b[u], j) : NAN;
     }
-    if (t[u] < n) write8<FULL>(y + static_cast<int64_t>(t[u]) * d + c[u], d - c[u], o);
+    if (t[u] < n) write8<FULL, true>(y + static_cast<int64_t>(t[u]) * d + c[u], d - c[u], o);
   }
 }
 
@@ -189,24 +139,22 @@ __device__ __forceinline__ void wave_run(const SortItems& a, int block, int64_t&
   e = s + part < a.n ? s + part : a.n;
 }
 
-constexpr int kRounds = 8;  // 64-item rounds of a wave whose keys are loaded together
+constexpr int kRounds = 8;  // 64-item rounds of a wave: at most 8192 items a block
 
-__device__ __forceinline__ void load_keys(const SortItems& a, int64_t i0, int64_t e, uint32_t (&key)[kRounds]) {
-#pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    const int64_t i = i0 + r * 64 + (threadIdx.x & 63);
-    key[r] = i < e ? key_of(a, i) : 0u;
+// Counts a wave's next 64 items; returns how many of the wave's items of the same digit come before
+// this lane's.  Equal digits are counted together: a list may hold one token thousands of times.
+__device__ __forceinline__ int count_items(int digit, bool valid, int bits, int32_t* cnt) {
+  const int lane = threadIdx.x & 63;
+  uint64_t same = __ballot(valid);  // the lanes with this lane's digit
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (digit >> b) & 1;
+    const uint64_t m = __ballot(one);
+    same &= one ? m : ~m;
   }
-}
-
-__device__ __forceinline__ void count_digits(const SortItems& a, int64_t s, int64_t e, int32_t* cnt) {
-  for (int64_t i0 = s; i0 < e; i0 += 64 * kRounds) {
-    uint32_t key[kRounds];
-    load_keys(a, i0, e, key);
-#pragma unroll
-    for (int r = 0; r < kRounds; ++r)
-      if (i0 + r * 64 + (threadIdx.x & 63) < e) atomicAdd(&cnt[(key[r] >> a.shift) & ((1 << a.bits) - 1)], 1);
-  }
+  const int first = valid ? __ffsll(static_cast<unsigned long long>(same)) - 1 : lane;
+  int at = 0;
+  if (valid && lane == first) at = atomicAdd(&cnt[digit], __popcll(same));
+  return __shfl(at, first, 64) + __popcll(same & ((1ull << lane) - 1));
 }
 
 // The first pass also clears the marks that its second launch sets for every row with a token.
@@ -226,7 +174,16 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_count(SortItems a, int3
   __syncthreads();
   int64_t s, e;
   wave_run(a, blockIdx.x, s, e);
-  count_digits(a, s, e, cnt);
+  uint32_t keys[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int64_t i = s + r * 64 + (threadIdx.x & 63);
+    keys[r] = i < e ? key_of(a, i) : 0u;
+  }
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r)
+    if (s + r * 64 < e)
+      count_items((keys[r] >> a.shift) & (bins - 1), s + r * 64 + (threadIdx.x & 63) < e, a.bits, cnt);
   __syncthreads();
   for (int d = threadIdx.x; d < bins; d += kSortThreads) counts[static_cast<int64_t>(blockIdx.x) * bins + d] = cnt[d];
 }
@@ -272,21 +229,6 @@ __device__ __forceinline__ void counts_to_places(SortLds<BITS>& lds, int bins, b
   __syncthreads();
 }
 
-// Places of a wave's next 64 items, in lane order for equal digits; cnt moves on.
-__device__ __forceinline__ int place_of(int digit, bool valid, int bits, int32_t* cnt) {
-  const int lane = threadIdx.x & 63;
-  uint64_t same = __ballot(valid);  // the lanes with this lane's digit
-  for (int b = 0; b < bits; ++b) {
-    const bool one = (digit >> b) & 1;
-    const uint64_t m = __ballot(one);
-    same &= one ? m : ~m;
-  }
-  const int first = valid ? __ffsll(static_cast<unsigned long long>(same)) - 1 : lane;
-  int at = 0;
-  if (valid && lane == first) at = atomicAdd(&cnt[digit], __popcll(same));
-  return __shfl(at, first, 64) + __popcll(same & ((1ull << lane) - 1));
-}
-
 // One pass over the items of one block; counts [blocks][bins] of all blocks.
 __global__ void __launch_bounds__(kSortThreads) emb_sort_place(SortItems a, const int32_t* __restrict__ counts) {
   __shared__ SortLds<kMaxBits> lds;
@@ -297,7 +239,18 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_place(SortItems a, cons
   __syncthreads();
   int64_t s, e;
   wave_run(a, block, s, e);
-  count_digits(a, s, e, lds.cnt[wid]);
+  uint32_t keys[kRounds];
+  int32_t token[kRounds], rank[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int64_t i = s + r * 64 + lane;
+    keys[r] = i < e ? key_of(a, i) : 0u;
+    token[r] = a.tokens != nullptr && i < e ? a.tokens[i] : static_cast<int32_t>(i);
+  }
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r)
+    if (s + r * 64 < e)
+      rank[r] = count_items((keys[r] >> a.shift) & (bins - 1), s + r * 64 + lane < e, a.bits, lds.cnt[wid]);
   {  // every thread adds up one digit of some blocks
     int total = 0, before = 0;
     const int digit = tid & (bins - 1), step = kSortThreads >> a.bits;
@@ -312,26 +265,13 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_place(SortItems a, cons
   }
   __syncthreads();
   counts_to_places(lds, bins, false);
-  for (int64_t i0 = s; i0 < e; i0 += 64 * kRounds) {
-    uint32_t keys[kRounds];
-    int32_t token[kRounds];
-    load_keys(a, i0, e, keys);
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      const int64_t i = i0 + r * 64 + lane;
-      token[r] = a.tokens != nullptr && i < e ? a.tokens[i] : static_cast<int32_t>(i);
-    }
-#pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      if (i0 + r * 64 >= e) break;
-      const bool valid = i0 + r * 64 + lane < e;
-      const int at = place_of((keys[r] >> a.shift) & (bins - 1), valid, a.bits, lds.cnt[wid]);
-      if (valid) {
-        a.keys_out[at] = keys[r];
-        a.tokens_out[at] = token[r];
-        if (a.marks != nullptr && a.keys == nullptr && keys[r] < a.ids.rows) a.marks[keys[r]] = 1;
-      }
-    }
+  for (int r = 0; r < kRounds; ++r) {
+    if (s + r * 64 + lane >= e) continue;
+    const int at = lds.cnt[wid][(keys[r] >> a.shift) & (bins - 1)] + rank[r];
+    a.keys_out[at] = keys[r];
+    a.tokens_out[at] = token[r];
+    if (a.marks != nullptr && a.keys == nullptr && keys[r] < a.ids.rows) a.marks[keys[r]] = 1;
   }
 }
 
@@ -357,19 +297,19 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_short(SortItems a, int 
   }
   for (int p = 0; p < passes; ++p, a.shift += a.bits) {
     for (int d = lane; d < bins; d += 64) lds.cnt[wid][d] = 0;  // (its own wave's: no barrier)
+    int rank[R];
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      if (s + r * 64 < n) atomicAdd(&lds.cnt[wid][(key[r] >> a.shift) & (bins - 1)], 1);
+      if (wid * (64 * R) + r * 64 < n)
+        rank[r] = count_items((key[r] >> a.shift) & (bins - 1), s + r * 64 < n, a.bits, lds.cnt[wid]);
     __syncthreads();
     counts_to_places(lds, bins, true);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const bool valid = s + r * 64 < n;
-      const int at = place_of((key[r] >> a.shift) & (bins - 1), valid, a.bits, lds.cnt[wid]);
-      if (valid) {
-        keys[at] = key[r];
-        tokens[at] = token[r];
-      }
+      if (s + r * 64 >= n) continue;
+      const int at = lds.cnt[wid][(key[r] >> a.shift) & (bins - 1)] + rank[r];
+      keys[at] = key[r];
+      tokens[at] = token[r];
     }
     __syncthreads();
 #pragma unroll
@@ -420,7 +360,7 @@ __device__ __forceinline__ void write_row(T* p, int left, float (&sum)[kCols], f
 #pragma unroll
     for (int j = 0; j < kCols; ++j) sum[j] *= scale;
   }
-  write8<FULL>(p, left, sum);
+  write8<FULL, true>(p, left, sum);
 }
 
 constexpr int kZeroRows = 64;
@@ -439,7 +379,7 @@ __device__ __forceinline__ void clear_rows(const Sorted& l, const uint8_t* marks
   for (int k = 0; rows != 0; ++k, rows &= rows - 1) {
     if (k % (kT / 64) != static_cast<int>(threadIdx.x >> 6)) continue;
     const int64_t r = r0 + __ffsll(static_cast<unsigned long long>(rows)) - 1;
-    if (c < d) write8<FULL>(dw + r * d + c, d - c, zero);
+    if (c < d) write8<FULL, true>(dw + r * d + c, d - c, zero);
   }
 }
 
@@ -493,7 +433,7 @@ __global__ void __launch_bounds__(kT) emb_bwd_wide(Sorted l, const T* __restrict
       if (k != cur) {
         if (left > 0) {
           if (head) {
-            write8<FULL>(part + (2 * ch) * d + c, left, sum);
+            write8<FULL, false>(part + (2 * ch) * d + c, left, sum);
           } else {
             write_row<FULL>(dw + static_cast<int64_t>(cur) * d + c, left, sum, scale, accumulate);
           }
@@ -517,7 +457,7 @@ __global__ void __launch_bounds__(kT) emb_bwd_wide(Sorted l, const T* __restrict
   if (left <= 0) return;
   const bool tail = live == m && after == cur;
   if (head || tail) {
-    write8<FULL>(part + (2 * ch + (head ? 0 : 1)) * d + c, left, sum);
+    write8<FULL, false>(part + (2 * ch + (head ? 0 : 1)) * d + c, left, sum);
   } else {
     write_row<FULL>(dw + static_cast<int64_t>(cur) * d + c, left, sum, scale, accumulate);
   }
@@ -557,7 +497,7 @@ __global__ void __launch_bounds__(kT) emb_bwd_narrow(Sorted l, const T* __restri
     for (int u = 0; u < kAhead; ++u) {
       if (key[u] != cur && j + u < j1) {
         if (head) {
-          write8<FULL>(part + (2 * ch) * d + c, left, sum);
+          write8<FULL, false>(part + (2 * ch) * d + c, left, sum);
         } else {
           write_row<FULL>(dw + static_cast<int64_t>(cur) * d + c, left, sum, scale, accumulate);
         }
@@ -575,7 +515,7 @@ __global__ void __launch_bounds__(kT) emb_bwd_narrow(Sorted l, const T* __restri
   }
   const bool tail = j1 < l.n && l.key(j1) == cur;
   if (head || tail) {
-    write8<FULL>(part + (2 * ch + (head ? 0 : 1)) * d + c, left, sum);
+    write8<FULL, false>(part + (2 * ch + (head ? 0 : 1)) * d + c, left, sum);
   } else {
     write_row<FULL>(dw + static_cast<int64_t>(cur) * d + c, left, sum, scale, accumulate);
   }
@@ -662,8 +602,10 @@ EmbeddingPlan embedding_bwd_plan(int64_t n, int64_t d, int64_t rows, int64_t bat
   p.passes = sorted ? 0 : (bits + most - 1) / most;
   p.bits = sorted ? 0 : (bits + p.passes - 1) / p.passes;
   // one block sorts a short list alone, in one launch; longer ones go in runs of 2048 tokens or,
-  // above 256 blocks, whose counts every block reads, in longer runs
-  const int64_t parts = n <= kShortSort ? 1 : ((n + 2047) / 2048 < 256 ? (n + 2047) / 2048 : 256);
+  // above 256 blocks, whose counts every block reads, of up to 8192 (kRounds rounds of 16 waves)
+  constexpr int64_t kMost = kRounds * kSortThreads;
+  int64_t parts = n <= kShortSort ? 1 : (n + 2047) / 2048;
+  if (parts > 256) parts = (n + kMost - 1) / kMost > 256 ? (n + kMost - 1) / kMost : 256;
   p.per_block = ((n + parts - 1) / parts + kSortThreads - 1) / kSortThreads * kSortThreads;
   p.sort_blocks = n > 0 ? (n + p.per_block - 1) / p.per_block : 0;
   int64_t c = 16;  // tokens of a chunk: long ones leave fewer partial sums, short ones more to run at once

@@ -82,7 +82,7 @@ void embedding_bwd(at::Tensor dy, c10::optional<at::Tensor> ids, int64_t period,
   const int64_t n = dy.size(0), d = dy.size(1);
   TORCH_CHECK(dw.dim() == 2 && dw.is_contiguous() && dw.size(1) == d && dw.scalar_type() == dy.scalar_type(),
               "embedding: bad dw");
-  TORCH_CHECK(n < (1ll << 31) && dw.size(0) < (1ll << 31) - 1, "embedding: too many tokens or rows");
+  TORCH_CHECK(n <= (1ll << 27) && dw.size(0) < (1ll << 31) - 1, "embedding: more than 2^27 tokens or 2^31 rows");
   const auto li = index_list(ids, n, start, dw.size(0), period, dw);
   TORCH_CHECK(ids.has_value() || (period >= 1 && n % period == 0 && period <= dw.size(0)),
               "embedding: the tokens are no whole sequences of positions");
