@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kT) emb_fwd(IndexList ids, const T* __restrict
 #pragma unroll
       for (int j = 0; j < kCols; ++j) o[j] += at[u] ? at8(b[u], j) : NAN;
     }
-    if (t[u] < n) write8<FULL, true>(y + static_cast<int64_t>(t[u]) * d + c[u], d - c[u], o);
+    if (t[u] < n) write8<FULL, false>(y + static_cast<int64_t>(t[u]) * d + c[u], d - c[u], o);
   }
 }
 
@@ -147,9 +147,9 @@ __device__ __forceinline__ int count_items(int digit, bool valid, int bits, int3
   const int lane = threadIdx.x & 63;
   uint64_t same = __ballot(valid);  // the lanes with this lane's digit
   for (int b = 0; b < bits; ++b) {
-    const bool one = (digit >> b) & 1;
-    const uint64_t m = __ballot(one);
-    same &= one ? m : ~m;
+    const uint32_t mine = static_cast<uint32_t>(static_cast<int32_t>(static_cast<uint32_t>(digit) << (31 - b)) >> 31);
+    const uint64_t m = __ballot(mine != 0);
+    same &= ~(m ^ (static_cast<uint64_t>(mine) << 32 | mine));
   }
   const int first = valid ? __ffsll(static_cast<unsigned long long>(same)) - 1 : lane;
   int at = 0;
@@ -239,6 +239,17 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_place(SortItems a, cons
   __syncthreads();
   int64_t s, e;
   wave_run(a, block, s, e);
+  // every thread adds up one digit of some blocks
+  int all = 0, earlier = 0;
+  const int my_digit = tid & (bins - 1), step = kSortThreads >> a.bits;
+#pragma unroll 8
+  for (int b = tid >> a.bits; b < blocks; b += step) {
+    const int c = counts[(static_cast<int64_t>(b) << a.bits) + my_digit];
+    all += c;
+    earlier += b < block ? c : 0;
+  }
+  atomicAdd(&lds.total[my_digit], all);
+  atomicAdd(&lds.before[my_digit], earlier);
   uint32_t keys[kRounds];
   int32_t token[kRounds], rank[kRounds];
 #pragma unroll
@@ -251,18 +262,6 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_place(SortItems a, cons
   for (int r = 0; r < kRounds; ++r)
     if (s + r * 64 < e)
       rank[r] = count_items((keys[r] >> a.shift) & (bins - 1), s + r * 64 + lane < e, a.bits, lds.cnt[wid]);
-  {  // every thread adds up one digit of some blocks
-    int total = 0, before = 0;
-    const int digit = tid & (bins - 1), step = kSortThreads >> a.bits;
-#pragma unroll 8
-    for (int b = tid >> a.bits; b < blocks; b += step) {
-      const int c = counts[(static_cast<int64_t>(b) << a.bits) + digit];
-      total += c;
-      before += b < block ? c : 0;
-    }
-    atomicAdd(&lds.total[digit], total);
-    atomicAdd(&lds.before[digit], before);
-  }
   __syncthreads();
   counts_to_places(lds, bins, false);
 #pragma unroll
@@ -383,20 +382,41 @@ __device__ __forceinline__ void clear_rows(const Sorted& l, const uint8_t* marks
   }
 }
 
+// What a launch has to do for one table: blocks [first, first + blocks) add up its tokens, then
+// [clear, clear + clears) clear rows.
+struct Work {
+  Sorted l;
+  void* dw;
+  float* part;
+  const uint8_t* marks;
+  float scale;
+  int accumulate, chunk;
+  int64_t first, blocks, clear, clears;
+};
+
+__device__ __forceinline__ Work work_of(const Work& a, const Work& b) {
+  const int64_t i = blockIdx.x;
+  return (i >= b.first && i < b.first + b.blocks) || i >= b.clear ? b : a;
+}
+
 // A wave takes a chunk of at most 64 tokens and 512 columns.  Lane i knows the i-th token; a run is
 // followed with scalar registers, so the branches cost nothing, and the gradient rows of one
 // batch are loaded while those of the batch before are added.
 template <typename T, bool FULL>
-__global__ void __launch_bounds__(kT) emb_bwd_wide(Sorted l, const T* __restrict__ dy, int d, int chunk, int slabs,
-                                                   int64_t blocks, float scale, T* __restrict__ dw, int accumulate,
-                                                   float* __restrict__ part, const uint8_t* __restrict__ marks) {
+__global__ void __launch_bounds__(kT) emb_bwd_wide(Work w0, Work w1, const T* __restrict__ dy, int d, int slabs) {
   constexpr int kAhead = sizeof(T) == 4 ? 4 : 8;
-  if (static_cast<int64_t>(blockIdx.x) >= blocks) {
-    clear_rows<FULL>(l, marks, blockIdx.x - blocks, slabs, dw, d);
+  const Work wk = work_of(w0, w1);
+  const Sorted l = wk.l;
+  T* const dw = static_cast<T*>(wk.dw);
+  float* const part = wk.part;
+  const float scale = wk.scale;
+  const int accumulate = wk.accumulate, chunk = wk.chunk;
+  if (static_cast<int64_t>(blockIdx.x) >= wk.clear) {
+    clear_rows<FULL>(l, wk.marks, blockIdx.x - wk.clear, slabs, dw, d);
     return;
   }
   const int lane = threadIdx.x & 63;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kT / 64) +
+  const int64_t unit = (static_cast<int64_t>(blockIdx.x) - wk.first) * (kT / 64) +
                        __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int64_t ch = unit / slabs;
   const int c = (static_cast<int>(unit - ch * slabs) * 64 + lane) * kCols, left = d - c;
@@ -466,15 +486,19 @@ __global__ void __launch_bounds__(kT) emb_bwd_wide(Sorted l, const T* __restrict
 // The same for rows of at most 256 columns: `lanes` threads (a power of two) hold a chunk's
 // columns, kT / lanes chunks a block.
 template <typename T, bool FULL>
-__global__ void __launch_bounds__(kT) emb_bwd_narrow(Sorted l, const T* __restrict__ dy, int d, int chunk, int lanes,
-                                                     int64_t blocks, float scale, T* __restrict__ dw, int accumulate,
-                                                     float* __restrict__ part, const uint8_t* __restrict__ marks) {
+__global__ void __launch_bounds__(kT) emb_bwd_narrow(Work w0, Work w1, const T* __restrict__ dy, int d, int lanes) {
   constexpr int kAhead = 8;
-  if (static_cast<int64_t>(blockIdx.x) >= blocks) {
-    clear_rows<FULL>(l, marks, blockIdx.x - blocks, 1, dw, d);
+  const Work wk = work_of(w0, w1);
+  const Sorted l = wk.l;
+  T* const dw = static_cast<T*>(wk.dw);
+  float* const part = wk.part;
+  const float scale = wk.scale;
+  const int accumulate = wk.accumulate, chunk = wk.chunk;
+  if (static_cast<int64_t>(blockIdx.x) >= wk.clear) {
+    clear_rows<FULL>(l, wk.marks, blockIdx.x - wk.clear, 1, dw, d);
     return;
   }
-  const int64_t ch = static_cast<int64_t>(blockIdx.x) * (kT / lanes) + threadIdx.x / lanes;
+  const int64_t ch = (static_cast<int64_t>(blockIdx.x) - wk.first) * (kT / lanes) + threadIdx.x / lanes;
   const int c = threadIdx.x % lanes * kCols;
   const int left = d - c;
   const int64_t j0 = ch * chunk, j1 = j0 + chunk < l.n ? j0 + chunk : l.n;
@@ -521,24 +545,6 @@ __global__ void __launch_bounds__(kT) emb_bwd_narrow(Sorted l, const T* __restri
   }
 }
 
-// the first place whose key is not below k
-__device__ __forceinline__ int64_t lower_bound(const Sorted& l, uint32_t k) {
-  if (l.keys == nullptr) {
-    const int64_t j = static_cast<int64_t>(k) * l.batch;
-    return j < l.n ? j : l.n;
-  }
-  int64_t lo = 0, hi = l.n;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (l.keys[mid] < k) {
-      lo = mid + 1;
-    } else {
-      hi = mid;
-    }
-  }
-  return lo;
-}
-
 // Block b joins the run that begins in chunk b and goes on behind it.
 template <typename T, bool FULL>
 __global__ void __launch_bounds__(kT) emb_bwd_join(Sorted l, const float* __restrict__ part, int d, int chunk, int lanes,
@@ -550,7 +556,14 @@ __global__ void __launch_bounds__(kT) emb_bwd_join(Sorted l, const float* __rest
   if (j1 >= l.n) return;
   const uint32_t k = l.key(j1);
   if (k >= l.rows || l.key(j1 - 1) != k || (j0 > 0 && l.key(j0) == k && l.key(j0 - 1) == k)) return;
-  const int64_t last = (lower_bound(l, k + 1) - 1) / chunk;  // the run's last chunk
+  int64_t last = ch + 1;  // the run's last chunk: 64 chunks' first keys at a time
+  for (;;) {
+    const int64_t j = (last + 1 + (tid & 63)) * chunk;
+    const uint64_t on = __ballot(j < l.n && l.key(j) == k);
+    const int more = on == ~0ull ? 64 : __ffsll(static_cast<unsigned long long>(~on)) - 1;
+    last += more;
+    if (more < 64) break;
+  }
   float sum[kCols];
 #pragma unroll
   for (int q = 0; q < kCols; ++q) sum[q] = 0.f;
@@ -618,73 +631,102 @@ EmbeddingPlan embedding_bwd_plan(int64_t n, int64_t d, int64_t rows, int64_t bat
   return p;
 }
 
-int embedding_bwd(int dt, const IndexList& ids, const void* dy, int64_t n, int64_t d, float scale, int64_t skip,
-                  void* dw, int accumulate, const EmbeddingPlan& p, uint32_t* keys, int32_t* tokens, int32_t* counts,
-                  float* part, uint8_t* marks, hipStream_t s) {
-  if (ids.rows <= 0 || d <= 0 || (n <= 0 && accumulate)) return 0;
-  Sorted l{nullptr, nullptr, n, ids.rows, ids.period > 0 ? n / ids.period : 1, ids.period};
-  if (ids.ids != nullptr && n > 0) {
-    SortItems a;
-    a.ids = ids;
-    a.skip = skip;
-    a.keys = nullptr;
-    a.tokens = nullptr;
-    a.n = n;
-    a.per_block = p.per_block;
-    a.shift = 0;
-    a.bits = p.bits;
-    a.keys_out = keys;
-    a.tokens_out = tokens;
-    a.marks = accumulate ? nullptr : marks;
-    if (p.sort_blocks == 1) {
-      const auto kernel = n <= 2 * kSortThreads   ? emb_sort_short<2>
-                          : n <= 4 * kSortThreads ? emb_sort_short<4>
-                          : n <= 8 * kSortThreads ? emb_sort_short<8>
-                                                  : emb_sort_short<16>;
-      kernel<<<1, kSortThreads, 0, s>>>(a, p.passes);
-    } else {
-      for (int q = 0; q < p.passes; ++q) {
-        const int to = (p.passes - 1 - q) & 1;
-        a.keys_out = keys + to * n;
-        a.tokens_out = tokens + to * n;
-        emb_sort_count<<<static_cast<unsigned>(p.sort_blocks), kSortThreads, 0, s>>>(a, counts);
-        emb_sort_place<<<static_cast<unsigned>(p.sort_blocks), kSortThreads, 0, s>>>(a, counts);
-        a.keys = a.keys_out;
-        a.tokens = a.tokens_out;
-        a.shift += a.bits;
-      }
+namespace {
+
+// The order of a table's tokens: sorted, unless they are positions.
+int sort_tokens(const EmbeddingGrad& t, int64_t n, Sorted& l, hipStream_t s) {
+  const EmbeddingPlan& p = t.plan;
+  l = Sorted{nullptr, nullptr, n, t.ids.rows, t.ids.period > 0 ? n / t.ids.period : 1, t.ids.period};
+  if (t.ids.ids == nullptr || n <= 0) return 0;
+  SortItems a;
+  a.ids = t.ids;
+  a.skip = t.skip;
+  a.keys = nullptr;
+  a.tokens = nullptr;
+  a.n = n;
+  a.per_block = p.per_block;
+  a.shift = 0;
+  a.bits = p.bits;
+  a.keys_out = t.keys;
+  a.tokens_out = t.tokens;
+  a.marks = t.accumulate ? nullptr : t.marks;
+  if (p.sort_blocks == 1) {
+    const auto kernel = n <= 2 * kSortThreads   ? emb_sort_short<2>
+                        : n <= 4 * kSortThreads ? emb_sort_short<4>
+                        : n <= 8 * kSortThreads ? emb_sort_short<8>
+                                                : emb_sort_short<16>;
+    kernel<<<1, kSortThreads, 0, s>>>(a, p.passes);
+  } else {
+    for (int q = 0; q < p.passes; ++q) {
+      const int to = (p.passes - 1 - q) & 1;
+      a.keys_out = t.keys + to * n;
+      a.tokens_out = t.tokens + to * n;
+      emb_sort_count<<<static_cast<unsigned>(p.sort_blocks), kSortThreads, 0, s>>>(a, t.counts);
+      emb_sort_place<<<static_cast<unsigned>(p.sort_blocks), kSortThreads, 0, s>>>(a, t.counts);
+      a.keys = a.keys_out;
+      a.tokens = a.tokens_out;
+      a.shift += a.bits;
     }
-    l.keys = keys;
-    l.tokens = tokens;
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return static_cast<int>(e);
   }
+  l.keys = t.keys;
+  l.tokens = t.tokens;
+  return static_cast<int>(hipGetLastError());
+}
+
+}  // namespace
+
+int embedding_bwd(int dt, const void* dy, int64_t n, int64_t d, const EmbeddingGrad* tables, int count, hipStream_t s) {
+  if (d <= 0 || count < 1 || count > 2) return -5;
   int lanes = 1;  // of a narrow chunk, and of a joining block's column slab
   while (lanes < kT && lanes * kCols < d) lanes *= 2;
-  const int64_t slabs = (d + 64 * kCols - 1) / (64 * kCols), join_slabs = (d + lanes * kCols - 1) / (lanes * kCols);
-  const int64_t zero = accumulate ? 0 : (ids.rows + kZeroRows - 1) / kZeroRows * slabs;
   const bool wide = lanes >= 64, full = d % kCols == 0;
+  const int64_t slabs = (d + 64 * kCols - 1) / (64 * kCols), join_slabs = (d + lanes * kCols - 1) / (lanes * kCols);
   const int64_t units = wide ? kT / 64 : kT / lanes;
-  const int64_t blocks = ((wide ? p.chunks * slabs : p.chunks) + units - 1) / units;
-  if (blocks + zero > 0x7fffffff || join_slabs > 65535) return -3;
-  const uint8_t* flags = l.keys != nullptr ? marks : nullptr;
+  Work w[2];
+  int64_t grid = 0;
+  for (int i = 0; i < count; ++i) {
+    const EmbeddingGrad& t = tables[i];
+    const int rc = sort_tokens(t, n, w[i].l, s);
+    if (rc != 0) return rc;
+    w[i].dw = t.dw;
+    w[i].part = t.part;
+    w[i].marks = w[i].l.keys != nullptr ? t.marks : nullptr;
+    w[i].scale = t.scale;
+    w[i].accumulate = t.accumulate;
+    w[i].chunk = t.plan.chunk;
+    w[i].first = grid;
+    w[i].blocks = ((wide ? t.plan.chunks * slabs : t.plan.chunks) + units - 1) / units;
+    grid += w[i].blocks;
+  }
+  for (int i = 0; i < count; ++i) {
+    w[i].clear = grid;
+    w[i].clears = tables[i].accumulate ? 0 : (w[i].l.rows + kZeroRows - 1) / kZeroRows * slabs;
+    grid += w[i].clears;
+  }
+  if (count == 1) {
+    w[1] = w[0];
+    w[1].first = w[1].clear = grid;
+    w[1].blocks = 0;
+  }
+  if (grid > 0x7fffffff || join_slabs > 65535) return -3;
+  if (grid == 0) return 0;
   SMPK_DISPATCH(dt, T, {
-    if (blocks + zero > 0) {
-      const unsigned grid = static_cast<unsigned>(blocks + zero);
-      if (wide) {
-        const auto kernel = full ? emb_bwd_wide<T, true> : emb_bwd_wide<T, false>;
-        kernel<<<grid, kT, 0, s>>>(l, static_cast<const T*>(dy), static_cast<int>(d), p.chunk, static_cast<int>(slabs),
-                                   blocks, scale, static_cast<T*>(dw), accumulate, part, flags);
-      } else {
-        const auto kernel = full ? emb_bwd_narrow<T, true> : emb_bwd_narrow<T, false>;
-        kernel<<<grid, kT, 0, s>>>(l, static_cast<const T*>(dy), static_cast<int>(d), p.chunk, lanes, blocks, scale,
-                                   static_cast<T*>(dw), accumulate, part, flags);
-      }
+    if (wide) {
+      const auto kernel = full ? emb_bwd_wide<T, true> : emb_bwd_wide<T, false>;
+      kernel<<<static_cast<unsigned>(grid), kT, 0, s>>>(w[0], w[1], static_cast<const T*>(dy), static_cast<int>(d),
+                                                       static_cast<int>(slabs));
+    } else {
+      const auto kernel = full ? emb_bwd_narrow<T, true> : emb_bwd_narrow<T, false>;
+      kernel<<<static_cast<unsigned>(grid), kT, 0, s>>>(w[0], w[1], static_cast<const T*>(dy), static_cast<int>(d),
+                                                       lanes);
     }
-    if (p.join && p.chunks > 1) {
+    for (int i = 0; i < count; ++i) {
+      const EmbeddingPlan& p = tables[i].plan;
+      if (!p.join || p.chunks <= 1) continue;
       const auto kernel = full ? emb_bwd_join<T, true> : emb_bwd_join<T, false>;
       kernel<<<dim3(static_cast<unsigned>(p.chunks), static_cast<unsigned>(join_slabs)), kT, 0, s>>>(
-          l, part, static_cast<int>(d), p.chunk, lanes, scale, static_cast<T*>(dw), accumulate);
+          w[i].l, w[i].part, static_cast<int>(d), p.chunk, lanes, w[i].scale, static_cast<T*>(w[i].dw),
+          w[i].accumulate);
     }
   });
   return static_cast<int>(hipGetLastError());

@@ -245,19 +245,31 @@ struct IndexList {
 int embedding_fwd(int dt, const IndexList& ids, const void* w, int64_t w_stride, float scale, int foreign_zero,
                   const IndexList& pos, const void* p, int64_t p_stride, void* y, int64_t n, int64_t d,
                   hipStream_t s);
-// How embedding_bwd goes about n tokens and a table of `rows` rows; its workspaces are keys and
-// tokens [2][n], counts [sort_blocks << bits], part [chunks][2][d] (join) and, for a dense gradient,
-// marks [rows rounded up to 16].  batch > 0: ids null, `batch` sequences of positions.
+// How the tokens of a table of `rows` rows are gone about; batch > 0: no ids, `batch` sequences of
+// positions.
 struct EmbeddingPlan {
   int passes, bits, chunk, join;
   int64_t per_block, sort_blocks, chunks;
 };
 EmbeddingPlan embedding_bwd_plan(int64_t n, int64_t d, int64_t rows, int64_t batch);
-// dw[v] = scale * sum of dy[t] over the tokens of row v, or added to dw (accumulate: rows without
-// tokens are not touched); row `skip` (-1: none) gets no gradient.
-int embedding_bwd(int dt, const IndexList& ids, const void* dy, int64_t n, int64_t d, float scale, int64_t skip,
-                  void* dw, int accumulate, const EmbeddingPlan& p, uint32_t* keys, int32_t* tokens, int32_t* counts,
-                  float* part, uint8_t* marks, hipStream_t s);
+// One table's gradient: dw[v] = scale * sum of dy[t] over the tokens of row v, or added to dw
+// (accumulate: rows without tokens are not touched); row `skip` (-1: none) gets none.  Workspaces:
+// keys and tokens [2][n] and counts [sort_blocks << bits] with ids, marks [rows rounded up to 16]
+// with ids and a dense gradient, part [chunks][2][d] with plan.join.
+struct EmbeddingGrad {
+  IndexList ids;
+  float scale;
+  int64_t skip;
+  void* dw;
+  int accumulate;
+  EmbeddingPlan plan;
+  uint32_t* keys;
+  int32_t *tokens, *counts;
+  float* part;
+  uint8_t* marks;
+};
+// Up to two tables at once; their gradients must not share memory.
+int embedding_bwd(int dt, const void* dy, int64_t n, int64_t d, const EmbeddingGrad* tables, int count, hipStream_t s);
 
 // ------------------------------------------------------------------ gradient norm (grad_norm.hip)
 // Up to kGradList tensors, each cut into chunks of one size: chunk b of a launch lies in tensor t

@@ -74,31 +74,57 @@ at::Tensor embedding_fwd(at::Tensor ids, at::Tensor weight, double scale, int64_
   return y;
 }
 
-// dw [rows, d] = (or += accumulate) the gradient of the table whose rows `ids` (or t % period) chose
-void embedding_bwd(at::Tensor dy, c10::optional<at::Tensor> ids, int64_t period, double scale, int64_t start,
-                   int64_t skip, at::Tensor dw, bool accumulate) {
-  const c10::DeviceGuard guard(dw.device());
-  TORCH_CHECK(dy.is_cuda() && dy.dim() == 2 && dy.is_contiguous() && dy.device() == dw.device(), "embedding: bad dy");
+// Gradients of the token table (ids, scale, start, skip) and of the position table (pos or, without
+// them, t % period): rows x d tensors of dy's type.  dw / dp: written, or added to (accumulate);
+// null: not wanted.
+void embedding_bwd(at::Tensor dy, at::Tensor ids, c10::optional<at::Tensor> pos, int64_t period, double scale,
+                   int64_t start, int64_t skip, c10::optional<at::Tensor> dw, bool dw_accumulate,
+                   c10::optional<at::Tensor> dp, bool dp_accumulate) {
+  const c10::DeviceGuard guard(dy.device());
+  TORCH_CHECK(dy.is_cuda() && dy.dim() == 2 && dy.is_contiguous(), "embedding: bad dy");
   const int64_t n = dy.size(0), d = dy.size(1);
-  TORCH_CHECK(dw.dim() == 2 && dw.is_contiguous() && dw.size(1) == d && dw.scalar_type() == dy.scalar_type(),
-              "embedding: bad dw");
-  TORCH_CHECK(n <= (1ll << 27) && dw.size(0) < (1ll << 31) - 1, "embedding: more than 2^27 tokens or 2^31 rows");
-  const auto li = index_list(ids, n, start, dw.size(0), period, dw);
-  TORCH_CHECK(ids.has_value() || (period >= 1 && n % period == 0 && period <= dw.size(0)),
-              "embedding: the tokens are no whole sequences of positions");
-  const auto p = smpk::embedding_bwd_plan(n, d, dw.size(0), ids.has_value() ? 0 : std::max<int64_t>(n / period, 1));
-  const auto i32 = dw.options().dtype(at::kInt);
-  const bool sort = ids.has_value() && n > 0;
-  auto order = at::empty({sort ? 4 * n : 0}, i32);
-  auto counts = at::empty({sort && p.sort_blocks > 1 ? p.sort_blocks << p.bits : 0}, i32);
-  auto part = at::empty({p.join ? p.chunks * 2 * d : 0}, dw.options().dtype(at::kFloat));
-  auto marks = at::empty({sort && !accumulate ? (dw.size(0) + 15) / 16 * 16 : 0}, dw.options().dtype(at::kByte));
-  int32_t* const o = order.data_ptr<int32_t>();
-  check(smpk::embedding_bwd(dt_code(dw, "weight"), li, dy.data_ptr(), n, d, static_cast<float>(scale), skip,
-                            dw.data_ptr(), accumulate ? 1 : 0, p, reinterpret_cast<uint32_t*>(o),
-                            sort ? o + 2 * n : o, counts.data_ptr<int32_t>(), part.data_ptr<float>(),
-                            marks.data_ptr<uint8_t>(), stream()),
-        "embedding_bwd");
+  TORCH_CHECK(n <= (1ll << 27), "embedding: more than 2^27 tokens");
+  smpk::EmbeddingGrad t[2];
+  int count = 0;
+  int64_t bytes = 0;
+  int64_t at[2][5];  // keys, tokens, counts, part, marks in the workspace
+  for (int i = 0; i < 2; ++i) {
+    const auto& g = i == 0 ? dw : dp;
+    if (!g.has_value()) continue;
+    TORCH_CHECK(g->dim() == 2 && g->is_contiguous() && g->size(1) == d && g->scalar_type() == dy.scalar_type() &&
+                    g->device() == dy.device() && g->size(0) < (1ll << 31) - 1,
+                "embedding: bad gradient");
+    smpk::EmbeddingGrad& e = t[count];
+    const int64_t rows = g->size(0);
+    const bool sequence = i == 1 && !pos.has_value();
+    if (sequence)
+      TORCH_CHECK(period >= 1 && n % period == 0 && period <= rows, "embedding: no whole sequences of positions");
+    e.ids = i == 0 ? index_list(ids, n, start, rows, 1, dy) : index_list(pos, n, 0, rows, period, dy);
+    e.scale = i == 0 ? static_cast<float>(scale) : 1.f;
+    e.skip = i == 0 ? skip : -1;
+    e.dw = g->data_ptr();
+    e.accumulate = i == 0 ? dw_accumulate : dp_accumulate;
+    e.plan = smpk::embedding_bwd_plan(n, d, rows, sequence ? std::max<int64_t>(n / period, 1) : 0);
+    const bool sort = !sequence && n > 0;
+    const int64_t size[5] = {sort ? 8 * n : 0, sort ? 8 * n : 0, sort ? e.plan.sort_blocks << (e.plan.bits + 2) : 0,
+                             e.plan.join ? e.plan.chunks * 8 * d : 0, sort && !e.accumulate ? rows : 0};
+    for (int k = 0; k < 5; ++k) {
+      at[count][k] = bytes;
+      bytes += (size[k] + 15) / 16 * 16;
+    }
+    ++count;
+  }
+  if (count == 0) return;
+  auto ws = at::empty({bytes}, dy.options().dtype(at::kByte));
+  uint8_t* const base = ws.data_ptr<uint8_t>();
+  for (int i = 0; i < count; ++i) {
+    t[i].keys = reinterpret_cast<uint32_t*>(base + at[i][0]);
+    t[i].tokens = reinterpret_cast<int32_t*>(base + at[i][1]);
+    t[i].counts = reinterpret_cast<int32_t*>(base + at[i][2]);
+    t[i].part = reinterpret_cast<float*>(base + at[i][3]);
+    t[i].marks = base + at[i][4];
+  }
+  check(smpk::embedding_bwd(dt_code(dy, "embedding"), dy.data_ptr(), n, d, t, count, stream()), "embedding_bwd");
 }
 
 // ------------------------------------------------------------------ block norm
@@ -282,30 +308,44 @@ void check_disjoint(const std::vector<at::Tensor>& in, const std::vector<at::Ten
   }
 }
 
-// {power fp64 [1], norm fp32 []}; with `out`, also out[i] = grads[i] * scale * min(1, max_norm / (norm + 1e-6))
+bool is_float(const at::Tensor& t) {
+  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16;
+}
+
+// {power fp64 [1], norm fp32 []}; with `out`, also out[i] = grads[i] * scale * min(1, max_norm / (norm + 1e-6)).
+// Tensors with gaps (slices, expanded views) go through dense copies.
 std::vector<at::Tensor> grad_norm(std::vector<at::Tensor> grads, bool inf, double scale,
                                   c10::optional<std::vector<at::Tensor>> out, double max_norm) {
-  TORCH_CHECK(!grads.empty(), "grad_norm: no tensors");
-  const c10::DeviceGuard guard(grads[0].device());
+  TORCH_CHECK_VALUE(!grads.empty() && grads[0].defined() && grads[0].is_cuda(), "no GPU tensors");
+  const at::Device device = grads[0].device();
+  const c10::DeviceGuard guard(device);
   int64_t total = 0;
-  for (size_t i = 0; i < grads.size(); ++i) {
-    const at::Tensor& t = grads[i];
-    TORCH_CHECK(t.is_cuda() && t.device() == grads[0].device() && t.is_non_overlapping_and_dense(),
-                "grad_norm: dense tensors of one GPU expected");
-    dt_code(t, "grad_norm");
-    total += t.numel();
-  }
+  std::vector<at::Tensor> dest;
   if (out.has_value()) {
-    TORCH_CHECK(out->size() == grads.size(), "grad_norm: lists of different lengths");
-    for (size_t i = 0; i < grads.size(); ++i) {
-      const at::Tensor& o = (*out)[i];
-      TORCH_CHECK(o.device() == grads[0].device() && o.sizes() == grads[i].sizes() &&
-                      (o.numel() == 0 || o.strides() == grads[i].strides()),
-                  "grad_norm: out differs from its gradient");
-      dt_code(o, "grad_norm");
-    }
-    check_disjoint(grads, *out);
+    TORCH_CHECK_VALUE(out->size() == grads.size(), grads.size(), " gradients, ", out->size(), " outputs");
+    dest = *out;
   }
+  for (size_t i = 0; i < grads.size(); ++i) {
+    at::Tensor& t = grads[i];
+    TORCH_CHECK_VALUE(t.defined() && t.layout() == at::kStrided && is_float(t), "tensor ", i, " is none of them");
+    TORCH_CHECK_VALUE(t.device() == device, "tensor ", i, " is on ", t.device(), ", not on ", device);
+    total += t.numel();
+    if (out.has_value()) {
+      at::Tensor& o = dest[i];
+      TORCH_CHECK_VALUE(o.defined() && o.layout() == at::kStrided && is_float(o) && o.device() == device &&
+                            o.sizes() == t.sizes(),
+                        "output ", i, " differs from its gradient in shape or device, or is none of them");
+      for (int64_t k = 0; k < o.dim(); ++k)
+        TORCH_CHECK_VALUE(o.stride(k) != 0 || o.size(k) <= 1, "output ", i, " is expanded: it cannot be written");
+    }
+    if (!t.is_non_overlapping_and_dense()) t = t.contiguous();
+    if (out.has_value()) {
+      at::Tensor& o = dest[i];
+      if (!o.is_non_overlapping_and_dense() || (o.numel() != 0 && o.strides() != t.strides()))
+        o = at::empty_like(t, t.options().dtype(o.scalar_type()));  // copied to the output at the end
+    }
+  }
+  if (out.has_value()) check_disjoint(grads, dest);
   const int64_t size = smpk::grad_chunk_size(total);
   std::vector<smpk::GradList> lists(1);
   lists[0].count = 0;
@@ -324,25 +364,28 @@ std::vector<at::Tensor> grad_norm(std::vector<at::Tensor> grads, bool inf, doubl
     smpk::GradList& l = lists.back();
     const int k = l.count++;
     l.p[k] = grads[i].data_ptr();
-    l.o[k] = out.has_value() ? (*out)[i].data_ptr() : nullptr;
+    l.o[k] = out.has_value() ? dest[i].data_ptr() : nullptr;
     l.n[k] = n;
     l.dt[k] = static_cast<uint8_t>(dt_code(grads[i], "grad_norm"));
-    l.odt[k] = out.has_value() ? static_cast<uint8_t>(dt_code((*out)[i], "grad_norm")) : 0;
+    l.odt[k] = out.has_value() ? static_cast<uint8_t>(dt_code(dest[i], "grad_norm")) : 0;
     l.first[k + 1] = l.first[k] + static_cast<uint32_t>((n + size - 1) / size);
   }
   const int64_t chunks = lists.back().first_chunk + lists.back().first[lists.back().count];
   const auto opts = grads[0].options();
-  auto part = at::empty({chunks < 1 ? 1 : chunks}, opts.dtype(at::kDouble));
+  auto part = at::empty({chunks + 1}, opts.dtype(at::kDouble));  // (the last holds the factor)
   auto power = at::empty({1}, opts.dtype(at::kDouble));
   auto norm = at::empty({}, opts.dtype(at::kFloat));
-  auto factor = at::empty({1}, opts.dtype(at::kFloat));
+  float* const factor = reinterpret_cast<float*>(part.data_ptr<double>() + chunks);
   for (const auto& l : lists)
     check(smpk::grad_partials(l, size, inf ? 1 : 0, part.data_ptr<double>(), stream()), "grad_partials");
   check(smpk::grad_join(part.data_ptr<double>(), chunks, inf ? 1 : 0, scale, max_norm, power.data_ptr<double>(),
-                        norm.data_ptr<float>(), out.has_value() ? factor.data_ptr<float>() : nullptr, stream()),
+                        norm.data_ptr<float>(), out.has_value() ? factor : nullptr, stream()),
         "grad_join");
-  if (out.has_value())
-    for (const auto& l : lists) check(smpk::grad_scale(l, size, factor.data_ptr<float>(), stream()), "grad_scale");
+  if (out.has_value()) {
+    for (const auto& l : lists) check(smpk::grad_scale(l, size, factor, stream()), "grad_scale");
+    for (size_t i = 0; i < dest.size(); ++i)
+      if (!dest[i].is_same((*out)[i])) (*out)[i].copy_(dest[i]);
+  }
   return {power, norm};
 }
 
@@ -359,6 +402,7 @@ void register_training_ops(py::module_& m) {
         py::arg("max_norm") = 0.0);
   m.def("embedding_fwd", &embedding_fwd, py::arg("ids"), py::arg("weight"), py::arg("scale"), py::arg("start"),
         py::arg("foreign_zero"), py::arg("pos"), py::arg("pos_weight"), py::arg("period"));
-  m.def("embedding_bwd", &embedding_bwd, py::arg("dy"), py::arg("ids"), py::arg("period"), py::arg("scale"),
-        py::arg("start"), py::arg("skip"), py::arg("dw"), py::arg("accumulate"));
+  m.def("embedding_bwd", &embedding_bwd, py::arg("dy"), py::arg("ids"), py::arg("pos"), py::arg("period"),
+        py::arg("scale"), py::arg("start"), py::arg("skip"), py::arg("dw"), py::arg("dw_accumulate"), py::arg("dp"),
+        py::arg("dp_accumulate"));
 }

@@ -17,14 +17,14 @@ from ._ext import ext, fused_ok
 from .linear import _fusable
 
 
-def _table_grad(weight, dy, ids, period, scale, start, skip):
-    """Gradient of one table; None when it went into the bound gradient in place."""
-    if _fusable(weight):
-        ext().embedding_bwd(dy, ids, period, scale, start, skip, weight.grad, True)
-        return None
-    dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
-    ext().embedding_bwd(dy, ids, period, scale, start, skip, dw, False)
-    return dw
+def _target(table, needed):
+    """(tensor the gradient goes to, whether it is added there): the bound gradient of a parameter
+    in the flat buffer, else a new tensor; (None, False) if it is not needed."""
+    if not needed:
+        return None, False
+    if table.is_leaf and _fusable(table):
+        return table.grad, True
+    return torch.empty(table.shape, dtype=table.dtype, device=table.device), False
 
 
 class _EmbeddingHIP(torch.autograd.Function):
@@ -52,12 +52,14 @@ class _EmbeddingHIP(torch.autograd.Function):
         weight, position_weight = ctx.tables
         period, scale, start, skip = ctx.args
         dy2 = dy.reshape(-1, weight.shape[1]).contiguous()
-        dw = dpw = None
-        if ctx.needs_input_grad[0]:
-            dw = _table_grad(weight, dy2, flat, 1, scale, start, skip)
-        if ctx.needs_input_grad[1]:
-            dpw = _table_grad(position_weight, dy2, pos, period, 1.0, 0, -1)
-        return dw, dpw, None, None, None, None, None
+        dw, dw_add = _target(weight, ctx.needs_input_grad[0])
+        dp, dp_add = _target(position_weight, ctx.needs_input_grad[1])
+        if dw_add and dp_add and dw.data_ptr() == dp.data_ptr():  # one parameter as both tables: one after the other
+            ext().embedding_bwd(dy2, flat, pos, period, scale, start, skip, dw, True, None, False)
+            ext().embedding_bwd(dy2, flat, pos, period, scale, start, skip, None, False, dp, True)
+        else:
+            ext().embedding_bwd(dy2, flat, pos, period, scale, start, skip, dw, dw_add, dp, dp_add)
+        return None if dw_add else dw, None if dp_add else dp, None, None, None, None, None
 
 
 def _embedding_torch(ids, weight, padding_idx, scale, vocab_start, position_ids, position_weight):

@@ -224,13 +224,18 @@ def mt_norms(lst, role, out, maxabs=False, scale=1.0):
 _GRAD_TYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
-def _grad_list(tensors, norm_type, scale):
+def _no_gaps(t):
+    """A tensor's elements fill one stretch of memory, in any order of its dimensions."""
+    want = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if st != want:
+            return False
+        want *= n
+    return True
+
+
+def _norm_args(tensors, norm_type, scale):
     tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
-    for t in tensors:
-        if not torch.is_tensor(t) or t.layout != torch.strided or t.dtype not in _GRAD_TYPES:
-            raise SMPInvalidArgumentError("gradients must be strided fp32 / fp16 / bf16 tensors")
-        if t.device != tensors[0].device:
-            raise SMPInvalidArgumentError(f"gradients on {t.device} and {tensors[0].device} in one list")
     norm_type, scale = float(norm_type), float(scale)
     if norm_type not in (2.0, math.inf):
         raise SMPInvalidArgumentError(f"norm_type must be 2 or inf, got {norm_type}")
@@ -239,25 +244,35 @@ def _grad_list(tensors, norm_type, scale):
     return tensors, norm_type == math.inf, scale
 
 
-def _dense(t):
-    """The tensor, or a copy of it without gaps (a slice, an expanded view)."""
-    return t if t.is_contiguous() or _no_gaps(t) else t.contiguous()
+def _grad_norm_hip(tensors, inf, scale, out=None, max_norm=0.0):
+    """(power, norm) by the kernels, whose binding checks the lists."""
+    try:
+        return ext().grad_norm(tensors, inf, scale, out, max_norm)
+    except (TypeError, ValueError) as e:
+        raise SMPInvalidArgumentError(f"gradients must be strided fp32 / fp16 / bf16 tensors of one device: {e}") from None
 
 
-def _no_gaps(t):
-    dims = sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1)
-    want = 1
-    for st, n in dims:
-        if st != want:
-            return False
-        want *= n
-    return True
+def _on_gpu(tensors):
+    return torch.is_tensor(tensors[0]) and tensors[0].is_cuda
 
 
-def _check_disjoint(src, dest):
-    """Gap-free tensors of the lists that share memory are refused (the GPU binding does the same)."""
+def _check_grads_cpu(tensors, dest=None):
+    for t in tensors:
+        if not torch.is_tensor(t) or t.layout != torch.strided or t.dtype not in _GRAD_TYPES:
+            raise SMPInvalidArgumentError("gradients must be strided fp32 / fp16 / bf16 tensors")
+        if t.device != tensors[0].device:
+            raise SMPInvalidArgumentError(f"gradients on {t.device} and {tensors[0].device} in one list")
+    if dest is None:
+        return
+    if len(dest) != len(tensors):
+        raise SMPInvalidArgumentError(f"{len(tensors)} gradients, {len(dest)} outputs")
     spans = []
-    for s, d in zip(src, dest):
+    for s, d in zip(tensors, dest):
+        if not torch.is_tensor(d) or d.shape != s.shape or d.dtype not in _GRAD_TYPES or d.device != s.device:
+            raise SMPInvalidArgumentError("outputs must be fp32 / fp16 / bf16 tensors of the gradients' shapes and device")
+        if any(st == 0 and n > 1 for st, n in zip(d.stride(), d.shape)):
+            raise SMPInvalidArgumentError("an expanded tensor cannot be written")
+        # (tensors with gaps, such as two column slices of one matrix, interleave without sharing an element)
         for t, write in ((d, True), (s, False)):
             if t.numel() and _no_gaps(t) and (write or t.data_ptr() != d.data_ptr() or t.dtype != d.dtype):
                 spans.append((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), write))
@@ -269,16 +284,7 @@ def _check_disjoint(src, dest):
         write_end = max(write_end, hi) if write else write_end
 
 
-@torch.no_grad()
-def grad_power(tensors, norm_type=2.0, scale=1.0):
-    """``sum (scale * g)^2`` over all tensors (``norm_type=inf``: ``max |scale * g|``) as a fp64
-    tensor of one element: what ranks that hold different gradients sum (or take the maximum of)
-    before the root.  A list without tensors gives zero, on the CPU."""
-    tensors, inf, scale = _grad_list(tensors, norm_type, scale)
-    if not tensors:
-        return torch.zeros(1, dtype=torch.float64)
-    if tensors[0].is_cuda:
-        return ext().grad_norm([_dense(t) for t in tensors], inf, scale)[0]
+def _grad_power_cpu(tensors, inf, scale):
     if inf:
         tops = [t.abs().max().double() for t in tensors if t.numel()]
         return (torch.stack(tops).max() if tops else torch.zeros((), dtype=torch.float64)).view(1) * scale
@@ -286,12 +292,32 @@ def grad_power(tensors, norm_type=2.0, scale=1.0):
 
 
 @torch.no_grad()
+def grad_power(tensors, norm_type=2.0, scale=1.0):
+    """``sum (scale * g)^2`` over all tensors (``norm_type=inf``: ``max |scale * g|``) as a fp64
+    tensor of one element: what ranks that hold different gradients sum (or take the maximum of)
+    before the root.  A list without tensors gives zero, on the CPU."""
+    tensors, inf, scale = _norm_args(tensors, norm_type, scale)
+    if not tensors:
+        return torch.zeros(1, dtype=torch.float64)
+    if _on_gpu(tensors):
+        return _grad_norm_hip(tensors, inf, scale)[0]
+    _check_grads_cpu(tensors)
+    return _grad_power_cpu(tensors, inf, scale)
+
+
+@torch.no_grad()
 def grad_norm(tensors, norm_type=2.0, scale=1.0):
     """L2 (or, ``norm_type=inf``, largest-value) norm of all elements of a list of tensors, times
     ``scale``: a fp32 scalar tensor, the same bits on every run, no host synchronisation.  The
     tensors may be of different types (fp32 / fp16 / bf16); a NaN anywhere gives NaN."""
-    power = grad_power(tensors, norm_type, scale)
-    return (power[0] if float(norm_type) == math.inf else power[0].sqrt()).float()
+    tensors, inf, scale = _norm_args(tensors, norm_type, scale)
+    if not tensors:
+        return torch.zeros((), dtype=torch.float32)
+    if _on_gpu(tensors):
+        return _grad_norm_hip(tensors, inf, scale)[1]
+    _check_grads_cpu(tensors)
+    power = _grad_power_cpu(tensors, inf, scale)[0]
+    return (power if inf else power.sqrt()).float()
 
 
 @torch.no_grad()
@@ -302,39 +328,19 @@ def clip_grad_norm_(tensors, max_norm, norm_type=2.0, scale=1.0, out=None):
     types: fp16 gradients into fp32 master gradients).  No host synchronisation: a norm that is
     not finite gives what the multiplication by 0 (infinite norm) or NaN gives, as
     ``torch.nn.utils.clip_grad_norm_`` does.  No two tensors of the lists may share memory."""
-    tensors, inf, scale = _grad_list(tensors, norm_type, scale)
+    tensors, inf, scale = _norm_args(tensors, norm_type, scale)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise SMPInvalidArgumentError(f"max_norm must not be negative or NaN, got {max_norm}")
-    dest = tensors
-    if out is not None:
-        dest = [out] if torch.is_tensor(out) else list(out)
-        if len(dest) != len(tensors):
-            raise SMPInvalidArgumentError(f"{len(tensors)} gradients, {len(dest)} outputs")
-        for t, o in zip(tensors, dest):
-            if not torch.is_tensor(o) or o.shape != t.shape or o.dtype not in _GRAD_TYPES or o.device != t.device:
-                raise SMPInvalidArgumentError("outputs must be fp32 / fp16 / bf16 tensors of the gradients' shapes "
-                                              "and device")
-    for o in dest:
-        if any(st == 0 and n > 1 for st, n in zip(o.stride(), o.shape)):
-            raise SMPInvalidArgumentError("an expanded tensor cannot be written")
+    dest = tensors if out is None else [out] if torch.is_tensor(out) else list(out)
     if not tensors:
+        if dest:
+            raise SMPInvalidArgumentError(f"no gradients, {len(dest)} outputs")
         return torch.zeros((), dtype=torch.float32)
-    if tensors[0].is_cuda:
-        src = [_dense(t) for t in tensors]
-        # where the output is laid out otherwise than its gradient (or has gaps), it is written by a copy
-        to = [o if o.stride() == s.stride() and _no_gaps(o) else torch.empty_like(s, dtype=o.dtype)
-              for s, o in zip(src, dest)]
-        try:
-            norm = ext().grad_norm(src, inf, scale, to, max_norm)[1]
-        except ValueError as e:
-            raise SMPInvalidArgumentError(str(e)) from None
-        for o, d in zip(dest, to):
-            if d is not o:
-                o.copy_(d)
-        return norm
-    _check_disjoint(tensors, dest)
-    power = grad_power(tensors, norm_type, scale)[0]
+    if _on_gpu(tensors):
+        return _grad_norm_hip(tensors, inf, scale, dest, max_norm)[1]
+    _check_grads_cpu(tensors, dest)
+    power = _grad_power_cpu(tensors, inf, scale)[0]
     norm = power if inf else power.sqrt()
     f = (max_norm / (norm + 1e-6)).clamp(max=1.0).mul(scale).float()
     for t, o in zip(tensors, dest):

@@ -201,6 +201,23 @@ def test_bound_gradient_accumulates_in_place(dtype, n):
         assert torch.equal(t.grad[~seen], before[t][~seen])
 
 
+def test_one_parameter_as_both_tables():
+    """Bound and dense gradients of a table that serves for tokens and positions alike."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    g = torch.Generator(device="cuda").manual_seed(8)
+    ids = torch.randint(0, 50, (6, 40), generator=g, device="cuda")
+    pos = torch.arange(40, device="cuda").expand(6, 40)
+    dy = torch.randn(6, 40, 520, generator=g, device="cuda")
+    w = torch.nn.Parameter(torch.randn(50, 520, generator=g, device="cuda"))
+    total, slack = (a + b for a, b in zip(table_grad(ids, dy, 50, 2.0), table_grad(pos, dy, 50, 1.0)))
+    (dw,) = torch.autograd.grad(embedding(ids, w, scale=2.0, position_weight=w), w, dy)
+    within(dw, total, 2 * slack)
+    w.grad, w._smp_fused_grad = torch.zeros_like(w), True
+    embedding(ids, w, scale=2.0, position_weight=w).backward(dy)
+    within(w.grad, total, 2 * slack)
+
+
 def test_same_bits_on_every_run_and_stream():
     g1 = check(8, 1000, 500, 200, torch.float32, seed=5)
     side = torch.cuda.Stream()
