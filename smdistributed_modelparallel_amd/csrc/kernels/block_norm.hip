@@ -168,31 +168,31 @@ __global__ void __launch_bounds__(1024) block_norm_fwd(BlockNormArgs a, int team
   }
 }
 
-// A unit (one team) takes rows of one gate row only.  split > 1: `split` units share the rows of
-// a gate row; split == 1: a unit takes whole gate rows, `units` apart.
-struct Turn {
-  int64_t row;
-  bool live, last;  // last: the gate row ends with this row (split == 1)
-  int64_t gate;
-};
-__device__ __forceinline__ Turn turn_of(const BlockNormArgs& a, int64_t unit, int64_t units, int64_t i) {
-  Turn t;
-  const int64_t groups = a.rows / a.gate_rows;
-  if (a.split > 1) {
-    const int64_t chunk = (a.gate_rows + a.split - 1) / a.split, j = unit % a.split * chunk + i;
-    t.gate = unit / a.split;
-    t.live = t.gate < groups && i < chunk && j < a.gate_rows;
-    t.row = t.gate * a.gate_rows + j;
-    t.last = false;
-  } else {
-    const int64_t j = i % a.gate_rows;
-    t.gate = unit + i / a.gate_rows * units;
-    t.live = t.gate < groups;
-    t.row = t.gate * a.gate_rows + j;
-    t.last = j == a.gate_rows - 1;
+// A unit (one team) takes consecutive rows of one gate row.  split > 1: `split` units share the rows
+// of a gate row; split == 1: a unit takes whole gate rows, `units` apart.
+struct Walk {
+  int64_t row, gate;
+  int64_t at, count;  // at-th of the unit's `count` rows of this gate row
+  bool live;
+  __device__ __forceinline__ Walk(const BlockNormArgs& a, int64_t unit) {
+    const int64_t chunk = (a.gate_rows + a.split - 1) / a.split, first = unit % a.split * chunk;
+    gate = unit / a.split;
+    at = 0;
+    count = a.gate_rows - first < chunk ? a.gate_rows - first : chunk;
+    live = gate < a.groups && count > 0;
+    row = gate * a.gate_rows + first;
   }
-  return t;
-}
+  // the gate row ends with this row, and all of it was this unit's
+  __device__ __forceinline__ bool last(const BlockNormArgs& a) const { return a.split == 1 && at == count - 1; }
+  __device__ __forceinline__ void next(const BlockNormArgs& a, int64_t units) {
+    ++row;
+    if (++at < count) return;
+    at = 0;
+    gate += units;
+    row = gate * a.gate_rows;
+    live = live && a.split == 1 && gate < a.groups;
+  }
+};
 
 enum { kW1, kB1, kW2, kB2, kG, kSums };
 
@@ -204,7 +204,7 @@ struct RowData {
 };
 
 template <typename T, int V, bool FULL>
-__device__ __forceinline__ void fetch(const BlockNormArgs& a, const Turn& t, int team_size, int lane, RowData<T, V>& r) {
+__device__ __forceinline__ void fetch(const BlockNormArgs& a, const Walk& t, int team_size, int lane, RowData<T, V>& r) {
   if (!t.live) return;
   r.st = reinterpret_cast<const float4*>(a.stats)[t.row];
 #pragma unroll
@@ -223,7 +223,8 @@ __device__ __forceinline__ void fetch(const BlockNormArgs& a, const Turn& t, int
 template <typename T, typename W, int V, bool FULL, int THREADS>
 __global__ void __launch_bounds__(THREADS) block_norm_bwd(BlockNormArgs a, int team_size, int64_t iterations) {
   extern __shared__ float lds[];  // [64] reductions, then [team_size * kCols * V] to join the teams' sums
-  const int tid = threadIdx.x, teams = blockDim.x / team_size, lane = tid % team_size, tm = tid / team_size;
+  const int tid = threadIdx.x, teams = blockDim.x / team_size;
+  const int tm = __builtin_amdgcn_readfirstlane(tid / team_size), lane = tid - tm * team_size;  // (whole waves)
   Team team{lds, tm * (team_size / 64), team_size / 64, 0};
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * teams + tm, units = static_cast<int64_t>(gridDim.x) * teams;
   float sum[kSums][V][kCols];
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(THREADS) block_norm_bwd(BlockNormArgs a, int t
   }
   int64_t gate_now = -1;
   RowData<T, V> r;
-  Turn t = turn_of(a, unit, units, 0);
+  Walk t(a, unit);
   fetch<T, V, FULL>(a, t, team_size, lane, r);
 
   for (int64_t i = 0; i < iterations; ++i) {
@@ -299,11 +300,10 @@ __global__ void __launch_bounds__(THREADS) block_norm_bwd(BlockNormArgs a, int t
         }
       }
     }
-    const Turn now = t;
-    if (i + 1 < iterations) {
-      t = turn_of(a, unit, units, i + 1);
-      fetch<T, V, FULL>(a, t, team_size, lane, r);
-    }
+    const Walk now = t;
+    const bool last = now.last(a);
+    t.next(a, units);
+    if (i + 1 < iterations) fetch<T, V, FULL>(a, t, team_size, lane, r);
     if (a.dy != nullptr) {
       team.sum2(p, q);
       p = a.rms ? 0.f : p / a.d;
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(THREADS) block_norm_bwd(BlockNormArgs a, int t
         for (int j = 0; j < kCols; ++j) ds[k][j] = st.w * (ds[k][j] - u - n2[k][j] * v);
         write8<FULL, true>(static_cast<T*>(a.dx) + now.row * a.d + c, left[k], ds[k]);
       }
-      if (a.gate_direct && now.last) {  // a whole gate row's sum is complete
+      if (a.gate_direct && last) {  // a whole gate row's sum is complete
 #pragma unroll
         for (int j = 0; j < kCols; ++j) sum[kG][k][j] *= a.alpha;
         if (a.gate_f32) {
@@ -469,9 +469,9 @@ int block_norm_bwd_plan(int64_t rows, int64_t d, int64_t gate_rows, BlockNormPla
   if (d < 1 || d > kMaxWidth || rows < 1) return -4;
   int v;
   p.team = team_of(d, v);
-  const int teams = p.team >= 512 ? 1 : 512 / p.team;  // LDS joins their sums: fewer partial rows than units
+  const int teams = p.team >= 256 ? 1 : 256 / p.team;  // LDS joins their sums: fewer partial rows than units
   p.threads = p.team * teams;
-  int64_t units = 512 * teams;  // two blocks for each CU
+  int64_t units = (p.team > 256 ? 512 : 768) * teams;
   if (units > rows) units = rows;
   const int64_t groups = rows / gate_rows;
   p.split = units / groups;

@@ -12,7 +12,10 @@ namespace smpk {
 namespace {
 
 constexpr int kT = 256;
-constexpr int64_t kShortSort = 16384;  // tokens that one block sorts alone
+// Longest list that is ordered in one launch: 8192 ids of a vocabulary of 12608 take 14 us so, and
+// 19 us in one block's registers; 65536 ids of 50257 take 80 us, and 28 us in radix passes.
+constexpr int64_t kRangeTokens = 16384;
+constexpr int64_t kRangeBlocks = 256;  // blocks of that launch: one for each CU
 
 // Row of a table for one token, or -1 where the id is not one of its rows.
 __device__ __forceinline__ int64_t row_of(const IndexList& l, int64_t t) {
@@ -146,7 +149,9 @@ constexpr int kRounds = 8;  // 64-item rounds of a wave: at most 8192 items a bl
 __device__ __forceinline__ int count_items(int digit, bool valid, int bits, int32_t* cnt) {
   const int lane = threadIdx.x & 63;
   uint64_t same = __ballot(valid);  // the lanes with this lane's digit
-  for (int b = 0; b < bits; ++b) {
+  const int one = __builtin_amdgcn_readlane(digit, __ffsll(static_cast<unsigned long long>(same | 1ull << 63)) - 1);
+  const int steps = __ballot(valid && digit != one) == 0 ? 0 : bits;  // runs of one token need no matching
+  for (int b = 0; b < steps; ++b) {
     const uint32_t mine = static_cast<uint32_t>(static_cast<int32_t>(static_cast<uint32_t>(digit) << (31 - b)) >> 31);
     const uint64_t m = __ballot(mine != 0);
     same &= ~(m ^ (static_cast<uint64_t>(mine) << 32 | mine));
@@ -274,60 +279,75 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_place(SortItems a, cons
   }
 }
 
-// All passes over a list of at most R * 1024 items in one block: the items stay in registers and
-// change places through LDS (one CU stores only one scattered 4-byte word a clock to memory).
-constexpr int kShortBits = 8;  // of a pass: the counters and 16384 items fit the 160 KB of LDS
-
-template <int R>
-__global__ void __launch_bounds__(kSortThreads) emb_sort_short(SortItems a, int passes) {
-  __shared__ SortLds<kShortBits> lds;
-  __shared__ uint32_t keys[R * kSortThreads];
-  __shared__ int32_t tokens[R * kSortThreads];
-  const int bins = 1 << a.bits, lane = threadIdx.x & 63, wid = threadIdx.x >> 6, n = static_cast<int>(a.n);
-  const int s = wid * (64 * R) + lane;  // this thread's items are 64 apart
-  uint32_t key[R];
-  int32_t token[R];
-  clear_marks(a, 0, 1);
+// The whole order in one launch, for vocabularies and lists that are not too large: every block
+// owns a range of rows and reads all ids twice -- from the caches, which hold them -- once to count
+// the tokens of its rows (and of the rows before, which say where its part of the list begins),
+// once to place them.  Waves and their items are taken in order, as above.
+template <int BITS>
+__global__ void __launch_bounds__(kSortThreads) emb_sort_ranges(SortItems a, int range) {
+  __shared__ SortLds<BITS> lds;
+  __shared__ int32_t below[kWaves], valid_ids[kWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, bins = 1 << a.bits;
+  const int64_t lo = static_cast<int64_t>(blockIdx.x) * range;
+  for (int d = lane; d < bins; d += 64) lds.cnt[wid][d] = 0;  // (its own wave's: no barrier)
+  const int64_t part = (a.n + kWaves - 1) / kWaves, s = wid * part, e = s + part < a.n ? s + part : a.n;
+  const uint32_t none = static_cast<uint32_t>(a.ids.rows);
+  int less = 0, held = 0;
+  for (int64_t i0 = s; i0 < e; i0 += 64 * kRounds) {
+    uint32_t key[kRounds];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int i = s + r * 64;
-    key[r] = i < n ? key_of(a, i) : 0u;
-    token[r] = i;
-  }
-  for (int p = 0; p < passes; ++p, a.shift += a.bits) {
-    for (int d = lane; d < bins; d += 64) lds.cnt[wid][d] = 0;  // (its own wave's: no barrier)
-    int rank[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (wid * (64 * R) + r * 64 < n)
-        rank[r] = count_items((key[r] >> a.shift) & (bins - 1), s + r * 64 < n, a.bits, lds.cnt[wid]);
-    __syncthreads();
-    counts_to_places(lds, bins, true);
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (s + r * 64 >= n) continue;
-      const int at = lds.cnt[wid][(key[r] >> a.shift) & (bins - 1)] + rank[r];
-      keys[at] = key[r];
-      tokens[at] = token[r];
+    for (int r = 0; r < kRounds; ++r) {
+      const int64_t i = i0 + r * 64 + lane;
+      key[r] = i < e ? key_of(a, i) : none;
     }
-    __syncthreads();
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (s + r * 64 < n) {
-        key[r] = keys[s + r * 64];
-        token[r] = tokens[s + r * 64];
+    for (int r = 0; r < kRounds; ++r) {
+      const int64_t local = static_cast<int64_t>(key[r]) - lo;
+      less += __popcll(__ballot(local < 0));
+      held += __popcll(__ballot(key[r] != none));
+      const bool mine = local >= 0 && local < range && key[r] != none;
+      if (__ballot(mine) != 0) count_items(mine ? static_cast<int>(local) : 0, mine, a.bits, lds.cnt[wid]);
+    }
+  }
+  if (lane == 0) {
+    below[wid] = less;
+    valid_ids[wid] = held;
+  }
+  __syncthreads();
+  int first = 0, live = 0;
+  for (int w = 0; w < kWaves; ++w) {
+    first += below[w];
+    live += valid_ids[w];
+  }
+  if (a.marks != nullptr && tid < range && lo + tid < a.ids.rows) {
+    int total = 0;
+    for (int w = 0; w < kWaves; ++w) total += lds.cnt[w][tid];
+    a.marks[lo + tid] = total != 0;
+  }
+  counts_to_places(lds, bins, true);
+  for (int64_t i0 = s; i0 < e; i0 += 64 * kRounds) {
+    uint32_t key[kRounds];
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      const int64_t i = i0 + r * 64 + lane;
+      key[r] = i < e ? key_of(a, i) : none;
+    }
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      const int64_t local = static_cast<int64_t>(key[r]) - lo;
+      const bool mine = local >= 0 && local < range && key[r] != none;
+      if (__ballot(mine) == 0) continue;
+      const int at = first + count_items(mine ? static_cast<int>(local) : 0, mine, a.bits, lds.cnt[wid]);
+      if (mine) {
+        a.keys_out[at] = key[r];
+        a.tokens_out[at] = static_cast<int32_t>(i0 + r * 64 + lane);
       }
     }
-    __syncthreads();
   }
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int i = s + r * 64;
-    if (i >= n) continue;
-    a.keys_out[i] = key[r];
-    a.tokens_out[i] = token[r];
-    if (a.marks != nullptr && key[r] < a.ids.rows && (i == 0 || keys[i - 1] != key[r])) a.marks[key[r]] = 1;
-  }
+  // the places of the tokens without a row, a part for each block
+  for (int64_t i = live + static_cast<int64_t>(blockIdx.x) * kSortThreads + tid; i < a.n;
+       i += static_cast<int64_t>(gridDim.x) * kSortThreads)
+    a.keys_out[i] = none;
 }
 
 // --------------------------------------------------------------------- sums over the sorted tokens
@@ -362,26 +382,6 @@ __device__ __forceinline__ void write_row(T* p, int left, float (&sum)[kCols], f
   write8<FULL, true>(p, left, sum);
 }
 
-constexpr int kZeroRows = 64;
-
-// A dense gradient: 64 rows x 512 columns a block, of which the rows without a token are cleared
-// (marks null: the rows from `period` on).
-template <bool FULL, typename T>
-__device__ __forceinline__ void clear_rows(const Sorted& l, const uint8_t* marks, int64_t block, int slabs, T* dw,
-                                           int d) {
-  const int lane = threadIdx.x & 63;
-  const int64_t window = block / slabs, r0 = window * kZeroRows, mine = r0 + lane;
-  const int c = (static_cast<int>(block - window * slabs) * 64 + lane) * kCols;
-  const bool empty = mine < l.rows && (l.n == 0 || (marks != nullptr ? marks[mine] == 0 : mine >= l.period));
-  uint64_t rows = __ballot(empty);  // the same in all waves, which take every fourth of them
-  const float zero[kCols] = {};
-  for (int k = 0; rows != 0; ++k, rows &= rows - 1) {
-    if (k % (kT / 64) != static_cast<int>(threadIdx.x >> 6)) continue;
-    const int64_t r = r0 + __ffsll(static_cast<unsigned long long>(rows)) - 1;
-    if (c < d) write8<FULL, true>(dw + r * d + c, d - c, zero);
-  }
-}
-
 // What a launch has to do for one table: blocks [first, first + blocks) add up its tokens, then
 // [clear, clear + clears) clear rows.
 struct Work {
@@ -392,7 +392,34 @@ struct Work {
   float scale;
   int accumulate, chunk;
   int64_t first, blocks, clear, clears;
+  int stream;  // zeros past the caches
 };
+
+constexpr int kZeroRows = 16;
+
+// A dense gradient: 16 rows x 512 columns a block, of which the rows without a token are cleared
+// (marks null: the rows from `period` on).
+template <bool FULL, typename T>
+__device__ __forceinline__ void clear_rows(const Work& wk, int64_t block, int slabs, T* dw, int d) {
+  const Sorted& l = wk.l;
+  const uint8_t* marks = wk.marks;
+  const int lane = threadIdx.x & 63;
+  const int64_t window = block / slabs, r0 = window * kZeroRows, mine = r0 + lane;
+  const int c = (static_cast<int>(block - window * slabs) * 64 + lane) * kCols;
+  const bool empty = lane < kZeroRows && mine < l.rows && (l.n == 0 || (marks != nullptr ? marks[mine] == 0 : mine >= l.period));
+  uint64_t rows = __ballot(empty);  // the same in all waves, which take every fourth of them
+  const float zero[kCols] = {};
+  for (int k = 0; rows != 0; ++k, rows &= rows - 1) {
+    if (k % (kT / 64) != static_cast<int>(threadIdx.x >> 6)) continue;
+    const int64_t r = r0 + __ffsll(static_cast<unsigned long long>(rows)) - 1;
+    if (c >= d) continue;
+    if (wk.stream) {
+      write8<FULL, true>(dw + r * d + c, d - c, zero);
+    } else {
+      write8<FULL, false>(dw + r * d + c, d - c, zero);
+    }
+  }
+}
 
 __device__ __forceinline__ Work work_of(const Work& a, const Work& b) {
   const int64_t i = blockIdx.x;
@@ -412,7 +439,7 @@ __global__ void __launch_bounds__(kT) emb_bwd_wide(Work w0, Work w1, const T* __
   const float scale = wk.scale;
   const int accumulate = wk.accumulate, chunk = wk.chunk;
   if (static_cast<int64_t>(blockIdx.x) >= wk.clear) {
-    clear_rows<FULL>(l, wk.marks, blockIdx.x - wk.clear, slabs, dw, d);
+    clear_rows<FULL>(wk, blockIdx.x - wk.clear, slabs, dw, d);
     return;
   }
   const int lane = threadIdx.x & 63;
@@ -495,7 +522,7 @@ __global__ void __launch_bounds__(kT) emb_bwd_narrow(Work w0, Work w1, const T* 
   const float scale = wk.scale;
   const int accumulate = wk.accumulate, chunk = wk.chunk;
   if (static_cast<int64_t>(blockIdx.x) >= wk.clear) {
-    clear_rows<FULL>(l, wk.marks, blockIdx.x - wk.clear, 1, dw, d);
+    clear_rows<FULL>(wk, blockIdx.x - wk.clear, 1, dw, d);
     return;
   }
   const int64_t ch = (static_cast<int64_t>(blockIdx.x) - wk.first) * (kT / lanes) + threadIdx.x / lanes;
@@ -549,6 +576,7 @@ __global__ void __launch_bounds__(kT) emb_bwd_narrow(Work w0, Work w1, const T* 
 template <typename T, bool FULL>
 __global__ void __launch_bounds__(kT) emb_bwd_join(Sorted l, const float* __restrict__ part, int d, int chunk, int lanes,
                                                    float scale, T* __restrict__ dw, int accumulate) {
+  constexpr int kBatch = 4;
   __shared__ float buf[kT][kCols];
   const int tid = threadIdx.x, lane = tid % lanes, g = tid / lanes, groups = kT / lanes;
   const int c = (blockIdx.y * lanes + lane) * kCols, left = d - c;
@@ -568,11 +596,19 @@ __global__ void __launch_bounds__(kT) emb_bwd_join(Sorted l, const float* __rest
 #pragma unroll
   for (int q = 0; q < kCols; ++q) sum[q] = 0.f;
   if (left > 0) {
-    for (int64_t m = ch + g; m <= last; m += groups) {
-      Raw8<float> r;
-      read8<FULL>(part + (2 * m + (m == ch ? 1 : 0)) * d + c, left, r);
+    for (int64_t m = ch + g; m <= last; m += kBatch * groups) {
+      Raw8<float> r[kBatch];
 #pragma unroll
-      for (int q = 0; q < kCols; ++q) sum[q] += at8(r, q);
+      for (int u = 0; u < kBatch; ++u) {
+        const int64_t k0 = m + u * groups < last ? m + u * groups : last;  // (past the end: dropped)
+        read8<FULL>(part + (2 * k0 + (k0 == ch ? 1 : 0)) * d + c, left, r[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        if (m + u * groups > last) break;
+#pragma unroll
+        for (int q = 0; q < kCols; ++q) sum[q] += at8(r[u], q);
+      }
     }
   }
 #pragma unroll
@@ -607,25 +643,35 @@ int embedding_fwd(int dt, const IndexList& ids, const void* w, int64_t w_stride,
 }
 
 EmbeddingPlan embedding_bwd_plan(int64_t n, int64_t d, int64_t rows, int64_t batch) {
-  const bool sorted = batch > 0;
-  EmbeddingPlan p;
+  const bool sorted = batch > 0 || n <= 0;
+  EmbeddingPlan p{};
   int bits = 1;
   while ((rows >> bits) != 0) ++bits;  // the keys 0 .. rows
-  const int most = n <= kShortSort ? kShortBits : kMaxBits;
-  p.passes = sorted ? 0 : (bits + most - 1) / most;
-  p.bits = sorted ? 0 : (bits + p.passes - 1) / p.passes;
-  // one block sorts a short list alone, in one launch; longer ones go in runs of 2048 tokens or,
-  // above 256 blocks, whose counts every block reads, of up to 8192 (kRounds rounds of 16 waves)
-  constexpr int64_t kMost = kRounds * kSortThreads;
-  int64_t parts = n <= kShortSort ? 1 : (n + 2047) / 2048;
-  if (parts > 256) parts = (n + kMost - 1) / kMost > 256 ? (n + kMost - 1) / kMost : 256;
-  p.per_block = ((n + parts - 1) / parts + kSortThreads - 1) / kSortThreads * kSortThreads;
-  p.sort_blocks = n > 0 ? (n + p.per_block - 1) / p.per_block : 0;
+  p.range = static_cast<int>((rows + kRangeBlocks - 1) / kRangeBlocks);
+  p.one_launch = n <= kRangeTokens && p.range <= 1 << kMaxBits;
+  if (p.one_launch) {
+    bits = 1;
+    while ((1 << bits) < p.range) ++bits;
+    p.passes = 1;
+    p.bits = bits;
+    p.per_block = 0;
+    p.sort_blocks = (rows + p.range - 1) / p.range;
+  } else {
+    p.passes = (bits + kMaxBits - 1) / kMaxBits;
+    p.bits = (bits + p.passes - 1) / p.passes;
+    // runs of 2048 tokens or, above 256 blocks, whose counts every block reads, of up to 8192
+    // (kRounds rounds of 16 waves)
+    constexpr int64_t kMost = kRounds * kSortThreads;
+    int64_t parts = (n + 2047) / 2048;
+    if (parts > 256) parts = (n + kMost - 1) / kMost > 256 ? (n + kMost - 1) / kMost : 256;
+    p.per_block = ((n + parts - 1) / parts + kSortThreads - 1) / kSortThreads * kSortThreads;
+    p.sort_blocks = (n + p.per_block - 1) / p.per_block;
+  }
   int64_t c = 16;  // tokens of a chunk: long ones leave fewer partial sums, short ones more to run at once
   while (c < 64 && n / (c * 2) >= 1024) c *= 2;
   // positions of up to 64 sequences: whole runs in a chunk, which leave nothing to join
   p.join = !(sorted && batch <= 64);
-  if (!p.join) c = c < batch ? batch : c / batch * batch;
+  if (!p.join && batch > 0) c = c < batch ? batch : c / batch * batch;
   p.chunk = static_cast<int>(c);
   p.chunks = (n + c - 1) / c;
   return p;
@@ -650,12 +696,9 @@ int sort_tokens(const EmbeddingGrad& t, int64_t n, Sorted& l, hipStream_t s) {
   a.keys_out = t.keys;
   a.tokens_out = t.tokens;
   a.marks = t.accumulate ? nullptr : t.marks;
-  if (p.sort_blocks == 1) {
-    const auto kernel = n <= 2 * kSortThreads   ? emb_sort_short<2>
-                        : n <= 4 * kSortThreads ? emb_sort_short<4>
-                        : n <= 8 * kSortThreads ? emb_sort_short<8>
-                                                : emb_sort_short<16>;
-    kernel<<<1, kSortThreads, 0, s>>>(a, p.passes);
+  if (p.one_launch) {
+    const auto kernel = p.bits <= 8 ? emb_sort_ranges<8> : emb_sort_ranges<kMaxBits>;
+    kernel<<<static_cast<unsigned>(p.sort_blocks), kSortThreads, 0, s>>>(a, p.range);
   } else {
     for (int q = 0; q < p.passes; ++q) {
       const int to = (p.passes - 1 - q) & 1;
@@ -680,7 +723,9 @@ int embedding_bwd(int dt, const void* dy, int64_t n, int64_t d, const EmbeddingG
   int lanes = 1;  // of a narrow chunk, and of a joining block's column slab
   while (lanes < kT && lanes * kCols < d) lanes *= 2;
   const bool wide = lanes >= 64, full = d % kCols == 0;
-  const int64_t slabs = (d + 64 * kCols - 1) / (64 * kCols), join_slabs = (d + lanes * kCols - 1) / (lanes * kCols);
+  const int join_lanes = wide ? 64 : lanes;  // four partial rows at once
+  const int64_t slabs = (d + 64 * kCols - 1) / (64 * kCols);
+  const int64_t join_slabs = (d + join_lanes * kCols - 1) / (join_lanes * kCols);
   const int64_t units = wide ? kT / 64 : kT / lanes;
   Work w[2];
   int64_t grid = 0;
@@ -694,6 +739,9 @@ int embedding_bwd(int dt, const void* dy, int64_t n, int64_t d, const EmbeddingG
     w[i].scale = t.scale;
     w[i].accumulate = t.accumulate;
     w[i].chunk = t.plan.chunk;
+    // cleared rows of a table that the caches hold (256 MB, of which the reads need a part) go through
+    // them: 62 MB 15.7 us against 21.7 us past them; 155 MB 35.2 us against 28.9 us
+    w[i].stream = w[i].l.rows * d * (dt == F32 ? 4 : 2) > (96ll << 20);
     w[i].first = grid;
     w[i].blocks = ((wide ? t.plan.chunks * slabs : t.plan.chunks) + units - 1) / units;
     grid += w[i].blocks;
@@ -725,7 +773,7 @@ int embedding_bwd(int dt, const void* dy, int64_t n, int64_t d, const EmbeddingG
       if (!p.join || p.chunks <= 1) continue;
       const auto kernel = full ? emb_bwd_join<T, true> : emb_bwd_join<T, false>;
       kernel<<<dim3(static_cast<unsigned>(p.chunks), static_cast<unsigned>(join_slabs)), kT, 0, s>>>(
-          w[i].l, w[i].part, static_cast<int>(d), p.chunk, lanes, w[i].scale, static_cast<T*>(w[i].dw),
+          w[i].l, w[i].part, static_cast<int>(d), p.chunk, join_lanes, w[i].scale, static_cast<T*>(w[i].dw),
           w[i].accumulate);
     }
   });

@@ -10,14 +10,14 @@
 // finite gradient overflows or underflows the sum, and the conversions stay far below the time
 // of the memory reads.  Maxima are taken on the bits of |g|, whose order as unsigned integers
 // puts infinities above all numbers and NaN above them: a NaN is never lost.
-#include "common.h"
 #include "kernels.h"
+#include "vec8.h"
 
 namespace smpk {
 namespace {
 
 constexpr int kT = 256;
-constexpr int kN = 8;  // elements a thread handles at a time: 16 or 32 bytes
+constexpr int kAhead = 4;  // vectors of 8 elements whose loads a thread has in flight together
 
 struct Chunk {
   int t;          // tensor in the table
@@ -40,28 +40,6 @@ __device__ __forceinline__ Chunk chunk_of(const GradList& l, uint32_t b, int64_t
   c.e = c.s + size < l.n[lo] ? c.s + size : l.n[lo];
   return c;
 }
-
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&o)[kN]) {
-#pragma unroll
-  for (int k = 0; k < kN; k += Vec16<T>::N) {
-    const Vec16<T> a = load16(p + k);
-#pragma unroll
-    for (int j = 0; j < Vec16<T>::N; ++j) o[k + j] = to_f32(a.v[j]);
-  }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&o)[kN]) {
-#pragma unroll
-  for (int k = 0; k < kN; k += Vec16<T>::N) {
-    Vec16<T> a;
-#pragma unroll
-    for (int j = 0; j < Vec16<T>::N; ++j) a.v[j] = from_f32<T>(o[k + j]);
-    store16(p + k, a);
-  }
-}
-
-__device__ __forceinline__ bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
@@ -107,17 +85,23 @@ struct Acc {
 
 template <typename T, bool INF>
 __device__ __forceinline__ void accumulate(const T* p, int64_t n, Acc<INF>& a) {
-  int64_t i = 0;
-  if (aligned(p)) {
-    for (i = static_cast<int64_t>(threadIdx.x) * kN; i + kN <= n; i += kT * kN) {
-      float x[kN];
-      load8(p + i, x);
+  int64_t i = static_cast<int64_t>(threadIdx.x) * kCols;
+  for (; i + (kAhead - 1) * kT * kCols + kCols <= n; i += kAhead * kT * kCols) {
+    Raw8<T> r[kAhead];
 #pragma unroll
-      for (int j = 0; j < kN; ++j) a.add(x[j]);
-    }
-    i = n / kN * kN;
+    for (int u = 0; u < kAhead; ++u) read8<true>(p + i + u * kT * kCols, kCols, r[u]);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) a.add(at8(r[u], j));
   }
-  for (i += threadIdx.x; i < n; i += kT) a.add(to_f32(p[i]));
+  for (; i < n; i += kT * kCols) {
+    const int left = n - i < kCols ? static_cast<int>(n - i) : kCols;
+    float x[kCols];
+    read8<false>(p + i, left, x);  // (zeros past the end)
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) a.add(x[j]);
+  }
 }
 
 template <bool INF>
@@ -140,14 +124,12 @@ __global__ void __launch_bounds__(kT) grad_partials(GradList l, int64_t size, do
   if (threadIdx.x == 0) part[l.first_chunk + blockIdx.x] = v;
 }
 
-// power = scale^2 * sum or scale * max; norm; factor = what each gradient is multiplied by
+// All partials joined by one block, in an order that depends on their number alone, not on the
+// block's: every block of a launch gets the same bits.  Returns scale^2 * sum, or scale * max.
 template <bool INF>
-__global__ void __launch_bounds__(1024) grad_join(const double* __restrict__ part, int64_t n, double scale,
-                                                  double max_norm, double* __restrict__ power,
-                                                  float* __restrict__ norm, float* __restrict__ factor) {
-  __shared__ double smem[16];
+__device__ __forceinline__ double join(const double* part, int64_t n, double scale, double* smem) {
   double v = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) {
+  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
     const double w = part[i];
     if (INF) {
       v = __double_as_longlong(w) > __double_as_longlong(v) ? w : v;
@@ -156,31 +138,52 @@ __global__ void __launch_bounds__(1024) grad_join(const double* __restrict__ par
     }
   }
   v = block_join<INF>(v, smem);
+  return INF ? v * scale : v * scale * scale;
+}
+
+// What each gradient is multiplied by: scale, less where the norm is above max_norm.
+template <bool INF>
+__device__ __forceinline__ float factor_of(double power, double scale, double max_norm) {
+  const double f = max_norm / ((INF ? power : sqrt(power)) + 1e-6);
+  return static_cast<float>((f > 1.0 ? 1.0 : f) * scale);  // (a NaN stays)
+}
+
+template <bool INF>
+__global__ void __launch_bounds__(1024) grad_join(const double* __restrict__ part, int64_t n, double scale,
+                                                  double max_norm, double* __restrict__ power,
+                                                  float* __restrict__ norm, float* __restrict__ factor) {
+  __shared__ double smem[16];
+  const double p = join<INF>(part, n, scale, smem);
   if (threadIdx.x == 0) {
-    const double p = INF ? v * scale : v * scale * scale;
-    const double r = INF ? p : sqrt(p);
     *power = p;
-    *norm = static_cast<float>(r);
-    double f = max_norm / (r + 1e-6);
-    f = f > 1.0 ? 1.0 : f;  // (a NaN stays)
-    if (factor != nullptr) *factor = static_cast<float>(f * scale);
+    *norm = static_cast<float>(INF ? p : sqrt(p));
+    if (factor != nullptr) *factor = factor_of<INF>(p, scale, max_norm);
   }
 }
 
 template <typename T, typename O>
 __device__ __forceinline__ void scale_chunk(const T* p, O* o, int64_t n, float f) {
-  int64_t i = 0;
-  if (aligned(p) && aligned(o)) {
-    for (i = static_cast<int64_t>(threadIdx.x) * kN; i + kN <= n; i += kT * kN) {
-      float x[kN];
-      load8(p + i, x);
+  int64_t i = static_cast<int64_t>(threadIdx.x) * kCols;
+  for (; i + (kAhead - 1) * kT * kCols + kCols <= n; i += kAhead * kT * kCols) {
+    Raw8<T> r[kAhead];
 #pragma unroll
-      for (int j = 0; j < kN; ++j) x[j] *= f;
-      store8(o + i, x);
+    for (int u = 0; u < kAhead; ++u) read8<true>(p + i + u * kT * kCols, kCols, r[u]);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      float x[kCols];
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) x[j] = at8(r[u], j) * f;
+      write8<true, false>(o + i + u * kT * kCols, kCols, x);
     }
-    i = n / kN * kN;
   }
-  for (i += threadIdx.x; i < n; i += kT) o[i] = from_f32<O>(to_f32(p[i]) * f);
+  for (; i < n; i += kT * kCols) {
+    const int left = n - i < kCols ? static_cast<int>(n - i) : kCols;
+    float x[kCols];
+    read8<false>(p + i, left, x);
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) x[j] *= f;
+    write8<false, false>(o + i, left, x);
+  }
 }
 
 template <typename T>
@@ -197,9 +200,9 @@ __device__ __forceinline__ void scale_to(const T* p, void* o, int odt, int64_t s
   }
 }
 
-__global__ void __launch_bounds__(kT) grad_scale(GradList l, int64_t size, const float* __restrict__ factor) {
-  const Chunk c = chunk_of(l, blockIdx.x, size);
-  const float f = *factor;
+// Last chunk first: what the norm read last is what the caches still hold.
+__device__ __forceinline__ void scale_one(const GradList& l, int64_t size, float f) {
+  const Chunk c = chunk_of(l, l.first[l.count] - 1 - blockIdx.x, size);
   const int64_t n = c.e - c.s;
   if (f == 1.f && l.p[c.t] == l.o[c.t]) return;  // in place and within the norm: nothing to change
   switch (l.dt[c.t]) {
@@ -212,6 +215,24 @@ __global__ void __launch_bounds__(kT) grad_scale(GradList l, int64_t size, const
     default:
       scale_to(static_cast<const bf16*>(l.p[c.t]), l.o[c.t], l.odt[c.t], c.s, n, f);
   }
+}
+
+__global__ void __launch_bounds__(kT) grad_scale(GradList l, int64_t size, const float* __restrict__ factor) {
+  scale_one(l, size, *factor);
+}
+
+// The same for few partials: each block joins them itself, which saves the launch of grad_join.
+template <bool INF>
+__global__ void __launch_bounds__(kT) grad_join_scale(GradList l, int64_t size, const double* __restrict__ part,
+                                                      int64_t n, double scale, double max_norm,
+                                                      double* __restrict__ power, float* __restrict__ norm) {
+  __shared__ double smem[kT / 64];
+  const double p = join<INF>(part, n, scale, smem);
+  if (l.first_chunk == 0 && blockIdx.x == 0 && threadIdx.x == 0) {
+    *power = p;
+    *norm = static_cast<float>(INF ? p : sqrt(p));
+  }
+  scale_one(l, size, factor_of<INF>(p, scale, max_norm));
 }
 
 }  // namespace
@@ -247,6 +268,15 @@ int grad_scale(const GradList& l, int64_t size, const float* factor, hipStream_t
   const uint32_t blocks = l.first[l.count];
   if (blocks == 0) return 0;
   grad_scale<<<blocks, kT, 0, s>>>(l, size, factor);
+  return static_cast<int>(hipGetLastError());
+}
+
+int grad_join_scale(const GradList& l, int64_t size, const double* part, int64_t n, int inf, double scale,
+                    double max_norm, double* power, float* norm, hipStream_t s) {
+  const uint32_t blocks = l.first[l.count];
+  if (blocks == 0) return 0;
+  const auto kernel = inf ? grad_join_scale<true> : grad_join_scale<false>;
+  kernel<<<blocks, kT, 0, s>>>(l, size, part, n, scale, max_norm, power, norm);
   return static_cast<int>(hipGetLastError());
 }
 

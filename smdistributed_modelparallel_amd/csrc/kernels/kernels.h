@@ -248,7 +248,7 @@ int embedding_fwd(int dt, const IndexList& ids, const void* w, int64_t w_stride,
 // How the tokens of a table of `rows` rows are gone about; batch > 0: no ids, `batch` sequences of
 // positions.
 struct EmbeddingPlan {
-  int passes, bits, chunk, join;
+  int passes, bits, chunk, join, one_launch, range;
   int64_t per_block, sort_blocks, chunks;
 };
 EmbeddingPlan embedding_bwd_plan(int64_t n, int64_t d, int64_t rows, int64_t batch);
@@ -292,6 +292,10 @@ int grad_partials(const GradList& l, int64_t size, int inf, double* part, hipStr
 // null) = scale * min(1, max_norm / (norm + 1e-6))
 int grad_join(const double* part, int64_t n, int inf, double scale, double max_norm, double* power, float* norm,
               float* factor, hipStream_t s);
+// Partials up to which the blocks of grad_join_scale join them all themselves: two loads a thread.
+constexpr int64_t kGradJoinEach = 512;
+int grad_join_scale(const GradList& l, int64_t size, const double* part, int64_t n, int inf, double scale,
+                    double max_norm, double* power, float* norm, hipStream_t s);
 // o = p * factor
 int grad_scale(const GradList& l, int64_t size, const float* factor, hipStream_t s);
 
@@ -301,7 +305,7 @@ int grad_scale(const GradList& l, int64_t size, const float* factor, hipStream_t
 struct BlockNormArgs {
   const void *x = nullptr, *res = nullptr, *w = nullptr, *b = nullptr, *pw = nullptr, *pb = nullptr, *gate = nullptr;
   int w_f32 = 0, gate_f32 = 0, rms = 0;
-  int64_t rows = 0, gate_rows = 1;
+  int64_t rows = 0, gate_rows = 1, groups = 0;  // groups: rows / gate_rows
   int d = 0;
   float alpha = 1.f, eps = 0.f;
   float* stats = nullptr;  // [rows][4]: mean, 1 / deviation of s, then of x

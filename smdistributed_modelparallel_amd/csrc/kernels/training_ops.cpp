@@ -106,7 +106,8 @@ void embedding_bwd(at::Tensor dy, at::Tensor ids, c10::optional<at::Tensor> pos,
     e.accumulate = i == 0 ? dw_accumulate : dp_accumulate;
     e.plan = smpk::embedding_bwd_plan(n, d, rows, sequence ? std::max<int64_t>(n / period, 1) : 0);
     const bool sort = !sequence && n > 0;
-    const int64_t size[5] = {sort ? 8 * n : 0, sort ? 8 * n : 0, sort ? e.plan.sort_blocks << (e.plan.bits + 2) : 0,
+    const int64_t lists = e.plan.one_launch ? 4 * n : 8 * n;
+    const int64_t size[5] = {sort ? lists : 0, sort ? lists : 0, sort && !e.plan.one_launch ? e.plan.sort_blocks << (e.plan.bits + 2) : 0,
                              e.plan.join ? e.plan.chunks * 8 * d : 0, sort && !e.accumulate ? rows : 0};
     for (int k = 0; k < 5; ++k) {
       at[count][k] = bytes;
@@ -135,9 +136,10 @@ const void* ptr(const Opt& t) { return t.has_value() ? t->data_ptr() : nullptr; 
 // Arguments that the forward and the backward share, checked.
 smpk::BlockNormArgs block_args(const Opt& x, const at::Tensor& res, const at::Tensor& w, const Opt& b, const Opt& pw,
                                const Opt& pb, const Opt& gate, int64_t gate_rows, double alpha, double eps, bool rms) {
-  TORCH_CHECK(res.is_cuda() && res.dim() == 2 && res.is_contiguous(), "block_norm: rows must be a dense matrix");
-  const int64_t d = res.size(1);
+  TORCH_CHECK(res.is_cuda() && res.dim() >= 1 && res.is_contiguous(), "block_norm: rows must be dense");
+  const int64_t d = res.size(-1);
   TORCH_CHECK(d >= 1 && d <= 16384, "block_norm: width ", d, " is not within 1 .. 16384");
+  const int64_t rows = res.numel() / d;
   dt_code(res, "block_norm");
   auto like = [&](const Opt& t) {
     return !t.has_value() || (t->device() == res.device() && t->is_contiguous() && t->sizes() == res.sizes() &&
@@ -152,7 +154,7 @@ smpk::BlockNormArgs block_args(const Opt& x, const at::Tensor& res, const at::Te
   TORCH_CHECK(vec(w) && vec(b) && vec(pw) && vec(pb), "block_norm: weights and biases must be alike");
   if (gate.has_value()) {
     TORCH_CHECK(gate->device() == res.device() && gate->is_contiguous() && gate_rows >= 1 &&
-                    gate->numel() == (res.size(0) + gate_rows - 1) / gate_rows * d && res.size(0) % gate_rows == 0 &&
+                    gate->numel() == rows / gate_rows * d && rows % gate_rows == 0 &&
                     (gate->scalar_type() == res.scalar_type() || gate->scalar_type() == at::kFloat),
                 "block_norm: bad gate");
   }
@@ -167,8 +169,9 @@ smpk::BlockNormArgs block_args(const Opt& x, const at::Tensor& res, const at::Te
   a.w_f32 = w.scalar_type() == at::kFloat;
   a.gate_f32 = gate.has_value() && gate->scalar_type() == at::kFloat;
   a.rms = rms;
-  a.rows = res.size(0);
+  a.rows = rows;
   a.gate_rows = gate.has_value() ? gate_rows : (a.rows < 1 ? 1 : a.rows);
+  a.groups = a.rows / a.gate_rows;
   a.d = static_cast<int>(d);
   a.alpha = static_cast<float>(alpha);
   a.eps = static_cast<float>(eps);
@@ -378,11 +381,21 @@ std::vector<at::Tensor> grad_norm(std::vector<at::Tensor> grads, bool inf, doubl
   float* const factor = reinterpret_cast<float*>(part.data_ptr<double>() + chunks);
   for (const auto& l : lists)
     check(smpk::grad_partials(l, size, inf ? 1 : 0, part.data_ptr<double>(), stream()), "grad_partials");
-  check(smpk::grad_join(part.data_ptr<double>(), chunks, inf ? 1 : 0, scale, max_norm, power.data_ptr<double>(),
-                        norm.data_ptr<float>(), out.has_value() ? factor : nullptr, stream()),
-        "grad_join");
+  const bool each = out.has_value() && chunks > 0 && chunks <= smpk::kGradJoinEach;
+  if (each) {
+    for (const auto& l : lists)
+      check(smpk::grad_join_scale(l, size, part.data_ptr<double>(), chunks, inf ? 1 : 0, scale, max_norm,
+                                  power.data_ptr<double>(), norm.data_ptr<float>(), stream()),
+            "grad_join_scale");
+  } else {
+    check(smpk::grad_join(part.data_ptr<double>(), chunks, inf ? 1 : 0, scale, max_norm, power.data_ptr<double>(),
+                          norm.data_ptr<float>(), out.has_value() ? factor : nullptr, stream()),
+          "grad_join");
+  }
   if (out.has_value()) {
-    for (const auto& l : lists) check(smpk::grad_scale(l, size, factor, stream()), "grad_scale");
+    if (!each)
+      for (auto l = lists.rbegin(); l != lists.rend(); ++l)
+        check(smpk::grad_scale(*l, size, factor, stream()), "grad_scale");
     for (size_t i = 0; i < dest.size(); ++i)
       if (!dest[i].is_same((*out)[i])) (*out)[i].copy_(dest[i]);
   }

@@ -179,11 +179,12 @@ MAX_BLOCK_NORM_WIDTH = 16384
 
 
 class _BlockNorm(torch.autograd.Function):
-    """(y, s) of ``block_norm`` on [rows, d] matrices; ``x`` None: y alone, the norm of residual."""
+    """(y, s) of ``block_norm``; ``x`` None: y alone, the norm of residual."""
 
     @staticmethod
     def forward(ctx, x, residual, weight, bias, post_weight, post_bias, gate, gate_rows, alpha, eps, rms):
         need = any(ctx.needs_input_grad)
+        x, residual = x.contiguous() if x is not None else None, residual.contiguous()
         y, s, stats = ext().block_norm_fwd(x, residual, weight, bias, post_weight, post_bias, gate, gate_rows, alpha,
                                            eps, rms, need)
         if need:
@@ -196,20 +197,18 @@ class _BlockNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, ds=None):
-        *inputs, stats = ctx.saved_tensors
-        need = list(ctx.needs_input_grad[:7])
-        none = (None,) * 11
         if dy is None and ds is None:
-            return none
-        into, bound = [], set()
-        for t, n in zip(inputs[2:], need[2:]):
+            return (None,) * 11
+        *inputs, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad[:7]
+        into, bound = [None] * 5, set()
+        for i, t in enumerate(inputs[2:]):
             # in place into the flat gradient buffer; a parameter used twice only once so
-            bind = n and t is not None and t.is_leaf and _fusable(t) and id(t) not in bound
-            # (the gradient of a gate with many rows may be written without a partial sum)
-            bind = bind and not (t is inputs[6] and t.numel() != t.shape[-1])
-            into.append(t.grad if bind else None)
-            if bind:
-                bound.add(id(t))
+            if need[2 + i] and t.is_leaf and _fusable(t) and id(t) not in bound:
+                # (the gradient of a gate with many rows may be written without a partial sum)
+                if i < 4 or t.numel() == t.shape[-1]:
+                    into[i] = t.grad
+                    bound.add(id(t))
         dy, ds = (t.contiguous() if t is not None else None for t in (dy, ds))
         return (*ext().block_norm_bwd(dy, ds, *inputs, *ctx.args, stats, need, into), None, None, None, None)
 
@@ -291,14 +290,12 @@ def block_norm(x, residual, weight, bias=None, post_weight=None, post_bias=None,
         h = x.float() if post_weight is None else _norm_torch(x.float(), post_weight, post_bias, eps, rms)
         s = residual.float() + residual_scale * (h if gate is None else gate.float() * h)
         return _norm_torch(s, weight, bias, eps, rms).to(x.dtype), s.to(x.dtype)
-    d, run = x.shape[-1], 1
+    run = 1
     if gate is not None:
         gate, run = _gate_matrix(gate if gate.dim() else gate.reshape(1), x.shape)
         gate = gate.contiguous()
     vectors = [t.contiguous() if t is not None else None for t in (weight, bias, post_weight, post_bias)]
-    y, s = _BlockNorm.apply(x.reshape(-1, d).contiguous(), residual.reshape(-1, d).contiguous(), *vectors, gate, run,
-                            residual_scale, eps, bool(rms))
-    return y.view(x.shape), s.view(x.shape)
+    return _BlockNorm.apply(x, residual, *vectors, gate, run, residual_scale, eps, bool(rms))
 
 
 def rms_norm(x, weight, eps=1e-5):
@@ -311,6 +308,4 @@ def rms_norm(x, weight, eps=1e-5):
         raise SMPInvalidArgumentError(f"bad eps {eps}")
     if not fused_ok(x):
         return _norm_torch(x.float(), weight, None, eps, True).to(x.dtype)
-    y = _BlockNorm.apply(None, x.reshape(-1, x.shape[-1]).contiguous(), weight.contiguous(), None, None, None, None, 1,
-                         1.0, eps, True)
-    return y.view(x.shape)
+    return _BlockNorm.apply(None, x, weight.contiguous(), None, None, None, None, 1, 1.0, eps, True)

@@ -88,7 +88,8 @@ def test_sizes(b, s, rows, dim, dtype):
 
 
 @pytest.mark.parametrize("b,s,rows,dim", [(8, 5000, 60000, 16), (3, 16384, 1023, 9), (3, 16384, 1024, 8), (1, 700001, 3000, 8),
-                                          (1, 600000, 1200000, 2), (2, 9000, 2, 3000), (64, 17, 40, 9000)])
+                                          (1, 600000, 1200000, 2), (2, 9000, 2, 3000), (64, 17, 40, 9000),
+                                          (2, 300, 300000, 8), (1, 131072, 262144, 8), (1, 131073, 5000, 16)])
 def test_long_lists(b, s, rows, dim):
     """Lists that many blocks sort, one to three passes, rows of several column slabs."""
     check(b, s, rows, dim, torch.bfloat16, positions="implicit")
