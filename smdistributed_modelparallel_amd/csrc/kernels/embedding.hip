@@ -17,16 +17,11 @@ constexpr int kT = 256;
 constexpr int64_t kRangeTokens = 16384;
 constexpr int64_t kRangeBlocks = 256;  // blocks of that launch: one for each CU
 
-// Row of a table for one token, or -1 where the id is not one of its rows.
-__device__ __forceinline__ int64_t row_of(const IndexList& l, int64_t t) {
-  int64_t id;
-  if (l.ids == nullptr) {
-    id = t % l.period;
-  } else {
-    id = l.wide ? static_cast<const int64_t*>(l.ids)[t] : static_cast<const int32_t*>(l.ids)[t];
-  }
-  id -= l.start;
-  return id >= 0 && id < l.rows ? id : -1;
+// Row of a table for one token of a list with ids; `rows` where the id is not one of its rows.
+__device__ __forceinline__ uint32_t row_of(const IndexList& l, int64_t t) {
+  const int64_t id = l.wide ? static_cast<const int64_t*>(l.ids)[t] : static_cast<const int32_t*>(l.ids)[t];
+  const uint64_t r = static_cast<uint64_t>(id) - static_cast<uint64_t>(l.start);
+  return static_cast<uint32_t>(r < static_cast<uint64_t>(l.rows) ? r : l.rows);
 }
 
 constexpr int kPerThread = 4;  // vectors of a thread, all loads in flight together
@@ -119,7 +114,7 @@ constexpr int kMaxBits = 10;
 
 struct SortItems {
   IndexList ids;  // first pass: keys and tokens come from the ids
-  int64_t skip;
+  uint32_t skip;  // row without a gradient; none of them: `rows`
   const uint32_t* keys;  // later passes (null in the first)
   const int32_t* tokens;
   uint32_t* keys_out;
@@ -132,8 +127,8 @@ struct SortItems {
 // Rows' keys are their numbers; tokens without a row come last, with the key `rows`.
 __device__ __forceinline__ uint32_t key_of(const SortItems& a, int64_t i) {
   if (a.keys != nullptr) return a.keys[i];
-  const int64_t r = row_of(a.ids, i);
-  return static_cast<uint32_t>(r < 0 || r == a.skip ? a.ids.rows : r);
+  const uint32_t r = row_of(a.ids, i);
+  return r == a.skip ? static_cast<uint32_t>(a.ids.rows) : r;
 }
 
 __device__ __forceinline__ void wave_run(const SortItems& a, int block, int64_t& s, int64_t& e) {
@@ -288,10 +283,10 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_ranges(SortItems a, int
   __shared__ SortLds<BITS> lds;
   __shared__ int32_t below[kWaves], valid_ids[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, bins = 1 << a.bits;
-  const int64_t lo = static_cast<int64_t>(blockIdx.x) * range;
+  const uint32_t lo = blockIdx.x * static_cast<uint32_t>(range), none = static_cast<uint32_t>(a.ids.rows);
+  const uint32_t mine_end = none - lo < static_cast<uint32_t>(range) ? none - lo : range;  // its rows: lo + [0, mine_end)
   for (int d = lane; d < bins; d += 64) lds.cnt[wid][d] = 0;  // (its own wave's: no barrier)
   const int64_t part = (a.n + kWaves - 1) / kWaves, s = wid * part, e = s + part < a.n ? s + part : a.n;
-  const uint32_t none = static_cast<uint32_t>(a.ids.rows);
   int less = 0, held = 0;
   for (int64_t i0 = s; i0 < e; i0 += 64 * kRounds) {
     uint32_t key[kRounds];
@@ -302,11 +297,9 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_ranges(SortItems a, int
     }
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
-      const int64_t local = static_cast<int64_t>(key[r]) - lo;
-      less += __popcll(__ballot(local < 0));
+      less += __popcll(__ballot(key[r] < lo));
       held += __popcll(__ballot(key[r] != none));
-      const bool mine = local >= 0 && local < range && key[r] != none;
-      if (__ballot(mine) != 0) count_items(mine ? static_cast<int>(local) : 0, mine, a.bits, lds.cnt[wid]);
+      if (key[r] - lo < mine_end) atomicAdd(&lds.cnt[wid][key[r] - lo], 1);
     }
   }
   if (lane == 0) {
@@ -319,7 +312,7 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_ranges(SortItems a, int
     first += below[w];
     live += valid_ids[w];
   }
-  if (a.marks != nullptr && tid < range && lo + tid < a.ids.rows) {
+  if (a.marks != nullptr && tid < static_cast<int>(mine_end)) {
     int total = 0;
     for (int w = 0; w < kWaves; ++w) total += lds.cnt[w][tid];
     a.marks[lo + tid] = total != 0;
@@ -334,10 +327,9 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_ranges(SortItems a, int
     }
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
-      const int64_t local = static_cast<int64_t>(key[r]) - lo;
-      const bool mine = local >= 0 && local < range && key[r] != none;
+      const bool mine = key[r] - lo < mine_end;
       if (__ballot(mine) == 0) continue;
-      const int at = first + count_items(mine ? static_cast<int>(local) : 0, mine, a.bits, lds.cnt[wid]);
+      const int at = first + count_items(mine ? static_cast<int>(key[r] - lo) : 0, mine, a.bits, lds.cnt[wid]);
       if (mine) {
         a.keys_out[at] = key[r];
         a.tokens_out[at] = static_cast<int32_t>(i0 + r * 64 + lane);
@@ -397,27 +389,33 @@ struct Work {
 
 constexpr int kZeroRows = 16;
 
+// The rows of a bit mask, every fourth of them for this wave, become zero.
+template <bool FULL, bool STREAM, typename T>
+__device__ __forceinline__ void zero_rows(uint64_t rows, T* at, int left, int d) {
+  const float zero[kCols] = {};
+  for (int k = 0; rows != 0; ++k, rows &= rows - 1) {
+    if (k % (kT / 64) != static_cast<int>(threadIdx.x >> 6) || left <= 0) continue;
+    const int64_t r = __ffsll(static_cast<unsigned long long>(rows)) - 1;
+    write8<FULL, STREAM>(at + r * d, left, zero);
+  }
+}
+
 // A dense gradient: 16 rows x 512 columns a block, of which the rows without a token are cleared
 // (marks null: the rows from `period` on).
 template <bool FULL, typename T>
 __device__ __forceinline__ void clear_rows(const Work& wk, int64_t block, int slabs, T* dw, int d) {
   const Sorted& l = wk.l;
-  const uint8_t* marks = wk.marks;
   const int lane = threadIdx.x & 63;
   const int64_t window = block / slabs, r0 = window * kZeroRows, mine = r0 + lane;
   const int c = (static_cast<int>(block - window * slabs) * 64 + lane) * kCols;
-  const bool empty = lane < kZeroRows && mine < l.rows && (l.n == 0 || (marks != nullptr ? marks[mine] == 0 : mine >= l.period));
-  uint64_t rows = __ballot(empty);  // the same in all waves, which take every fourth of them
-  const float zero[kCols] = {};
-  for (int k = 0; rows != 0; ++k, rows &= rows - 1) {
-    if (k % (kT / 64) != static_cast<int>(threadIdx.x >> 6)) continue;
-    const int64_t r = r0 + __ffsll(static_cast<unsigned long long>(rows)) - 1;
-    if (c >= d) continue;
-    if (wk.stream) {
-      write8<FULL, true>(dw + r * d + c, d - c, zero);
-    } else {
-      write8<FULL, false>(dw + r * d + c, d - c, zero);
-    }
+  const bool empty = lane < kZeroRows && mine < l.rows &&
+                     (l.n == 0 || (wk.marks != nullptr ? wk.marks[mine] == 0 : mine >= l.period));
+  const uint64_t rows = __ballot(empty);  // the same in all waves
+  T* const at = dw + r0 * d + c;
+  if (wk.stream) {  // (two loops: the compiler would make one store of two that differ in this alone)
+    zero_rows<FULL, true>(rows, at, d - c, d);
+  } else {
+    zero_rows<FULL, false>(rows, at, d - c, d);
   }
 }
 
@@ -686,7 +684,7 @@ int sort_tokens(const EmbeddingGrad& t, int64_t n, Sorted& l, hipStream_t s) {
   if (t.ids.ids == nullptr || n <= 0) return 0;
   SortItems a;
   a.ids = t.ids;
-  a.skip = t.skip;
+  a.skip = static_cast<uint32_t>(t.skip >= 0 && t.skip < t.ids.rows ? t.skip : t.ids.rows);
   a.keys = nullptr;
   a.tokens = nullptr;
   a.n = n;
