@@ -4,6 +4,8 @@
 
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <algorithm>
 #include <vector>
@@ -11,6 +13,10 @@
 #include "kernels.h"
 
 namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+typedef c10::optional<at::Tensor> Opt;
 
 int dt_code(const at::Tensor& t, const char* name) {
   switch (t.scalar_type()) {
@@ -44,6 +50,10 @@ smpk::IndexList index_list(const c10::optional<at::Tensor>& ids, int64_t n, int6
     l.wide = ids->scalar_type() == at::kLong;
   }
   return l;
+}
+
+void check_table_dims(const at::Tensor& w) {
+  TORCH_CHECK(w.is_cuda() && w.dim() == 2, "embedding: a table must be a GPU matrix");
 }
 
 void check_table(const at::Tensor& w) {
@@ -128,8 +138,91 @@ void embedding_bwd(at::Tensor dy, at::Tensor ids, c10::optional<at::Tensor> pos,
   check(smpk::embedding_bwd(dt_code(dy, "embedding"), dy.data_ptr(), n, d, t, count, stream()), "embedding_bwd");
 }
 
+// The gradient of `t` goes straight into its bound slot of the flat buffer: the caller saw the
+// parameter's mark, the slot has to be there still.
+bool bound(const at::Tensor& t, bool marked) {
+  if (!marked || !t.defined() || !t.is_leaf()) return false;
+  const at::Tensor& g = t.grad();
+  return g.defined() && g.scalar_type() == t.scalar_type() && g.sizes() == t.sizes() && g.is_contiguous();
+}
+
+// Backward passes here launch kernels that autograd does not see: a second derivative is an error.
+variable_list once(variable_list grads, const char* name) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (auto& g : grads)
+    if (g.defined()) g = g.detach().set_requires_grad(true);  // whatever is built on it reaches the error
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      std::string(name) + " cannot be differentiated twice", static_cast<int64_t>(grads.size()));
+  return (*error)(std::move(grads));
+}
+
+// Autograd's nodes are C++: a short call's time is the host's, and the backward needs no interpreter.
+class EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
+ public:
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& weight, const Opt& pos_weight,
+                            const at::Tensor& ids, const Opt& pos, int64_t period, double scale, int64_t start,
+                            bool foreign_zero, int64_t skip, bool mark_w, bool mark_p) {
+    // the tables' values are not needed again: they may change before the backward
+    ctx->saved_data["weight"] = weight;
+    if (pos_weight.has_value()) ctx->saved_data["pos_weight"] = *pos_weight;
+    ctx->save_for_backward({ids, pos.has_value() ? *pos : at::Tensor()});
+    ctx->saved_data["args"] = std::vector<int64_t>{period, start, skip, mark_w, mark_p};
+    ctx->saved_data["scale"] = scale;
+    return embedding_fwd(ids, weight, scale, start, foreign_zero, pos, pos_weight, period);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto args = ctx->saved_data["args"].toIntVector();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const at::Tensor w = ctx->saved_data["weight"].toTensor();
+    const bool two = ctx->saved_data.count("pos_weight") != 0;
+    const at::Tensor p = two ? ctx->saved_data["pos_weight"].toTensor() : at::Tensor();
+    variable_list out(11);
+    const at::Tensor dy = grads[0].reshape({-1, w.size(1)}).contiguous();
+    Opt dw, dp, pos;
+    bool add_w = false, add_p = false;
+    auto target = [&](const at::Tensor& t, bool marked, Opt& g, bool& add, at::Tensor& result) {
+      add = bound(t, marked);
+      g = add ? t.grad() : at::empty(t.sizes(), t.options());
+      if (!add) result = *g;
+    };
+    if (ctx->needs_input_grad(0)) target(w, args[3], dw, add_w, out[0]);
+    if (two && ctx->needs_input_grad(1)) target(p, args[4], dp, add_p, out[1]);
+    if (saved[1].defined()) pos = saved[1];
+    if (add_w && add_p && dw->data_ptr() == dp->data_ptr()) {  // one parameter as both tables: one after the other
+      embedding_bwd(dy, saved[0], pos, args[0], scale, args[1], args[2], dw, true, c10::nullopt, false);
+      embedding_bwd(dy, saved[0], pos, args[0], scale, args[1], args[2], c10::nullopt, false, dp, true);
+    } else {
+      embedding_bwd(dy, saved[0], pos, args[0], scale, args[1], args[2], dw, add_w, dp, add_p);
+    }
+    return once(std::move(out), "embedding");
+  }
+};
+
+// scale * weight[ids - start] (+ pos_weight[pos]) -> [*ids.shape, dim], differentiable in both tables
+at::Tensor embedding(at::Tensor weight, Opt pos_weight, at::Tensor ids, Opt pos, double scale, int64_t start,
+                     bool foreign_zero, int64_t skip, bool mark_w, bool mark_p) {
+  check_table_dims(weight);
+  auto rows_dense = [](const at::Tensor& t) { return t.stride(1) == 1 ? t : t.contiguous(); };
+  auto shape = ids.sizes().vec();
+  shape.push_back(weight.size(1));
+  const int64_t period = pos_weight.has_value() && !pos.has_value() ? ids.size(-1) : 1;
+  const at::Tensor flat = ids.reshape({-1}).contiguous();
+  if (pos.has_value()) pos = pos->reshape({-1}).contiguous();
+  weight = rows_dense(weight);
+  if (pos_weight.has_value()) {
+    check_table_dims(*pos_weight);
+    pos_weight = rows_dense(*pos_weight);
+  }
+  const bool grad = at::GradMode::is_enabled() &&
+                    (weight.requires_grad() || (pos_weight.has_value() && pos_weight->requires_grad()));
+  if (!grad) return embedding_fwd(flat, weight, scale, start, foreign_zero, pos, pos_weight, period).view(shape);
+  return EmbeddingFunction::apply(weight, pos_weight, flat, pos, period, scale, start, foreign_zero, skip, mark_w, mark_p)
+      .view(shape);
+}
+
 // ------------------------------------------------------------------ block norm
-typedef c10::optional<at::Tensor> Opt;
 
 const void* ptr(const Opt& t) { return t.has_value() ? t->data_ptr() : nullptr; }
 
@@ -280,6 +373,79 @@ std::vector<Opt> block_norm_bwd(Opt dy, Opt ds, Opt x, at::Tensor res, at::Tenso
   return out;
 }
 
+class BlockNormFunction : public torch::autograd::Function<BlockNormFunction> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Opt& x, const at::Tensor& res, const at::Tensor& w,
+                               const Opt& b, const Opt& pw, const Opt& pb, const Opt& gate, int64_t gate_rows,
+                               double alpha, double eps, bool rms, std::vector<int64_t> marks) {
+    auto out = block_norm_fwd(x, res, w, b, pw, pb, gate, gate_rows, alpha, eps, rms, true);
+    auto opt = [](const Opt& t) { return t.has_value() ? *t : at::Tensor(); };
+    // s is not kept: the backward forms it again from x and the residual (block_norm.hip)
+    ctx->save_for_backward({opt(x), res, w, opt(b), opt(pw), opt(pb), opt(gate), out[2]});
+    ctx->saved_data["marks"] = marks;
+    ctx->saved_data["gate_rows"] = gate_rows;
+    ctx->saved_data["alpha"] = alpha;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["rms"] = rms;
+    ctx->set_materialize_grads(false);
+    out.resize(x.has_value() ? 2 : 1);
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list result(12);
+    auto opt = [](const at::Tensor& t) { return t.defined() ? Opt(t) : Opt(); };
+    const Opt dy = opt(grads[0].defined() ? grads[0].contiguous() : grads[0]);
+    const Opt ds = grads.size() > 1 ? opt(grads[1].defined() ? grads[1].contiguous() : grads[1]) : Opt();
+    if (!dy.has_value() && !ds.has_value()) return result;
+    const auto v = ctx->get_saved_variables();
+    const auto marks = ctx->saved_data["marks"].toIntVector();
+    std::vector<bool> need(7, false);
+    for (size_t i = 0, edge = 0; i < 7; ++i)  // (autograd counts the tensors that are there)
+      if (v[i].defined()) need[i] = ctx->needs_input_grad(edge++);
+    std::vector<Opt> into(5);
+    for (size_t i = 0; i < 5; ++i) {
+      const at::Tensor& t = v[2 + i];
+      if (!need[2 + i] || !bound(t, marks[i] != 0)) continue;
+      if (i == 4 && t.numel() != t.size(-1)) continue;  // a gate with many rows may be written without a partial sum
+      bool again = false;  // a parameter used twice is added to in place only once
+      for (size_t k = 0; k < i; ++k) again = again || (into[k].has_value() && into[k]->is_same(t.grad()));
+      if (!again) into[i] = t.grad();
+    }
+    const auto out = block_norm_bwd(dy, ds, opt(v[0]), v[1], v[2], opt(v[3]), opt(v[4]), opt(v[5]), opt(v[6]),
+                                    ctx->saved_data["gate_rows"].toInt(), ctx->saved_data["alpha"].toDouble(),
+                                    ctx->saved_data["eps"].toDouble(), ctx->saved_data["rms"].toBool(), v[7], need,
+                                    into);
+    for (size_t i = 0; i < 7; ++i)
+      if (out[i].has_value()) result[i] = *out[i];
+    return once(std::move(result), "block_norm");
+  }
+};
+
+// {y, s} (y alone without x), differentiable in all tensors; marks: which of w, b, pw, pb, gate are
+// parameters bound to the flat gradient buffer
+variable_list block_norm(Opt x, at::Tensor res, at::Tensor w, Opt b, Opt pw, Opt pb, Opt gate, int64_t gate_rows,
+                         double alpha, double eps, bool rms, std::vector<int64_t> marks) {
+  TORCH_CHECK(marks.size() == 5, "block_norm: bad lists");
+  auto dense = [](Opt& t) {
+    if (t.has_value()) t = t->contiguous();
+  };
+  dense(x);
+  dense(b);
+  dense(pw);
+  dense(pb);
+  dense(gate);
+  res = res.contiguous();
+  w = w.contiguous();
+  bool grad = res.requires_grad() || w.requires_grad();
+  for (const Opt* t : {&x, &b, &pw, &pb, &gate}) grad = grad || (t->has_value() && (*t)->requires_grad());
+  if (grad && at::GradMode::is_enabled())
+    return BlockNormFunction::apply(x, res, w, b, pw, pb, gate, gate_rows, alpha, eps, rms, marks);
+  auto out = block_norm_fwd(x, res, w, b, pw, pb, gate, gate_rows, alpha, eps, rms, false);
+  out.resize(x.has_value() ? 2 : 1);
+  return out;
+}
+
 // --------------------------------------------------------------- gradient norm
 // [start, end) of the memory of a dense tensor
 std::pair<uintptr_t, uintptr_t> extent(const at::Tensor& t) {
@@ -405,17 +571,12 @@ std::vector<at::Tensor> grad_norm(std::vector<at::Tensor> grads, bool inf, doubl
 }  // namespace
 
 void register_training_ops(py::module_& m) {
-  m.def("block_norm_fwd", &block_norm_fwd, py::arg("x"), py::arg("res"), py::arg("w"), py::arg("b"), py::arg("pw"),
+  m.def("block_norm", &block_norm, py::arg("x"), py::arg("res"), py::arg("w"), py::arg("b"), py::arg("pw"),
         py::arg("pb"), py::arg("gate"), py::arg("gate_rows"), py::arg("alpha"), py::arg("eps"), py::arg("rms"),
-        py::arg("need_stats"));
-  m.def("block_norm_bwd", &block_norm_bwd, py::arg("dy"), py::arg("ds"), py::arg("x"), py::arg("res"), py::arg("w"),
-        py::arg("b"), py::arg("pw"), py::arg("pb"), py::arg("gate"), py::arg("gate_rows"), py::arg("alpha"),
-        py::arg("eps"), py::arg("rms"), py::arg("stats"), py::arg("need"), py::arg("into"));
+        py::arg("marks"));
   m.def("grad_norm", &grad_norm, py::arg("grads"), py::arg("inf"), py::arg("scale"), py::arg("out") = py::none(),
         py::arg("max_norm") = 0.0);
-  m.def("embedding_fwd", &embedding_fwd, py::arg("ids"), py::arg("weight"), py::arg("scale"), py::arg("start"),
-        py::arg("foreign_zero"), py::arg("pos"), py::arg("pos_weight"), py::arg("period"));
-  m.def("embedding_bwd", &embedding_bwd, py::arg("dy"), py::arg("ids"), py::arg("pos"), py::arg("period"),
-        py::arg("scale"), py::arg("start"), py::arg("skip"), py::arg("dw"), py::arg("dw_accumulate"), py::arg("dp"),
-        py::arg("dp_accumulate"));
+  m.def("embedding", &embedding, py::arg("weight"), py::arg("pos_weight"), py::arg("ids"), py::arg("pos"),
+        py::arg("scale"), py::arg("start"), py::arg("foreign_zero"), py::arg("skip"), py::arg("mark_w"),
+        py::arg("mark_p"));
 }

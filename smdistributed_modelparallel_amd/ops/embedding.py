@@ -4,62 +4,16 @@
 into the tables' dtype, in one kernel (`csrc/kernels/embedding.hip`).  The backward adds the
 gradient rows of each token's occurrences in token order and in fp32 -- the same bits on every
 run -- and writes the parameters' flat-buffer gradients in place where they are bound
-(`parallel/flat.py`): only the rows that occur are touched then, and no dense gradient exists.
+(`parallel/flat.py`): only the rows that occur are touched then, and no dense gradient exists
+(autograd gets none for them; their post-accumulate hooks still fire).
 CPU tensors (and torch.autocast regions) use plain torch operations.
 """
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ..backend.exceptions import SMPInvalidArgumentError
 from ._ext import ext, fused_ok
-from .linear import _fusable
-
-
-def _target(table, needed):
-    """(tensor the gradient goes to, whether it is added there): the bound gradient of a parameter
-    in the flat buffer, else a new tensor; (None, False) if it is not needed."""
-    if not needed:
-        return None, False
-    if table.is_leaf and _fusable(table):
-        return table.grad, True
-    return torch.empty(table.shape, dtype=table.dtype, device=table.device), False
-
-
-class _EmbeddingHIP(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, weight, position_weight, ids, position_ids, padding_idx, scale, vocab_start):
-        flat = ids.reshape(-1).contiguous()
-        pos = position_ids.reshape(-1).contiguous() if position_ids is not None else None
-        period = ids.shape[-1] if position_weight is not None and pos is None else 1
-        start = vocab_start or 0
-        w = weight if weight.stride(1) == 1 else weight.contiguous()
-        pw = position_weight
-        if pw is not None and pw.stride(1) != 1:
-            pw = pw.contiguous()
-        y = ext().embedding_fwd(flat, w, scale, start, vocab_start is not None, pos, pw, period)
-        ctx.save_for_backward(flat, pos)
-        # the tables' values are not needed again: they may change before the backward
-        ctx.tables = (weight, position_weight)
-        ctx.args = (period, scale, start, -1 if padding_idx is None else padding_idx - start)
-        return y.view(*ids.shape, weight.shape[1])
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        flat, pos = ctx.saved_tensors
-        weight, position_weight = ctx.tables
-        period, scale, start, skip = ctx.args
-        dy2 = dy.reshape(-1, weight.shape[1]).contiguous()
-        dw, dw_add = _target(weight, ctx.needs_input_grad[0])
-        dp, dp_add = _target(position_weight, ctx.needs_input_grad[1])
-        if dw_add and dp_add and dw.data_ptr() == dp.data_ptr():  # one parameter as both tables: one after the other
-            ext().embedding_bwd(dy2, flat, pos, period, scale, start, skip, dw, True, None, False)
-            ext().embedding_bwd(dy2, flat, pos, period, scale, start, skip, None, False, dp, True)
-        else:
-            ext().embedding_bwd(dy2, flat, pos, period, scale, start, skip, dw, dw_add, dp, dp_add)
-        return None if dw_add else dw, None if dp_add else dp, None, None, None, None, None
 
 
 def _embedding_torch(ids, weight, padding_idx, scale, vocab_start, position_ids, position_weight):
@@ -136,5 +90,9 @@ def embedding(ids, weight, padding_idx=None, scale=1.0, vocab_start=None, positi
             raise SMPInvalidArgumentError(f"ids {tuple(ids.shape)} need position_ids: the position table has "
                                           f"{position_weight.shape[0]} rows")
     if fused_ok(weight):
-        return _EmbeddingHIP.apply(weight, position_weight, ids, position_ids, padding_idx, scale, vocab_start)
+        start = vocab_start or 0
+        return ext().embedding(weight, position_weight, ids, position_ids, scale, start, vocab_start is not None,
+                               -1 if padding_idx is None else padding_idx - start,
+                               getattr(weight, "_smp_fused_grad", False),
+                               getattr(position_weight, "_smp_fused_grad", False))
     return _embedding_torch(ids, weight, padding_idx, scale, vocab_start, position_ids, position_weight)

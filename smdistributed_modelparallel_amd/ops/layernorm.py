@@ -8,7 +8,6 @@ input / weight dtypes.
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ..backend.exceptions import SMPInvalidArgumentError
 from ._ext import ext, fused_ok
@@ -178,39 +177,11 @@ def add_layer_norm(x, residual, weight, bias, eps=1e-5, dropout_p=0.0, drawn=Non
 MAX_BLOCK_NORM_WIDTH = 16384
 
 
-class _BlockNorm(torch.autograd.Function):
-    """(y, s) of ``block_norm``; ``x`` None: y alone, the norm of residual."""
-
-    @staticmethod
-    def forward(ctx, x, residual, weight, bias, post_weight, post_bias, gate, gate_rows, alpha, eps, rms):
-        need = any(ctx.needs_input_grad)
-        x, residual = x.contiguous() if x is not None else None, residual.contiguous()
-        y, s, stats = ext().block_norm_fwd(x, residual, weight, bias, post_weight, post_bias, gate, gate_rows, alpha,
-                                           eps, rms, need)
-        if need:
-            # s is not kept: the backward forms it again from x and the residual (block_norm.hip)
-            ctx.save_for_backward(x, residual, weight, bias, post_weight, post_bias, gate, stats)
-            ctx.args = (gate_rows, alpha, eps, rms)
-            ctx.set_materialize_grads(False)
-        return (y, s) if x is not None else y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, ds=None):
-        if dy is None and ds is None:
-            return (None,) * 11
-        *inputs, stats = ctx.saved_tensors
-        need = ctx.needs_input_grad[:7]
-        into, bound = [None] * 5, set()
-        for i, t in enumerate(inputs[2:]):
-            # in place into the flat gradient buffer; a parameter used twice only once so
-            if need[2 + i] and t.is_leaf and _fusable(t) and id(t) not in bound:
-                # (the gradient of a gate with many rows may be written without a partial sum)
-                if i < 4 or t.numel() == t.shape[-1]:
-                    into[i] = t.grad
-                    bound.add(id(t))
-        dy, ds = (t.contiguous() if t is not None else None for t in (dy, ds))
-        return (*ext().block_norm_bwd(dy, ds, *inputs, *ctx.args, stats, need, into), None, None, None, None)
+def _block_norm_hip(x, residual, weight, bias, post_weight, post_bias, gate, gate_rows, alpha, eps, rms):
+    """[y, s] by the kernels (x None: [y], the norm of residual); parameters bound to the flat
+    gradient buffer take their gradients there in place."""
+    marks = [int(getattr(t, "_smp_fused_grad", False)) for t in (weight, bias, post_weight, post_bias, gate)]
+    return ext().block_norm(x, residual, weight, bias, post_weight, post_bias, gate, gate_rows, alpha, eps, rms, marks)
 
 
 def _gate_matrix(gate, shape):
@@ -293,9 +264,8 @@ def block_norm(x, residual, weight, bias=None, post_weight=None, post_bias=None,
     run = 1
     if gate is not None:
         gate, run = _gate_matrix(gate if gate.dim() else gate.reshape(1), x.shape)
-        gate = gate.contiguous()
-    vectors = [t.contiguous() if t is not None else None for t in (weight, bias, post_weight, post_bias)]
-    return _BlockNorm.apply(x, residual, *vectors, gate, run, residual_scale, eps, bool(rms))
+    y, s = _block_norm_hip(x, residual, weight, bias, post_weight, post_bias, gate, run, residual_scale, eps, bool(rms))
+    return y, s
 
 
 def rms_norm(x, weight, eps=1e-5):
@@ -308,4 +278,4 @@ def rms_norm(x, weight, eps=1e-5):
         raise SMPInvalidArgumentError(f"bad eps {eps}")
     if not fused_ok(x):
         return _norm_torch(x.float(), weight, None, eps, True).to(x.dtype)
-    return _BlockNorm.apply(None, x, weight.contiguous(), None, None, None, None, 1, 1.0, eps, True)
+    return _block_norm_hip(None, x, weight, None, None, None, None, 1, 1.0, eps, True)[0]

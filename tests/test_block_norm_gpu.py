@@ -193,6 +193,15 @@ def test_bound_gradients_and_a_shared_parameter():
         within(k, p[k].grad, exact + start[k].double(), room + ref.FEW * start[k].double().abs())
 
 
+def test_second_derivatives_are_refused():
+    t = inputs((2, 3, 16), torch.float32, torch.float32, False, True, "none")
+    x = t["x"].requires_grad_()
+    y, _ = call(t, 1.0, 1e-5, False)
+    (dx,) = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        dx.sum().backward()
+
+
 def test_no_rows_on_the_gpu():
     w = torch.ones(8, device="cuda", requires_grad=True)
     x = torch.empty(0, 8, device="cuda", requires_grad=True)

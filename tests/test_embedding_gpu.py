@@ -219,6 +219,28 @@ def test_one_parameter_as_both_tables():
     within(w.grad, total, 2 * slack)
 
 
+def test_second_derivatives_are_refused():
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    w = torch.randn(6, 16, device="cuda", requires_grad=True)
+    dy = torch.ones(2, 16, device="cuda", requires_grad=True)
+    (dw,) = torch.autograd.grad(embedding(torch.tensor([1, 1], device="cuda"), w), w, dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        dw.sum().backward()
+
+
+def test_table_changed_before_the_backward():
+    """The tables' values are not part of the gradient: an optimizer may have changed them."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    w = torch.randn(6, 16, device="cuda", requires_grad=True)
+    y = embedding(torch.tensor([1, 1, 5], device="cuda"), w)
+    with torch.no_grad():
+        w.zero_()
+    (dw,) = torch.autograd.grad(y, w, torch.ones_like(y))
+    assert dw[:, 0].tolist() == [0, 2, 0, 0, 0, 1]
+
+
 def test_same_bits_on_every_run_and_stream():
     g1 = check(8, 1000, 500, 200, torch.float32, seed=5)
     side = torch.cuda.Stream()
