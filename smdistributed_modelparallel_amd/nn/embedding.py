@@ -10,8 +10,8 @@ Uneven splits follow ``get_local_channels``.
 """
 import torch
 import torch.nn as nn
-import torch.nn.functional as F
 
+from ..ops.embedding import lookup
 from .utils import (
     _allgather,
     fwd_allreduce_for_tp,
@@ -61,18 +61,16 @@ class DistributedEmbedding(nn.Module):
 
     def forward(self, ids):
         if self._tp == 1:
-            return F.embedding(ids, self.weight, self.padding_idx)
+            return lookup(ids, self.weight, self.padding_idx)
         b = ids.shape[0]
         full_ids = ids if self.skip_allgather else _allgather(ids, 0)
         if self.vocab_parallel:
-            local = full_ids - self.vocab_start_idx
-            outside = (local < 0) | (local >= self.local_vocab)
-            emb = F.embedding(local.clamp(0, self.local_vocab - 1), self.weight)
-            emb = emb.masked_fill(outside.unsqueeze(-1), 0.0)
+            # ids of the other ranks' shards give zeros here
+            emb = lookup(full_ids, self.weight, vocab_start=self.vocab_start_idx)
             if self.output_full_batch or self.skip_allgather:
                 return fwd_allreduce_for_tp(emb)
             return reduce_scatter_for_tp(emb, 0, split_shapes=[b] * tp_size())
-        emb = F.embedding(full_ids, self.weight, self.padding_idx)  # [B, s, d_local]
+        emb = lookup(full_ids, self.weight, self.padding_idx)  # [B, s, d_local]
         return scatter_and_merge_for_tp(emb, 0, emb.dim() - 1, split_shapes=[b] * tp_size(),
                                         merge_shapes=get_merge_shapes(self.embedding_dim))
 

@@ -39,6 +39,7 @@ from ..ops.dropout import dropout_seed_offset
 from ..ops._ext import fused_ok
 from ..ops.cross_entropy import cross_entropy
 from ..ops.dropout import add3
+from ..ops.embedding import embedding
 from ..ops.dropout import dropout_add as _dropout_add
 from ..ops import linear as _lin
 from ..ops.gelu import bias_gelu
@@ -248,6 +249,21 @@ def _runs_here(module):
     if state.core.pp_size() > 1 and not mm.is_executor(module):
         return False
     return mm.get_checkpoint_activations_config(module) is None
+
+
+# SMP_FUSE_EMBEDDING=0: the embeddings' own modules and a separate sum, the A/B baseline
+_FUSE_EMBEDDING = [os.environ.get("SMP_FUSE_EMBEDDING", "1") != "0"]
+
+
+def _plain_lookup(m):
+    """The module is nothing but a lookup in a table of this process on the GPU: ops.embedding may
+    read its weight without calling it (no hook, option, shard gathering, other stage or checkpoint)."""
+    return (_FUSE_EMBEDDING[0] and type(m) is nn.Embedding and fused_ok(m.weight)
+            and m.weight.dtype in (torch.float32, torch.float16, torch.bfloat16) and m.padding_idx is None
+            and m.max_norm is None and not m.scale_grad_by_freq and not m.sparse
+            and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+            and not nn.modules.module._has_any_global_hook() and state.sdp is None
+            and (state.core is None or state.core.pp_size() == 1) and _runs_here(m))
 
 
 class _LMHeadLinear(nn.Linear):
@@ -942,6 +958,19 @@ class DistributedTransformerLMHead(DistributedModule):
                 if self.tie_input_output_embedding:
                     self.lm_head.weight = self.word_embedding.weight
 
+    def _embed(self, input_ids, position_ids, default_positions):
+        """Token embeddings plus position embeddings: one kernel for both tables where their modules
+        are plain lookups of this process (same bits as the two lookups and their sum)."""
+        word = self.word_embedding
+        pos = self.position_embedding if self.use_positional_embedding else None
+        if _plain_lookup(word) and (pos is None or (_plain_lookup(pos) and pos.weight.dtype == word.weight.dtype)):
+            if pos is None:
+                return embedding(input_ids, word.weight)
+            return embedding(input_ids, word.weight, position_ids=None if default_positions else position_ids,
+                             position_weight=pos.weight)
+        hidden = word(input_ids)
+        return hidden if pos is None else hidden + pos(position_ids)
+
     def forward(self, inputs):
         if self.add_cross_attention:
             input_ids, attention_mask, token_type_ids, position_ids, cross_states, cross_mask, labels = inputs
@@ -953,7 +982,8 @@ class DistributedTransformerLMHead(DistributedModule):
         if self.use_positional_embedding and position_ids is None and s > self.num_positions:
             # host-side shape check: position ids past the table are an out-of-bounds gather
             raise SMPInvalidArgumentError(f"sequence length {s} exceeds num_positions {self.num_positions}")
-        if position_ids is None:
+        default_positions = position_ids is None
+        if default_positions:
             position_ids = torch.arange(0, s, dtype=torch.long, device=device).unsqueeze(0).expand(B, -1)
         elif position_ids.shape[0] != B:
             position_ids = position_ids.expand(B, -1)
@@ -968,9 +998,7 @@ class DistributedTransformerLMHead(DistributedModule):
         if prescaled and not self.distribute_embedding:
             input_ids, position_ids, token_type_ids = shard_sequence(input_ids, position_ids, token_type_ids,
                                                                      bwd_allgather=False)
-        hidden = self.word_embedding(input_ids)
-        if self.use_positional_embedding:
-            hidden = hidden + self.position_embedding(position_ids)
+        hidden = self._embed(input_ids, position_ids, default_positions and not prescaled)
         if token_type_ids is not None:
             if self.num_token_types <= 0:
                 raise SMPInvalidArgumentError("token_type_ids provided but num_token_types == 0")

@@ -96,3 +96,11 @@ def embedding(ids, weight, padding_idx=None, scale=1.0, vocab_start=None, positi
                                getattr(weight, "_smp_fused_grad", False),
                                getattr(position_weight, "_smp_fused_grad", False))
     return _embedding_torch(ids, weight, padding_idx, scale, vocab_start, position_ids, position_weight)
+
+
+def lookup(ids, weight, padding_idx=None, vocab_start=None):
+    """``embedding`` without scale and positions, for modules: tables of other types (fp64) and
+    empty shards go through plain torch operations."""
+    if weight.dtype in _FLOATS and 0 not in weight.shape:
+        return embedding(ids, weight, padding_idx, vocab_start=vocab_start)
+    return _embedding_torch(ids, weight, padding_idx, 1.0, vocab_start, None, None)

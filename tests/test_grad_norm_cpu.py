@@ -92,3 +92,9 @@ def test_refusals(args, kwargs):
     with pytest.raises(SMPInvalidArgumentError):
         clip_grad_norm_(*args, **kwargs)
     assert not _BIG.any()
+
+
+def test_clip_master_grads_by_largest_value_over_stages():
+    from tests.dist_utils import run_workers
+
+    assert all("OK clip" in o for o in run_workers("clip_inf", 2, timeout=120))

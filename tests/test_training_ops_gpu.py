@@ -1,0 +1,137 @@
+"""The embedding, block-norm and gradient-norm operators together, as a training step uses them."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+class Net(torch.nn.Module):
+    """Embedding -> blocks (linear + gelu) joined by FusedBlockNorm -> tied head."""
+
+    def __init__(self, vocab, d, layers, rms):
+        from smdistributed_modelparallel_amd import nn as smp_nn
+
+        super().__init__()
+        self.tok = torch.nn.Parameter(torch.randn(vocab, d) * 0.3)
+        self.pos = torch.nn.Parameter(torch.randn(40, d) * 0.1)
+        self.first = torch.nn.Parameter(torch.ones(d))
+        self.blocks = torch.nn.ModuleList(torch.nn.Linear(d, d) for _ in range(layers))
+        self.norms = torch.nn.ModuleList(
+            smp_nn.FusedBlockNorm(d, rms=rms, gate=0.5, residual_scale=0.7) for _ in range(layers))
+
+    def forward(self, ids):
+        from smdistributed_modelparallel_amd.ops.embedding import embedding
+        from smdistributed_modelparallel_amd.ops.layernorm import rms_norm
+
+        s = embedding(ids, self.tok, padding_idx=0, scale=2.0, position_weight=self.pos)
+        y = rms_norm(s, self.first)
+        for block, norm in zip(self.blocks, self.norms):
+            y, s = norm(torch.nn.functional.gelu(block(y)), s)
+        return y @ self.tok.t()
+
+
+def reference(net, ids, rms, target):
+    """The same in 64 bits by elementary operations; (loss, gradients by name)."""
+    p = {n: t.detach().double().requires_grad_() for n, t in net.named_parameters()}
+
+    def norm(v, w, b):
+        c = v if rms else v - v.mean(-1, keepdim=True)
+        out = c * (c.pow(2).mean(-1, keepdim=True) + 1e-5).rsqrt() * w
+        return out if b is None else out + b
+
+    keep = (ids != 0).unsqueeze(-1)
+    tok = torch.where(keep, p["tok"][ids], p["tok"].detach()[ids])  # padding takes no gradient here
+    s = 2.0 * tok + p["pos"][: ids.shape[1]]
+    y = s * (s.pow(2).mean(-1, keepdim=True) + 1e-5).rsqrt() * p["first"]
+    for i in range(len(net.blocks)):
+        x = torch.nn.functional.gelu(y @ p[f"blocks.{i}.weight"].t() + p[f"blocks.{i}.bias"])
+        k = f"norms.{i}."
+        s = s + 0.7 * p[k + "gate"] * norm(x, p[k + "post_weight"], p.get(k + "post_bias"))
+        y = norm(s, p[k + "weight"], p.get(k + "bias"))
+    loss = torch.nn.functional.cross_entropy((y @ p["tok"].t()).flatten(0, 1), target.flatten())
+    return loss, dict(zip(p, torch.autograd.grad(loss, list(p.values()))))
+
+
+@pytest.mark.parametrize("rms", [False, True])
+def test_step(rms):
+    from smdistributed_modelparallel_amd.optimizers import FusedAdam, clip_grad_norm_
+
+    torch.manual_seed(0)
+    net = Net(300, 136, 3, rms).cuda()
+    ids = torch.randint(0, 300, (6, 33), device="cuda")
+    ids[2, 20:] = 0
+    target = torch.randint(0, 300, (6, 33), device="cuda")
+    opt = FusedAdam(net.parameters(), lr=1e-3)
+    for _ in range(2):
+        want_loss, want = reference(net, ids, rms, target)
+        opt.zero_grad()
+        loss = torch.nn.functional.cross_entropy(net(ids).flatten(0, 1), target.flatten())
+        loss.backward()
+        # fp32 forward and backward of a few layers: some hundred roundings of 2^-24, and the sums' own
+        assert abs(float(loss) - float(want_loss)) < 1e-4
+        for n, q in net.named_parameters():
+            assert float((q.grad.double() - want[n]).norm()) <= 1e-4 * float(want[n].norm()), n
+        total = torch.stack([g.norm() for g in want.values()]).norm()
+        assert abs(float(clip_grad_norm_(net.parameters(), 0.5 * float(total))) - float(total)) <= 1e-4 * float(total)
+        clipped = torch.stack([q.grad.double().norm() for q in net.parameters()]).norm()
+        assert abs(float(clipped) / float(total) - 0.5) <= 1e-4
+        opt.step()
+
+
+def test_same_bits_on_every_run():
+    from smdistributed_modelparallel_amd.ops.multi_tensor import grad_norm
+
+    runs = []
+    for _ in range(2):
+        torch.manual_seed(1)
+        net = Net(500, 200, 2, False).cuda().bfloat16()
+        ids = torch.randint(0, 500, (16, 40), device="cuda")
+        net(ids).float().pow(2).mean().backward()
+        grads = [q.grad for n, q in net.named_parameters() if not n.startswith("blocks")]
+        runs.append([grad_norm(grads)] + grads)
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+@pytest.mark.parametrize("positions", [True, False])
+def test_lm_head_model_uses_the_fused_lookup(positions, monkeypatch):
+    """The GPT model's embeddings through the operator: logits of the same bits as by the modules,
+    gradients within the rounding of one sum order."""
+    from smdistributed_modelparallel_amd.models import build_gpt
+    from smdistributed_modelparallel_amd.nn import transformer
+    from smdistributed_modelparallel_amd.ops._ext import track_calls
+
+    ids = torch.randint(0, 512, (4, 50), device="cuda")
+    out = []
+    for fused in (True, False):
+        monkeypatch.setattr(transformer, "_FUSE_EMBEDDING", [fused])
+        torch.manual_seed(3)
+        m = build_gpt("gpt2-tiny", dropout=0.0, use_positional_embedding=positions, num_layers=2).cuda().bfloat16()
+        with track_calls() as calls:
+            loss, logits = m((ids, None, None, None, ids))
+        assert ("embedding" in calls) == fused
+        loss.backward()
+        out.append((logits.detach(), {n: p.grad for n, p in m.named_parameters()}))
+    assert torch.equal(out[0][0], out[1][0])
+    for n, g in out[0][1].items():
+        h = out[1][1][n].float()
+        assert float((g.float() - h).norm()) <= 2.0 ** -8 * float(h.norm()), n
+    hooked = []
+    monkeypatch.setattr(transformer, "_FUSE_EMBEDDING", [True])
+    m.word_embedding.register_forward_hook(lambda *a: hooked.append(1))
+    with track_calls() as calls:
+        m((ids, None, None, None, ids))
+    assert hooked and "embedding" not in calls
+
+
+def test_distributed_embedding_module():
+    from smdistributed_modelparallel_amd.nn import DistributedEmbedding
+    from smdistributed_modelparallel_amd.ops._ext import track_calls
+
+    m = DistributedEmbedding(40, 24, padding_idx=3).cuda()
+    ids = torch.randint(0, 40, (5, 7), device="cuda")
+    with track_calls() as calls:
+        y = m(ids)
+    assert calls == {"embedding": 1} and torch.equal(y, m.weight[ids])
+    y.sum().backward()
+    assert torch.equal(m.weight.grad[:, 0], torch.bincount(ids.flatten(), minlength=40).float() * (torch.arange(40, device="cuda") != 3))
+    assert m.double()(ids).dtype == torch.float64
