@@ -431,26 +431,23 @@ void register_ipc_p2p(py::module& m) {
       .def("stats", &IpcP2P::stats);
 }
 
-// Page-locks the storage of an ordinary CPU tensor in place (hipHostRegister): exact-size
-// pinned host memory for large optimizer-state arrays -- the caching pinned allocator rounds
-// every block up to a power of two, which at hundreds of GB costs tens of GB of host RAM.
-void host_register(const at::Tensor& t) {
-  TORCH_CHECK(t.device().is_cpu() && t.is_contiguous(), "host_register: a contiguous CPU tensor is required");
-  const size_t bytes = static_cast<size_t>(t.numel()) * t.element_size();
-  if (bytes == 0) return;
-  hip_check(hipHostRegister(t.data_ptr(), bytes, hipHostRegisterDefault), "hipHostRegister");
-}
-
-void host_unregister_ptr(uint64_t ptr) {
-  if (ptr != 0) (void)hipHostUnregister(reinterpret_cast<void*>(static_cast<uintptr_t>(ptr)));
+// fp32 host tensor of exactly n elements in page-locked memory of its own (hipHostMalloc), freed with
+// its storage: the caching pinned allocator rounds every block up to a power of two, which at
+// hundreds of GB of optimizer state costs tens of GB of host RAM.
+at::Tensor host_alloc(int64_t n) {
+  TORCH_CHECK(n >= 0, "host_alloc: negative size");
+  const auto options = at::TensorOptions().dtype(at::kFloat);
+  if (n == 0) return at::empty({0}, options);
+  void* p = nullptr;
+  hip_check(hipHostMalloc(&p, static_cast<size_t>(n) * sizeof(float), hipHostMallocDefault), "hipHostMalloc");
+  return at::from_blob(p, {n}, [](void* q) { (void)hipHostFree(q); }, options);
 }
 
 void register_grad_tracker(py::module& m);
 void register_ipc_allreduce(py::module& m);
 
 void register_bindings(py::module& m) {
-  m.def("host_register", &host_register);
-  m.def("host_unregister_ptr", &host_unregister_ptr);
+  m.def("host_alloc", &host_alloc);
   register_grad_tracker(m);
   register_ipc_p2p(m);
   register_ipc_allreduce(m);

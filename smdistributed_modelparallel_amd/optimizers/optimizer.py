@@ -67,17 +67,12 @@ class _Staged:
 
 
 def _pinned_full(n, fill):
-    """fp32 host array of exactly n elements, page-locked in place (hipHostRegister) so the
-    offload streams copy at PCIe rate without the pinned allocator's power-of-two rounding."""
-    import weakref
-
+    """fp32 host array of exactly n elements in page-locked memory (hipHostMalloc), so the offload
+    streams copy at PCIe rate without the pinned allocator's power-of-two rounding.  (Page-locking
+    memory that exists already, hipHostRegister, is refused on some hosts.)"""
     from ..ops._ext import ext
 
-    t = torch.full((n,), float(fill), dtype=torch.float32)
-    if n:
-        ext().host_register(t)
-        weakref.finalize(t, ext().host_unregister_ptr, t.data_ptr())
-    return t
+    return ext().host_alloc(n).fill_(float(fill))
 
 
 class DistributedOptimizer(torch.optim.Optimizer):

@@ -170,8 +170,9 @@ class PipelineTransport:
             self._ipc = ext().IpcP2P(device.index if device.index is not None else torch.cuda.current_device())
             self._gate_fn = ext().IpcP2P.gate_fn()
             if os.environ.get("SMP_P2P_COMM_STREAM", "1") != "0":
-                lo, hi = torch.cuda.Stream.priority_range()
-                self._comm = torch.cuda.Stream(device=device, priority=min(lo, hi))
+                # default priority like every other stream: work on streams of different priorities
+                # can wait for each other for good
+                self._comm = torch.cuda.Stream(device=device)
         self.bytes_sent = 0
         self.bytes_recv = 0
         self.release_wait_timeouts = 0
