@@ -207,7 +207,7 @@ at::Tensor embedding(at::Tensor weight, Opt pos_weight, at::Tensor ids, Opt pos,
   auto rows_dense = [](const at::Tensor& t) { return t.stride(1) == 1 ? t : t.contiguous(); };
   auto shape = ids.sizes().vec();
   shape.push_back(weight.size(1));
-  const int64_t period = pos_weight.has_value() && !pos.has_value() ? ids.size(-1) : 1;
+  const int64_t period = pos_weight.has_value() && !pos.has_value() ? std::max<int64_t>(ids.size(-1), 1) : 1;
   const at::Tensor flat = ids.reshape({-1}).contiguous();
   if (pos.has_value()) pos = pos->reshape({-1}).contiguous();
   weight = rows_dense(weight);

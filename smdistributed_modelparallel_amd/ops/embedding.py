@@ -6,14 +6,15 @@ gradient rows of each token's occurrences in token order and in fp32 -- the same
 run -- and writes the parameters' flat-buffer gradients in place where they are bound
 (`parallel/flat.py`): only the rows that occur are touched then, and no dense gradient exists
 (autograd gets none for them; their post-accumulate hooks still fire).
-CPU tensors (and torch.autocast regions) use plain torch operations.
+CPU tensors use plain torch operations.  torch.autocast changes nothing: both tables and the
+result are of one type.
 """
 import math
 
 import torch
 
 from ..backend.exceptions import SMPInvalidArgumentError
-from ._ext import ext, fused_ok
+from ._ext import ext
 
 
 def _embedding_torch(ids, weight, padding_idx, scale, vocab_start, position_ids, position_weight):
@@ -36,6 +37,7 @@ def _embedding_torch(ids, weight, padding_idx, scale, vocab_start, position_ids,
     return (y.float() * scale + p.float()).to(weight.dtype)
 
 
+MAX_TOKENS = 1 << 27
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
@@ -59,6 +61,8 @@ def embedding(ids, weight, padding_idx=None, scale=1.0, vocab_start=None, positi
     if not torch.is_tensor(weight) or weight.dim() != 2 or weight.dtype not in _FLOATS or 0 in weight.shape:
         raise SMPInvalidArgumentError("weight must be a [rows, dim] fp32 / fp16 / bf16 tensor")
     _check_ids("ids", ids, weight.device)
+    if ids.numel() > MAX_TOKENS:
+        raise SMPInvalidArgumentError(f"{ids.numel()} tokens in one call: at most {MAX_TOKENS} are supported")
     rows = weight.shape[0]
     scale = float(scale)
     if not math.isfinite(scale):
@@ -89,7 +93,7 @@ def embedding(ids, weight, padding_idx=None, scale=1.0, vocab_start=None, positi
         elif ids.dim() == 0 or ids.shape[-1] > position_weight.shape[0]:
             raise SMPInvalidArgumentError(f"ids {tuple(ids.shape)} need position_ids: the position table has "
                                           f"{position_weight.shape[0]} rows")
-    if fused_ok(weight):
+    if weight.is_cuda:
         start = vocab_start or 0
         return ext().embedding(weight, position_weight, ids, position_ids, scale, start, vocab_start is not None,
                                -1 if padding_idx is None else padding_idx - start,

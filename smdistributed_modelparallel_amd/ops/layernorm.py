@@ -238,7 +238,11 @@ def block_norm(x, residual, weight, bias=None, post_weight=None, post_bias=None,
     root-mean-square norm.  ``x`` and ``residual`` [..., dim] are alike; the weights and biases
     [dim] have their dtype or are fp32.  ``gate`` (that dtype or fp32) broadcasts to ``x``: one
     vector, one for each sample ([batch, 1, dim]), or one value for each element; None is 1.
-    All arithmetic is fp32, and the second norm is taken of ``s`` before it is rounded."""
+    All arithmetic is fp32, and the second norm is taken of ``s`` before it is rounded.  Under
+    torch.autocast, where a block's output and the residual differ in type, the residual's holds."""
+    if torch.is_tensor(x) and torch.is_tensor(residual) and torch.is_autocast_enabled(x.device.type):
+        x = x.to(residual.dtype)
+        gate = gate.to(residual.dtype) if torch.is_tensor(gate) else gate
     _check_rows(x, "x")
     if not torch.is_tensor(residual) or residual.shape != x.shape or residual.dtype != x.dtype \
             or residual.device != x.device:
@@ -257,7 +261,7 @@ def block_norm(x, residual, weight, bias=None, post_weight=None, post_bias=None,
         lead = x.dim() - gate.dim()
         if lead < 0 or any(n not in (1, m) for n, m in zip(gate.shape, x.shape[lead:])):
             raise SMPInvalidArgumentError(f"gate {tuple(gate.shape)} does not broadcast to {tuple(x.shape)}")
-    if not fused_ok(x):
+    if not x.is_cuda:
         h = x.float() if post_weight is None else _norm_torch(x.float(), post_weight, post_bias, eps, rms)
         s = residual.float() + residual_scale * (h if gate is None else gate.float() * h)
         return _norm_torch(s, weight, bias, eps, rms).to(x.dtype), s.to(x.dtype)
@@ -276,6 +280,6 @@ def rms_norm(x, weight, eps=1e-5):
     eps = float(eps)
     if not (math.isfinite(eps) and eps >= 0.0):
         raise SMPInvalidArgumentError(f"bad eps {eps}")
-    if not fused_ok(x):
+    if not x.is_cuda:
         return _norm_torch(x.float(), weight, None, eps, True).to(x.dtype)
     return _block_norm_hip(None, x, weight, None, None, None, None, 1, 1.0, eps, True)[0]

@@ -238,3 +238,44 @@ def test_same_bits_and_graph_replays():
         torch.cuda.synchronize()
         for a, e in zip(out, step()):
             assert torch.equal(a, e)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements: the last rows are right, and the weight gradients see all rows."""
+    from smdistributed_modelparallel_amd.ops.layernorm import block_norm
+
+    rows, d = 270_000, 8192
+    x = torch.zeros(rows, d, device="cuda", dtype=torch.bfloat16)
+    r = torch.zeros_like(x)
+    t = inputs((1, 2, d), torch.bfloat16, torch.float32, False, True, "channel")
+    x[-2:], r[-2:] = t["x"][0], t["residual"][0]
+    names = ("weight", "bias", "post_weight", "post_bias", "gate")
+    leaf = {k: t[k].clone().requires_grad_() for k in names}
+    x.requires_grad_()
+    y, s = block_norm(x, r, leaf["weight"], leaf["bias"], leaf["post_weight"], leaf["post_bias"], leaf["gate"], 0.5)
+    dy = torch.zeros_like(y)
+    dy[-2:] = torch.randn(2, d, device="cuda").bfloat16()
+    grads = torch.autograd.grad(y, [x] + [leaf[k] for k in names], dy)
+    want, slack = ref.exact(t, 0.5, 1e-5, False, dy[-2:].unsqueeze(0)), ref.slack(t, 0.5, 1e-5, False, dy[-2:].unsqueeze(0))
+    within("y", y.detach()[-2:], want["y"][0], slack["y"][0])
+    within("s", s.detach()[-2:], want["s"][0], slack["s"][0])
+    within("dx", grads[0][-2:], want["dx"][0], slack["dx"][0])
+    for k, g in zip(names, grads[1:]):  # rows without gradient add zeros
+        within("d" + k, g, want["d" + k], slack["d" + k])
+
+
+@pytest.mark.parametrize("device", ["cpu", "cuda"])
+def test_autocast_takes_the_residuals_type(device):
+    from smdistributed_modelparallel_amd.nn import FusedBlockNorm
+
+    torch.manual_seed(0)
+    lin, norm = torch.nn.Linear(48, 48).to(device), FusedBlockNorm(48, gate=0.5).to(device)
+    r = torch.randn(5, 48, device=device)
+    with torch.autocast(device, dtype=torch.bfloat16):
+        x = lin(r)
+        y, s = norm(x, r)
+    assert x.dtype == torch.bfloat16 and y.dtype == s.dtype == torch.float32
+    y2, s2 = norm(x.float(), r)
+    assert torch.equal(y, y2) and torch.equal(s, s2)
+    y.sum().backward()
+    assert lin.weight.grad.isfinite().all()

@@ -297,3 +297,45 @@ def test_graph_replays():
         torch.cuda.synchronize()
         for a, e in zip(out, step()):
             assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize("positions", [False, True])
+def test_no_tokens(positions):
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    w, p = (torch.randn(n, 20, device="cuda", requires_grad=True) for n in (7, 5))
+    for shape in ((0,), (3, 0), (0, 4)):
+        y = embedding(torch.empty(shape, dtype=torch.long, device="cuda"), w, position_weight=p if positions else None)
+        assert y.shape == shape + (20,)
+        leaves = [w, p] if positions else [w]
+        for g, t in zip(torch.autograd.grad(y, leaves, torch.empty_like(y)), leaves):
+            assert torch.equal(g, torch.zeros_like(t))
+
+
+def test_two_streams_at_once():
+    """Calls of two streams share nothing: each gives what it gives alone."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    def work(k):
+        g = torch.Generator(device="cuda").manual_seed(k)
+        w = torch.randn(4000, 512, generator=g, device="cuda").requires_grad_()
+        ids = torch.randint(0, 4000 >> k, (9000,), generator=g, device="cuda")
+        dy = torch.randn(9000, 512, generator=g, device="cuda")
+        return w, ids, dy
+
+    def step(w, ids, dy):
+        y = embedding(ids, w)
+        return [y.detach()] + list(torch.autograd.grad(y, w, dy))
+
+    data = [work(k) for k in range(2)]
+    alone = [step(*d) for d in data]
+    streams = [torch.cuda.Stream() for _ in data]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        both = []
+        for s, d in zip(streams, data):
+            with torch.cuda.stream(s):
+                both.append(step(*d))
+        torch.cuda.synchronize()
+        for a, b in zip(alone, both):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
