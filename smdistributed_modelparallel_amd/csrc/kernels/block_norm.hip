@@ -43,14 +43,25 @@ __device__ __forceinline__ void read_opt(const void* p, bool f32, int64_t at, in
   }
 }
 
-// Sums over a team of `waves` waves; `slot` alternates so that one barrier suffices.
+// Sums over a team: SUB lanes of a wave (8, 16 or 32; 0: whole waves).
+template <int SUB>
 struct Team {
   float* smem;  // [2][2][16]
-  int first, waves, slot;
+  int first, waves, slot;  // `slot` alternates so that one barrier suffices
+
+  __device__ __forceinline__ static float in_wave(float v) {
+    if constexpr (SUB == 0) {
+      return wave_sum_fixed(v);
+    } else {
+#pragma unroll
+      for (int o = 1; o < SUB; o <<= 1) v += __shfl_xor(v, o, 64);
+      return v;
+    }
+  }
   __device__ __forceinline__ void sum2(float& a, float& b) {
-    a = wave_sum_fixed(a);
-    b = wave_sum_fixed(b);
-    if (waves == 1) return;
+    a = in_wave(a);
+    b = in_wave(b);
+    if (SUB != 0 || waves == 1) return;
     float* s = smem + slot * 32;
     slot ^= 1;
     if ((threadIdx.x & 63) == 0) {
@@ -65,8 +76,8 @@ struct Team {
     }
   }
   __device__ __forceinline__ void sum1(float& a) {
-    a = wave_sum_fixed(a);
-    if (waves == 1) return;
+    a = in_wave(a);
+    if (SUB != 0 || waves == 1) return;
     float* s = smem + slot * 32;
     slot ^= 1;
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = a;
@@ -77,9 +88,9 @@ struct Team {
 };
 
 // Mean, then the mean square of the differences: values of any offset keep their deviation.
-template <int V, bool FULL>
+template <int V, bool FULL, int SUB>
 __device__ __forceinline__ void moments(const float (&v)[V][kCols], const int (&left)[V], int d, float eps, bool rms,
-                                        Team& team, float& mean, float& rstd) {
+                                        Team<SUB>& team, float& mean, float& rstd) {
   mean = 0.f;
   if (!rms) {
     float a = 0.f;
@@ -104,16 +115,17 @@ __device__ __forceinline__ void moments(const float (&v)[V][kCols], const int (&
   rstd = rsqrtf(q / d + eps);
 }
 
-// team_size threads for a row: 64 (and blockDim.x / 64 rows a block), or all of the block
-template <typename T, int V, bool FULL>
-__global__ void __launch_bounds__(1024) block_norm_fwd(BlockNormArgs a, int team_size) {
+// threads_of_row threads for a row: SUB, 64 (and blockDim.x / that rows a block), or all of the block
+template <typename T, int V, bool FULL, int SUB>
+__global__ void __launch_bounds__(1024) block_norm_fwd(BlockNormArgs a, int threads_of_row) {
   __shared__ float smem[64];
-  const int tid = threadIdx.x, lane = team_size == 64 ? tid & 63 : tid;
-  Team team{smem, 0, team_size / 64, 0};
-  const int64_t row = team_size == 64
-                          ? static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 6) + __builtin_amdgcn_readfirstlane(tid >> 6)
-                          : blockIdx.x;
-  if (row >= a.rows) return;  // (whole waves of their own rows: no barrier follows for them)
+  const int team_size = SUB != 0 ? SUB : threads_of_row;
+  const int tid = threadIdx.x, lane = team_size <= 64 ? tid & (team_size - 1) : tid;
+  Team<SUB> team{smem, 0, team_size / 64, 0};
+  int64_t row = blockIdx.x;
+  if (SUB != 0) row = row * (blockDim.x / team_size) + tid / team_size;
+  if (SUB == 0 && team_size == 64) row = row * (blockDim.x >> 6) + __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (row >= a.rows) return;  // (all lanes of their own rows: no barrier or sum follows for them)
   int left[V];
   float s[V][kCols], h[V][kCols];
   Raw8<T> rs[V], rh[V];
@@ -134,7 +146,7 @@ __global__ void __launch_bounds__(1024) block_norm_fwd(BlockNormArgs a, int team
     }
   float mean2 = 0.f, rstd2 = 1.f, mean1, rstd1;
   if (a.x != nullptr) {
-    if (a.pw != nullptr) moments<V, FULL>(h, left, a.d, a.eps, a.rms, team, mean2, rstd2);
+    if (a.pw != nullptr) moments<V, FULL, SUB>(h, left, a.d, a.eps, a.rms, team, mean2, rstd2);
     const int64_t gate_row = a.gate != nullptr ? row / a.gate_rows * a.d : 0;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
@@ -152,7 +164,7 @@ __global__ void __launch_bounds__(1024) block_norm_fwd(BlockNormArgs a, int team
       write8<FULL, true>(static_cast<T*>(a.s) + row * a.d + c, left[k], s[k]);
     }
   }
-  moments<V, FULL>(s, left, a.d, a.eps, a.rms, team, mean1, rstd1);
+  moments<V, FULL, SUB>(s, left, a.d, a.eps, a.rms, team, mean1, rstd1);
   if (lane == 0 && a.stats != nullptr)
     reinterpret_cast<float4*>(a.stats)[row] = make_float4(mean1, rstd1, mean2, rstd2);
 #pragma unroll
@@ -171,165 +183,168 @@ __global__ void __launch_bounds__(1024) block_norm_fwd(BlockNormArgs a, int team
 // A unit (one team) takes consecutive rows of one gate row.  split > 1: `split` units share the rows
 // of a gate row; split == 1: a unit takes whole gate rows, `units` apart.
 struct Walk {
-  int64_t row, gate;
-  int64_t at, count;  // at-th of the unit's `count` rows of this gate row
+  int row, gate;
+  int at, count;  // at-th of the unit's `count` rows of this gate row
   bool live;
-  __device__ __forceinline__ Walk(const BlockNormArgs& a, int64_t unit) {
-    const int64_t chunk = (a.gate_rows + a.split - 1) / a.split, first = unit % a.split * chunk;
-    gate = unit / a.split;
+  __device__ __forceinline__ Walk(const BlockNormArgs& a, int unit) {
+    const int rows = static_cast<int>(a.gate_rows), split = static_cast<int>(a.split);
+    const int chunk = (rows + split - 1) / split, first = unit % split * chunk;
+    gate = unit / split;
     at = 0;
-    count = a.gate_rows - first < chunk ? a.gate_rows - first : chunk;
+    count = rows - first < chunk ? rows - first : chunk;
     live = gate < a.groups && count > 0;
-    row = gate * a.gate_rows + first;
+    row = live ? gate * rows + first : 0;
   }
   // the gate row ends with this row, and all of it was this unit's
   __device__ __forceinline__ bool last(const BlockNormArgs& a) const { return a.split == 1 && at == count - 1; }
-  __device__ __forceinline__ void next(const BlockNormArgs& a, int64_t units) {
+  __device__ __forceinline__ void next(const BlockNormArgs& a, int units) {
     ++row;
     if (++at < count) return;
     at = 0;
-    gate += units;
-    row = gate * a.gate_rows;
-    live = live && a.split == 1 && gate < a.groups;
+    live = live && a.split == 1 && a.groups - gate > units;
+    gate = live ? gate + units : 0;
+    row = gate * static_cast<int>(a.gate_rows);
   }
 };
 
 enum { kW1, kB1, kW2, kB2, kG, kSums };
 
-// A row's loads, issued while the row before is worked on.
-template <typename T, int V>
-struct RowData {
-  Raw8<T> x[V], res[V], dy[V], ds[V];
-  float4 st;
-};
-
-template <typename T, int V, bool FULL>
-__device__ __forceinline__ void fetch(const BlockNormArgs& a, const Walk& t, int team_size, int lane, RowData<T, V>& r) {
-  if (!t.live) return;
-  r.st = reinterpret_cast<const float4*>(a.stats)[t.row];
+// A whole gate row's gradient, alpha * sum.
+template <typename T, bool FULL>
+__device__ __forceinline__ void write_gate(const BlockNormArgs& a, int64_t gate, int c, int left, float (&sum)[kCols]) {
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const int c = (k * team_size + lane) * kCols, left = a.d - c;
-    if (left <= 0) continue;
-    const int64_t at = t.row * a.d + c;
-    read8<FULL>(static_cast<const T*>(a.res) + at, left, r.res[k]);
-    if (a.x != nullptr) read8<FULL>(static_cast<const T*>(a.x) + at, left, r.x[k]);
-    if (a.dy != nullptr) read8<FULL>(static_cast<const T*>(a.dy) + at, left, r.dy[k]);
-    if (a.ds != nullptr) read8<FULL>(static_cast<const T*>(a.ds) + at, left, r.ds[k]);
+  for (int j = 0; j < kCols; ++j) sum[j] *= a.alpha;
+  if (a.gate_f32) {
+    write8<FULL, true>(static_cast<float*>(a.dgate) + gate * a.d + c, left, sum);
+  } else {
+    write8<FULL, true>(static_cast<T*>(a.dgate) + gate * a.d + c, left, sum);
   }
 }
 
-// The weights stay in registers, in their own type W (T or fp32): a unit works on many rows.
-template <typename T, typename W, int V, bool FULL, int THREADS>
-__global__ void __launch_bounds__(THREADS) block_norm_bwd(BlockNormArgs a, int team_size, int64_t iterations) {
-  extern __shared__ float lds[];  // [64] reductions, then [team_size * kCols * V] to join the teams' sums
-  const int tid = threadIdx.x, teams = blockDim.x / team_size;
-  const int tm = __builtin_amdgcn_readfirstlane(tid / team_size), lane = tid - tm * team_size;  // (whole waves)
-  Team team{lds, tm * (team_size / 64), team_size / 64, 0};
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * teams + tm, units = static_cast<int64_t>(gridDim.x) * teams;
-  float sum[kSums][V][kCols];
-  Raw8<W> w[V], pw[V], pb[V];
-  float ag[V][kCols];  // alpha * gate
-  int left[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const int c = (k * team_size + lane) * kCols;
-    left[k] = a.d - c;
-#pragma unroll
-    for (int j = 0; j < kCols; ++j) {
-      w[k].v[j] = pw[k].v[j] = from_f32<W>(1.f);
-      pb[k].v[j] = from_f32<W>(0.f);
-      ag[k][j] = a.alpha;
-    }
-    if (left[k] > 0) {
-      read8<FULL>(static_cast<const W*>(a.w) + c, left[k], w[k]);
-      if (a.pw != nullptr) read8<FULL>(static_cast<const W*>(a.pw) + c, left[k], pw[k]);
-      if (a.pb != nullptr) read8<FULL>(static_cast<const W*>(a.pb) + c, left[k], pb[k]);
-    }
-#pragma unroll
-    for (int q = 0; q < kSums; ++q)
-#pragma unroll
-      for (int j = 0; j < kCols; ++j) sum[q][k][j] = 0.f;
-  }
-  int64_t gate_now = -1;
-  RowData<T, V> r;
-  Walk t(a, unit);
-  fetch<T, V, FULL>(a, t, team_size, lane, r);
+// A row's loads, issued while the row before is worked on.
+template <typename T>
+struct RowData {
+  Raw8<T> x, res, dy, ds;
+  float4 st;
+};
 
-  for (int64_t i = 0; i < iterations; ++i) {
-    if (a.gate != nullptr && t.live && t.gate != gate_now) {
+template <typename T, bool FULL>
+__device__ __forceinline__ void load_row(const BlockNormArgs& a, int64_t row, int c, int left, RowData<T>& r) {
+  if (left <= 0) return;
+  const int64_t at = row * a.d + c;
+  read8<FULL>(static_cast<const T*>(a.res) + at, left, r.res);
+  if (a.x != nullptr) read8<FULL>(static_cast<const T*>(a.x) + at, left, r.x);
+  if (a.dy != nullptr) read8<FULL>(static_cast<const T*>(a.dy) + at, left, r.dy);
+  if (a.ds != nullptr) read8<FULL>(static_cast<const T*>(a.ds) + at, left, r.ds);
+}
+
+template <typename T, bool FULL>
+__device__ __forceinline__ void fetch(const BlockNormArgs& a, const Walk& t, int c, int left, RowData<T>& r) {
+  if (!t.live || left <= 0) return;
+  r.st = reinterpret_cast<const float4*>(a.stats)[t.row];
+  load_row<T, FULL>(a, t.row, c, left, r);
+}
+
+// Rows of up to 6144 elements, one vector a thread, with the column sums in registers.  The weights
+// stay there too, in their own type W (T or fp32): a unit works on many rows.  These registers
+// allow 12 waves a CU.
+template <typename T, typename W, bool FULL, int SUB>
+__global__ void __launch_bounds__(768) block_norm_bwd(BlockNormArgs a, int threads_of_row, int iterations) {
+  extern __shared__ float lds[];  // [64] reductions, then [team_size * kCols] to join the teams' sums
+  const int team_size = SUB != 0 ? SUB : threads_of_row;
+  const int tid = threadIdx.x, teams = blockDim.x / team_size;
+  const int tm = SUB != 0 ? tid / team_size : __builtin_amdgcn_readfirstlane(tid / team_size);
+  const int lane = tid - tm * team_size, c = lane * kCols, left = a.d - c;
+  Team<SUB> team{lds, tm * (team_size / 64), team_size / 64, 0};
+  const int unit = blockIdx.x * teams + tm, units = gridDim.x * teams;
+  float sum[kSums][kCols];
+  Raw8<W> w, pw, pb;
+  float ag[kCols];  // alpha * gate
+#pragma unroll
+  for (int j = 0; j < kCols; ++j) {
+    w.v[j] = pw.v[j] = from_f32<W>(1.f);
+    pb.v[j] = from_f32<W>(0.f);
+    ag[j] = a.alpha;
+#pragma unroll
+    for (int q = 0; q < kSums; ++q) sum[q][j] = 0.f;
+  }
+  if (left > 0) {
+    read8<FULL>(static_cast<const W*>(a.w) + c, left, w);
+    if (a.pw != nullptr) read8<FULL>(static_cast<const W*>(a.pw) + c, left, pw);
+    if (a.pb != nullptr) read8<FULL>(static_cast<const W*>(a.pb) + c, left, pb);
+  }
+  int gate_now = -1;
+  RowData<T> r;
+  Walk t(a, unit);
+  fetch<T, FULL>(a, t, c, left, r);
+
+  for (int i = 0; i < iterations; ++i) {
+    if (a.gate != nullptr && t.live && t.gate != gate_now && left > 0) {
       gate_now = t.gate;
+      read_opt<FULL, T>(a.gate, a.gate_f32, static_cast<int64_t>(t.gate) * a.d + c, left, 1.f, ag);
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const int c = (k * team_size + lane) * kCols;
-        if (left[k] <= 0) continue;
-        read_opt<FULL, T>(a.gate, a.gate_f32, t.gate * a.d + c, left[k], 1.f, ag[k]);
-#pragma unroll
-        for (int j = 0; j < kCols; ++j) ag[k][j] *= a.alpha;
-      }
+      for (int j = 0; j < kCols; ++j) ag[j] *= a.alpha;
     }
-    float n1[V][kCols], n2[V][kCols], dy[V][kCols], ds[V][kCols];
+    float n1[kCols], n2[kCols], dy[kCols], ds[kCols];
     const float4 st = r.st;
+    const bool live = t.live && left > 0;
     float p = 0.f, q = 0.f;
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      if (left[k] <= 0 || !t.live) continue;
+    if (live) {
 #pragma unroll
       for (int j = 0; j < kCols; ++j) {
-        n1[k][j] = at8(r.res[k], j);
-        n2[k][j] = 0.f;
-        ds[k][j] = a.ds != nullptr ? at8(r.ds[k], j) : 0.f;
+        n1[j] = at8(r.res, j);
+        n2[j] = 0.f;
+        ds[j] = a.ds != nullptr ? at8(r.ds, j) : 0.f;
       }
       if (a.x != nullptr) {
 #pragma unroll
         for (int j = 0; j < kCols; ++j) {
-          n2[k][j] = in_row<FULL>(j, left[k]) ? (at8(r.x[k], j) - st.z) * st.w : 0.f;
-          n1[k][j] = fmaf(ag[k][j], fmaf(n2[k][j], at8(pw[k], j), at8(pb[k], j)), n1[k][j]);
+          n2[j] = in_row<FULL>(j, left) ? (at8(r.x, j) - st.z) * st.w : 0.f;
+          n1[j] = fmaf(ag[j], fmaf(n2[j], at8(pw, j), at8(pb, j)), n1[j]);
         }
       }
       if (a.dy != nullptr) {
 #pragma unroll
         for (int j = 0; j < kCols; ++j) {
-          const float g = at8(r.dy[k], j);
-          n1[k][j] = in_row<FULL>(j, left[k]) ? (n1[k][j] - st.x) * st.y : 0.f;
-          sum[kW1][k][j] = fmaf(g, n1[k][j], sum[kW1][k][j]);
-          sum[kB1][k][j] += g;
-          dy[k][j] = g * at8(w[k], j);
-          p += dy[k][j];
-          q = fmaf(dy[k][j], n1[k][j], q);
+          const float g = at8(r.dy, j);
+          n1[j] = in_row<FULL>(j, left) ? (n1[j] - st.x) * st.y : 0.f;
+          sum[kW1][j] = fmaf(g, n1[j], sum[kW1][j]);
+          sum[kB1][j] += g;
+          dy[j] = g * at8(w, j);
+          p += dy[j];
+          q = fmaf(dy[j], n1[j], q);
         }
       }
     }
-    const Walk now = t;
-    const bool last = now.last(a);
+    const int64_t at = static_cast<int64_t>(t.row) * a.d + c;
+    const int gate = t.gate;
+    const bool last = t.last(a);
     t.next(a, units);
-    if (i + 1 < iterations) fetch<T, V, FULL>(a, t, team_size, lane, r);
+    if (i + 1 < iterations) fetch<T, FULL>(a, t, c, left, r);
     if (a.dy != nullptr) {
       team.sum2(p, q);
       p = a.rms ? 0.f : p / a.d;
       q /= a.d;
     }
     float u = 0.f, v = 0.f;
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      if (left[k] <= 0 || !now.live) continue;
-      const int64_t at = now.row * a.d + (k * team_size + lane) * kCols;
+    if (live) {
       if (a.dy != nullptr) {
 #pragma unroll
-        for (int j = 0; j < kCols; ++j) ds[k][j] = fmaf(st.y, dy[k][j] - p - n1[k][j] * q, ds[k][j]);
+        for (int j = 0; j < kCols; ++j) ds[j] = fmaf(st.y, dy[j] - p - n1[j] * q, ds[j]);
       }
-      if (a.dres != nullptr) write8<FULL, true>(static_cast<T*>(a.dres) + at, left[k], ds[k]);
-      if (a.x == nullptr) continue;
+      if (a.dres != nullptr) write8<FULL, true>(static_cast<T*>(a.dres) + at, left, ds);
+      if (a.x != nullptr) {
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) {
-        const float s = in_row<FULL>(j, left[k]) ? ds[k][j] : 0.f;
-        sum[kG][k][j] = fmaf(s, fmaf(n2[k][j], at8(pw[k], j), at8(pb[k], j)), sum[kG][k][j]);
-        const float dh = s * ag[k][j];
-        sum[kW2][k][j] = fmaf(dh, n2[k][j], sum[kW2][k][j]);
-        sum[kB2][k][j] += dh;
-        ds[k][j] = dh * at8(pw[k], j);  // the gradient of n2; of x itself without a norm
-        u += ds[k][j];
-        v = fmaf(ds[k][j], n2[k][j], v);
+        for (int j = 0; j < kCols; ++j) {
+          const float s = in_row<FULL>(j, left) ? ds[j] : 0.f;
+          sum[kG][j] = fmaf(s, fmaf(n2[j], at8(pw, j), at8(pb, j)), sum[kG][j]);
+          const float dh = s * ag[j];
+          sum[kW2][j] = fmaf(dh, n2[j], sum[kW2][j]);
+          sum[kB2][j] += dh;
+          ds[j] = dh * at8(pw, j);  // the gradient of n2; of x itself without a norm
+          u += ds[j];
+          v = fmaf(ds[j], n2[j], v);
+        }
       }
     }
     if (a.pw != nullptr) {
@@ -339,37 +354,25 @@ __global__ void __launch_bounds__(THREADS) block_norm_bwd(BlockNormArgs a, int t
     } else {
       u = v = 0.f;
     }
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const int c = (k * team_size + lane) * kCols;
-      if (left[k] <= 0 || !now.live || a.x == nullptr) continue;
+    if (live && a.x != nullptr) {
       if (a.dx != nullptr) {
 #pragma unroll
-        for (int j = 0; j < kCols; ++j) ds[k][j] = st.w * (ds[k][j] - u - n2[k][j] * v);
-        write8<FULL, true>(static_cast<T*>(a.dx) + now.row * a.d + c, left[k], ds[k]);
+        for (int j = 0; j < kCols; ++j) ds[j] = st.w * (ds[j] - u - n2[j] * v);
+        write8<FULL, true>(static_cast<T*>(a.dx) + at, left, ds);
       }
-      if (a.gate_direct && last) {  // a whole gate row's sum is complete
+      if (a.gate_direct && last) {
+        write_gate<T, FULL>(a, gate, c, left, sum[kG]);
 #pragma unroll
-        for (int j = 0; j < kCols; ++j) sum[kG][k][j] *= a.alpha;
-        if (a.gate_f32) {
-          write8<FULL, true>(static_cast<float*>(a.dgate) + now.gate * a.d + c, left[k], sum[kG][k]);
-        } else {
-          write8<FULL, true>(static_cast<T*>(a.dgate) + now.gate * a.d + c, left[k], sum[kG][k]);
-        }
-#pragma unroll
-        for (int j = 0; j < kCols; ++j) sum[kG][k][j] = 0.f;
+        for (int j = 0; j < kCols; ++j) sum[kG][j] = 0.f;
       }
     }
   }
 
   // partial sums: of the teams together for the vectors, of each unit for its gate row
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const int c = (k * team_size + lane) * kCols;
-#pragma unroll
-    for (int j = 0; j < kCols; ++j) sum[kG][k][j] *= a.alpha;
-    if (a.gate_part != nullptr && c < a.d) write8<FULL, false>(a.gate_part + unit * a.d + c, a.d - c, sum[kG][k]);
-  }
+  for (int j = 0; j < kCols; ++j) sum[kG][j] *= a.alpha;
+  if (a.gate_part != nullptr && left > 0)
+    write8<FULL, false>(a.gate_part + static_cast<int64_t>(unit) * a.d + c, left, sum[kG]);
 #pragma unroll
   for (int q = 0; q < kSums; ++q) {
     if (a.part[q] == nullptr) continue;
@@ -378,25 +381,183 @@ __global__ void __launch_bounds__(THREADS) block_norm_bwd(BlockNormArgs a, int t
       __syncthreads();
       if (tm == m) {
 #pragma unroll
-        for (int k = 0; k < V; ++k)
-#pragma unroll
-          for (int j = 0; j < kCols; ++j) buf[(k * kCols + j) * team_size + lane] = sum[q][k][j];
+        for (int j = 0; j < kCols; ++j) buf[j * team_size + lane] = sum[q][j];
       }
       __syncthreads();
       if (tm == 0) {
 #pragma unroll
-        for (int k = 0; k < V; ++k)
-#pragma unroll
-          for (int j = 0; j < kCols; ++j) sum[q][k][j] += buf[(k * kCols + j) * team_size + lane];
+        for (int j = 0; j < kCols; ++j) sum[q][j] += buf[j * team_size + lane];
       }
     }
+    if (tm == 0 && left > 0) write8<FULL, false>(a.part[q] + static_cast<int64_t>(blockIdx.x) * a.d + c, left, sum[q]);
+  }
+}
+
+// Wider rows, whose elements leave no registers for the column sums: one row a block.  What the
+// column sums need of a row's reductions goes to a.pq.
+template <typename T, int V, bool FULL>
+__global__ void __launch_bounds__(1024) block_norm_bwd_rows(BlockNormArgs a) {
+  __shared__ float smem[64];
+  const int team_size = blockDim.x, lane = threadIdx.x;
+  Team<0> team{smem, 0, team_size / 64, 0};
+  const int64_t row = blockIdx.x, gate_row = a.gate != nullptr ? row / a.gate_rows * a.d : 0;
+  const float4 st = reinterpret_cast<const float4*>(a.stats)[row];
+  RowData<T> r[V];  // all loads first
+  float n1[V][kCols], n2[V][kCols], dy[V][kCols], ds[V][kCols];
+  int left[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const int c = (k * team_size + lane) * kCols;
-      if (tm == 0 && c < a.d)
-        write8<FULL, false>(a.part[q] + static_cast<int64_t>(blockIdx.x) * a.d + c, a.d - c, sum[q][k]);
+  for (int k = 0; k < V; ++k) {
+    const int c = (k * team_size + lane) * kCols;
+    left[k] = a.d - c;
+    load_row<T, FULL>(a, row, c, left[k], r[k]);
+  }
+  float p = 0.f, q = 0.f;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const int c = (k * team_size + lane) * kCols;
+    if (left[k] <= 0) continue;
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) {
+      n1[k][j] = at8(r[k].res, j);
+      n2[k][j] = a.x != nullptr ? at8(r[k].x, j) : 0.f;
+      dy[k][j] = a.dy != nullptr ? at8(r[k].dy, j) : 0.f;
+      ds[k][j] = a.ds != nullptr ? at8(r[k].ds, j) : 0.f;
+    }
+    if (a.x != nullptr) {
+      float pw[kCols], pb[kCols], g[kCols];
+      read_opt<FULL, T>(a.pw, a.w_f32, c, left[k], 1.f, pw);
+      read_opt<FULL, T>(a.pb, a.w_f32, c, left[k], 0.f, pb);
+      read_opt<FULL, T>(a.gate, a.gate_f32, gate_row + c, left[k], 1.f, g);
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) {
+        n2[k][j] = in_row<FULL>(j, left[k]) ? (n2[k][j] - st.z) * st.w : 0.f;
+        n1[k][j] = fmaf(a.alpha * g[j], fmaf(n2[k][j], pw[j], pb[j]), n1[k][j]);
+      }
+    }
+    if (a.dy != nullptr) {
+      float w[kCols];
+      read_opt<FULL, T>(a.w, a.w_f32, c, left[k], 1.f, w);
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) {
+        n1[k][j] = in_row<FULL>(j, left[k]) ? (n1[k][j] - st.x) * st.y : 0.f;
+        dy[k][j] *= w[j];
+        p += dy[k][j];
+        q = fmaf(dy[k][j], n1[k][j], q);
+      }
     }
   }
+  if (a.dy != nullptr) {
+    team.sum2(p, q);
+    p = a.rms ? 0.f : p / a.d;
+    q /= a.d;
+  }
+  if (lane == 0) reinterpret_cast<float2*>(a.pq)[row] = make_float2(p, q);
+  float u = 0.f, v = 0.f;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const int c = (k * team_size + lane) * kCols;
+    if (left[k] <= 0) continue;
+    if (a.dy != nullptr) {
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) ds[k][j] = fmaf(st.y, dy[k][j] - p - n1[k][j] * q, ds[k][j]);
+    }
+    if (a.dres != nullptr) write8<FULL, true>(static_cast<T*>(a.dres) + row * a.d + c, left[k], ds[k]);
+    if (a.x == nullptr) continue;
+    float pw[kCols], g[kCols];
+    read_opt<FULL, T>(a.pw, a.w_f32, c, left[k], 1.f, pw);
+    read_opt<FULL, T>(a.gate, a.gate_f32, gate_row + c, left[k], 1.f, g);
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) {
+      ds[k][j] = in_row<FULL>(j, left[k]) ? a.alpha * g[j] * ds[k][j] * pw[j] : 0.f;
+      u += ds[k][j];
+      v = fmaf(ds[k][j], n2[k][j], v);
+    }
+  }
+  if (a.dx == nullptr) return;
+  if (a.pw != nullptr) {
+    team.sum2(u, v);
+    u = a.rms ? 0.f : u / a.d;
+    v /= a.d;
+  } else {
+    u = v = 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const int c = (k * team_size + lane) * kCols;
+    if (left[k] <= 0) continue;
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) ds[k][j] = st.w * (ds[k][j] - u - n2[k][j] * v);
+    write8<FULL, true>(static_cast<T*>(a.dx) + row * a.d + c, left[k], ds[k]);
+  }
+}
+
+// The column sums of wide rows: a thread takes 8 columns of a unit's rows and forms n1, n2 and dS
+// again from the rows and their reductions.  blockIdx.y: the unit.
+template <typename T, bool FULL>
+__global__ void __launch_bounds__(256) block_norm_bwd_columns(BlockNormArgs a, int iterations) {
+  const int c = (blockIdx.x * 256 + threadIdx.x) * kCols, left = a.d - c;
+  if (left <= 0) return;
+  const int unit = blockIdx.y, units = gridDim.y;
+  float w[kCols], pw[kCols], pb[kCols], ag[kCols], sum[kSums][kCols];
+  read_opt<FULL, T>(a.w, a.w_f32, c, left, 1.f, w);
+  read_opt<FULL, T>(a.pw, a.w_f32, c, left, 1.f, pw);
+  read_opt<FULL, T>(a.pb, a.w_f32, c, left, 0.f, pb);
+#pragma unroll
+  for (int j = 0; j < kCols; ++j) {
+    ag[j] = a.alpha;
+#pragma unroll
+    for (int q = 0; q < kSums; ++q) sum[q][j] = 0.f;
+  }
+  int gate_now = -1;
+  Walk t(a, unit);
+  RowData<T> r;
+  float2 pq = make_float2(0.f, 0.f);
+  auto load = [&] {
+    fetch<T, FULL>(a, t, c, left, r);
+    if (t.live) pq = reinterpret_cast<const float2*>(a.pq)[t.row];
+  };
+  load();
+  for (int i = 0; i < iterations && t.live; ++i) {
+    if (a.gate != nullptr && t.gate != gate_now) {
+      gate_now = t.gate;
+      read_opt<FULL, T>(a.gate, a.gate_f32, static_cast<int64_t>(t.gate) * a.d + c, left, 1.f, ag);
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) ag[j] *= a.alpha;
+    }
+    const RowData<T> now = r;
+    const float4 st = now.st;
+    const float p = pq.x, q = pq.y;
+    const bool last = t.last(a);
+    const int gate = t.gate;
+    t.next(a, units);
+    if (i + 1 < iterations) load();
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) {
+      const float n2 = a.x != nullptr ? (at8(now.x, j) - st.z) * st.w : 0.f;
+      const float h = fmaf(n2, pw[j], pb[j]);
+      const float s = a.x != nullptr ? fmaf(ag[j], h, at8(now.res, j)) : at8(now.res, j);
+      const float n1 = (s - st.x) * st.y, dy = a.dy != nullptr ? at8(now.dy, j) : 0.f;
+      float d = a.ds != nullptr ? at8(now.ds, j) : 0.f;
+      if (a.dy != nullptr) d = fmaf(st.y, dy * w[j] - p - n1 * q, d);
+      const float dh = d * ag[j];
+      sum[kW1][j] = fmaf(dy, n1, sum[kW1][j]);
+      sum[kB1][j] += dy;
+      sum[kG][j] = fmaf(d, h, sum[kG][j]);
+      sum[kW2][j] = fmaf(dh, n2, sum[kW2][j]);
+      sum[kB2][j] += dh;
+    }
+    if (a.gate_direct && last) {
+      write_gate<T, FULL>(a, gate, c, left, sum[kG]);
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) sum[kG][j] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kCols; ++j) sum[kG][j] *= a.alpha;
+  if (a.gate_part != nullptr) write8<FULL, false>(a.gate_part + static_cast<int64_t>(unit) * a.d + c, left, sum[kG]);
+#pragma unroll
+  for (int q = 0; q < kSums; ++q)
+    if (a.part[q] != nullptr) write8<FULL, false>(a.part[q] + static_cast<int64_t>(unit) * a.d + c, left, sum[q]);
 }
 
 // out[g][c] = (or +=) the sum over `split` partial rows; 32 columns x 32 row groups a block
@@ -435,14 +596,12 @@ __global__ void __launch_bounds__(1024) block_norm_join(BlockNormJoin l, int d) 
   }
 }
 
-// Teams of the backward: one vector a thread up to 4096 elements, two beyond.
-int team_of(int64_t d, int& v) {
-  const int64_t vectors = (d + kCols - 1) / kCols;
-  v = vectors <= 512 ? 1 : 2;
-  return static_cast<int>(((vectors + v - 1) / v + 63) / 64 * 64);
-}
-
 constexpr int64_t kMaxWidth = 16384;
+// Widest row whose column sums stay in registers: one vector a thread in the 12 waves of a CU.
+constexpr int64_t kMaxSummed = 6144;
+
+// Threads of a row of up to 32 vectors: lanes of one wave, which takes several rows then.
+int sub_of(int64_t vectors) { return vectors <= 8 ? 8 : vectors <= 16 ? 16 : vectors <= 32 ? 32 : 0; }
 
 }  // namespace
 
@@ -451,27 +610,34 @@ int block_norm_fwd(int dt, const BlockNormArgs& a, hipStream_t s) {
   if (a.rows <= 0) return 0;
   const int64_t vectors = (a.d + kCols - 1) / kCols;
   const bool wave = vectors <= 256;
+  const int sub = sub_of(vectors);
   const int v = vectors <= 64 ? 1 : vectors <= 128 ? 2 : wave ? 4 : vectors <= 1024 ? 1 : 2;
-  const int team = wave ? 64 : static_cast<int>(((vectors + v - 1) / v + 63) / 64 * 64);
-  const int64_t blocks = wave ? (a.rows + 3) / 4 : a.rows;
+  const int team = sub ? sub : wave ? 64 : static_cast<int>(((vectors + v - 1) / v + 63) / 64 * 64);
+  const int64_t rows_of_block = wave ? 256 / team : 1, blocks = (a.rows + rows_of_block - 1) / rows_of_block;
   if (blocks > 0x7fffffff) return -3;
   SMPK_DISPATCH(dt, T, {
     const bool full = a.d % kCols == 0;
-    const auto kernel = v == 1   ? (full ? block_norm_fwd<T, 1, true> : block_norm_fwd<T, 1, false>)
-                        : v == 2 ? (full ? block_norm_fwd<T, 2, true> : block_norm_fwd<T, 2, false>)
-                                 : (full ? block_norm_fwd<T, 4, true> : block_norm_fwd<T, 4, false>);
+    const auto kernel = sub == 8    ? (full ? block_norm_fwd<T, 1, true, 8> : block_norm_fwd<T, 1, false, 8>)
+                        : sub == 16 ? (full ? block_norm_fwd<T, 1, true, 16> : block_norm_fwd<T, 1, false, 16>)
+                        : sub == 32 ? (full ? block_norm_fwd<T, 1, true, 32> : block_norm_fwd<T, 1, false, 32>)
+                        : v == 1    ? (full ? block_norm_fwd<T, 1, true, 0> : block_norm_fwd<T, 1, false, 0>)
+                        : v == 2    ? (full ? block_norm_fwd<T, 2, true, 0> : block_norm_fwd<T, 2, false, 0>)
+                                    : (full ? block_norm_fwd<T, 4, true, 0> : block_norm_fwd<T, 4, false, 0>);
     kernel<<<static_cast<unsigned>(blocks), wave ? 256 : team, 0, s>>>(a, team);
   });
   return static_cast<int>(hipGetLastError());
 }
 
 int block_norm_bwd_plan(int64_t rows, int64_t d, int64_t gate_rows, BlockNormPlan& p) {
-  if (d < 1 || d > kMaxWidth || rows < 1) return -4;
-  int v;
-  p.team = team_of(d, v);
-  const int teams = p.team >= 256 ? 1 : 256 / p.team;  // LDS joins their sums: fewer partial rows than units
+  if (d < 1 || d > kMaxWidth || rows < 1 || rows > 0x7fffffff) return -4;
+  const int64_t vectors = (d + kCols - 1) / kCols;
+  p.two_pass = d > kMaxSummed;
+  p.team = p.two_pass ? 256 : sub_of(vectors) ? sub_of(vectors) : static_cast<int>((vectors + 63) / 64 * 64);
+  // teams of a block: as many waves as a CU holds, in three blocks of 4 waves or, for wider teams, in
+  // one; LDS joins their sums, so that partial rows are fewer than units
+  const int teams = p.two_pass ? 1 : p.team <= 256 ? 256 / p.team : 768 / p.team;
   p.threads = p.team * teams;
-  int64_t units = (p.team > 256 ? 512 : 768) * teams;
+  int64_t units = (p.two_pass ? 1024 / ((vectors + 255) / 256) : p.team <= 256 ? 768 : 256) * teams;
   if (units > rows) units = rows;
   const int64_t groups = rows / gate_rows;
   p.split = units / groups;
@@ -481,31 +647,50 @@ int block_norm_bwd_plan(int64_t rows, int64_t d, int64_t gate_rows, BlockNormPla
   p.blocks = (used + teams - 1) / teams;
   p.units = p.blocks * teams;
   p.iterations = p.split > 1 ? (gate_rows + p.split - 1) / p.split : (groups + p.units - 1) / p.units * gate_rows;
-  p.lds = static_cast<int>((64 + (teams > 1 ? p.team * kCols * v : 0)) * sizeof(float));
+  p.lds = static_cast<int>((64 + (teams > 1 ? p.team * kCols : 0)) * sizeof(float));
   return 0;
 }
 
 namespace {
-template <typename T, typename W>
+template <typename T, typename W, bool FULL>
 void launch_bwd(const BlockNormArgs& a, const BlockNormPlan& p, hipStream_t s) {
-  const bool full = a.d % kCols == 0;
-  int v;
-  team_of(a.d, v);
-  const auto kernel = v == 1 ? (full ? block_norm_bwd<T, W, 1, true, 512> : block_norm_bwd<T, W, 1, false, 512>)
-                      : p.threads <= 512
-                          ? (full ? block_norm_bwd<T, W, 2, true, 512> : block_norm_bwd<T, W, 2, false, 512>)
-                          : (full ? block_norm_bwd<T, W, 2, true, 1024> : block_norm_bwd<T, W, 2, false, 1024>);
-  kernel<<<static_cast<unsigned>(p.blocks), p.threads, p.lds, s>>>(a, p.team, p.iterations);
+  const int iterations = static_cast<int>(p.iterations);
+  if (p.two_pass) {
+    const int64_t vectors = (a.d + kCols - 1) / kCols;
+    const int v = vectors <= 1024 ? 1 : 2;
+    const auto kernel = v == 1 ? block_norm_bwd_rows<T, 1, FULL> : block_norm_bwd_rows<T, 2, FULL>;
+    kernel<<<static_cast<unsigned>(a.rows), static_cast<unsigned>(((vectors + v - 1) / v + 63) / 64 * 64), 0, s>>>(a);
+    bool sums = a.gate_direct || a.gate_part != nullptr;
+    for (float* q : a.part) sums = sums || q != nullptr;
+    if (!sums) return;
+    const unsigned columns = static_cast<unsigned>((vectors + 255) / 256);
+    block_norm_bwd_columns<T, FULL><<<dim3(columns, static_cast<unsigned>(p.units)), 256, 0, s>>>(a, iterations);
+    return;
+  }
+  const auto kernel = p.team == 8    ? block_norm_bwd<T, W, FULL, 8>
+                      : p.team == 16 ? block_norm_bwd<T, W, FULL, 16>
+                      : p.team == 32 ? block_norm_bwd<T, W, FULL, 32>
+                                     : block_norm_bwd<T, W, FULL, 0>;
+  kernel<<<static_cast<unsigned>(p.blocks), p.threads, p.lds, s>>>(a, p.team, iterations);
+}
+template <typename T, typename W>
+void launch_bwd_of(const BlockNormArgs& a, const BlockNormPlan& p, hipStream_t s) {
+  if (a.d % kCols == 0) {
+    launch_bwd<T, W, true>(a, p, s);
+  } else {
+    launch_bwd<T, W, false>(a, p, s);
+  }
 }
 }  // namespace
 
 int block_norm_bwd(int dt, const BlockNormArgs& a, const BlockNormPlan& p, hipStream_t s) {
   if (a.rows <= 0) return 0;
+  if (p.two_pass && a.pq == nullptr) return -5;
   SMPK_DISPATCH(dt, T, {
     if (a.w_f32) {
-      launch_bwd<T, float>(a, p, s);
+      launch_bwd_of<T, float>(a, p, s);
     } else {
-      launch_bwd<T, T>(a, p, s);
+      launch_bwd_of<T, T>(a, p, s);
     }
   });
   return static_cast<int>(hipGetLastError());

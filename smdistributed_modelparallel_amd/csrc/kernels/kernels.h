@@ -316,10 +316,11 @@ struct BlockNormArgs {
   int64_t split = 1;
   int gate_direct = 0;          // a unit has whole gate rows: it writes dgate itself
   float* gate_part = nullptr;   // else [units][d]
+  float* pq = nullptr;          // [rows][2], with two_pass
   float* part[5] = {};          // [blocks][d] of dw1, db1, dw2, db2, dgate (one gate row for all)
 };
 struct BlockNormPlan {
-  int team, threads, lds;
+  int team, threads, lds, two_pass;  // two_pass: rows, then their column sums (a.pq between them)
   int64_t blocks, units, split, iterations;
 };
 // out[g] = or += the sum of the partial rows g * split .. (g + 1) * split - 1

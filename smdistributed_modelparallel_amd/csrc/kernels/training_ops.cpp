@@ -336,7 +336,11 @@ std::vector<Opt> block_norm_bwd(Opt dy, Opt ds, Opt x, at::Tensor res, at::Tenso
   const auto f32 = res.options().dtype(at::kFloat);
   const int64_t groups = a.rows / a.gate_rows;
   const bool gate_rows_own = need[6] && groups > 1;  // one sum for each gate row, not one for all rows
-  at::Tensor parts, gate_part;
+  at::Tensor parts, gate_part, pq;
+  if (p.two_pass) {
+    pq = at::empty({a.rows, 2}, f32);
+    a.pq = pq.data_ptr<float>();
+  }
   int sums = 0;
   for (int i = 0; i < 5; ++i) sums += target[i].defined() && !(i == 4 && gate_rows_own);
   if (sums) parts = at::empty({sums, p.blocks, a.d}, f32);

@@ -175,6 +175,7 @@ def add_layer_norm(x, residual, weight, bias, eps=1e-5, dropout_p=0.0, drawn=Non
 
 # ------------------------------------------------- the norms before and after a block, fused
 MAX_BLOCK_NORM_WIDTH = 16384
+MAX_BLOCK_NORM_ROWS = 1 << 30
 
 
 def _block_norm_hip(x, residual, weight, bias, post_weight, post_bias, gate, gate_rows, alpha, eps, rms):
@@ -224,6 +225,8 @@ def _check_rows(t, name):
         raise SMPInvalidArgumentError(f"{name} must be a fp32 / fp16 / bf16 tensor [..., dim]")
     if not 1 <= t.shape[-1] <= MAX_BLOCK_NORM_WIDTH:
         raise SMPInvalidArgumentError(f"{name}: widths of 1 to {MAX_BLOCK_NORM_WIDTH} are supported, got {t.shape[-1]}")
+    if t.numel() // t.shape[-1] > MAX_BLOCK_NORM_ROWS:
+        raise SMPInvalidArgumentError(f"{name}: at most {MAX_BLOCK_NORM_ROWS} rows are supported")
 
 
 def block_norm(x, residual, weight, bias=None, post_weight=None, post_bias=None, gate=None, residual_scale=1.0,

@@ -115,6 +115,7 @@ _X, _W = torch.zeros(2, 3, 8), torch.ones(8)
     ((_X, _X, _W), {"eps": -1e-5}),
     ((torch.zeros(1, 16385), torch.zeros(1, 16385), torch.ones(16385)), {}),
     ((torch.zeros(3, 0), torch.zeros(3, 0), torch.ones(0)), {}),
+    ((torch.zeros(1).half().expand((1 << 30) + 1, 1), torch.zeros(1).half().expand((1 << 30) + 1, 1), torch.ones(1)), {}),
 ])
 def test_refusals(args, kwargs):
     with pytest.raises(SMPInvalidArgumentError):

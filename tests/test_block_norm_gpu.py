@@ -58,7 +58,8 @@ def check(shape, dtype, wdtype=None, rms=False, post=True, gate="none", alpha=0.
 
 
 SHAPES = [(1, 1, 1), (1, 1, 64), (2, 3, 7), (3, 5, 8), (1, 700, 40), (5, 41, 512), (2, 129, 1600), (7, 33, 1601),
-          (3, 50, 2056), (2, 20, 4096), (2, 9, 6144), (1, 7, 8192), (1, 5, 8193), (2, 3, 12288), (1, 3, 16384)]
+          (3, 50, 2056), (2, 20, 4096), (2, 9, 6144), (3, 5, 6145), (1, 7, 8192), (1, 5, 8193), (2, 3, 12288), (1, 3, 16384),
+          (9, 100, 65), (4, 11, 128), (3, 70, 129), (3, 50, 250), (2, 40, 257), (2, 17, 5000)]
 
 
 @pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
@@ -84,7 +85,9 @@ def test_one_output_used(use, post):
 
 
 @pytest.mark.parametrize("shape,gate", [((3000, 3, 24), "sample"), ((30, 300, 24), "full"), ((600, 40, 72), "sample"),
-                                        ((2, 9000, 48), "sample"), ((1, 20000, 96), "channel"), ((9000, 2, 16), "none")])
+                                        ((2, 9000, 48), "sample"), ((1, 20000, 96), "channel"), ((9000, 2, 16), "none"),
+                                        ((5, 300, 6152), "sample"), ((700, 2, 6200), "sample"), ((3, 90, 8192), "full"),
+                                        ((40, 40, 9001), "channel")])
 def test_many_rows(shape, gate):
     """More gate rows than units, fewer, and one for all rows; fp32 gate beside 16-bit rows."""
     check(shape, torch.bfloat16, torch.float32, gate=gate, gdtype=torch.float32)
