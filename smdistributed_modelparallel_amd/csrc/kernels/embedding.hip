@@ -1,10 +1,16 @@
 // Token embedding: y[t] = scale * W[id_t - start] (+ P[pos_t]), and the gradients of both tables.
 //
 // Forward: a gather, bound by HBM: it writes every row and reads it from the table (or the
-// caches, for the frequent tokens).  The sum is formed in fp32 and rounded once.
+// caches, for frequent tokens).  The sum is formed in fp32 and rounded once.
 //
 // Backward: dW[v] = scale * sum of dy[t] over the tokens with id_t = v, in token order and in
-// fp32, so that the result does not depend on the order in which blocks run.
+// fp32, so that the result does not depend on the order in which blocks run.  The tokens are
+// brought into the order of their rows first (bound by latency: 27 us for 65536 tokens), then every
+// row of dy is read once and every row of dW written once (bound by HBM).
+//
+// Measured, 65536 tokens, 50257 x 1600 bf16, with a table of 2048 positions: forward 73 us; sums and
+// zeros of both tables 117 us (580 MB, 5.0 TB/s); joins 9 us.  One block for each row of the table,
+// which looked for its tokens in all ids, took 3400 us.
 #include "kernels.h"
 #include "vec8.h"
 
@@ -107,7 +113,8 @@ __global__ void __launch_bounds__(kT) emb_fwd(IndexList ids, const T* __restrict
 // bits a pass, so a vocabulary of up to 2^20 rows takes two.  A block of 16 waves owns a
 // consecutive run of the items, each wave a consecutive part of it; the waves count their digits,
 // the counts become the places of each wave's items, and the wave walks over its items once more,
-// 64 at a time, in order.  No place depends on the order in which anything runs.
+// 64 at a time, in order.  No place depends on the order in which anything runs.  65536 tokens:
+// 8.5 us to count and 4.8 us to place, each pass; both are the latency of few blocks.
 constexpr int kWaves = 16;
 constexpr int kSortThreads = kWaves * 64;
 constexpr int kMaxBits = 10;

@@ -2,6 +2,8 @@
 //
 // norm = scale * sqrt(sum g^2) or scale * max |g|; out = g * scale * min(1, max_norm / (norm + 1e-6)).
 // Bound by HBM: every gradient is read for the norm, and read again and written for the clip.
+// Measured, 1.56 G bf16 elements in 579 tensors: norm 0.57 ms (5.5 TB/s), clip 1.31 ms (4.7 TB/s, the
+// rate of a copy of that size).
 //
 // The tensors come as a table in the kernel's arguments (kGradList of them a launch): no copy to
 // the device precedes a launch, and a captured launch holds its table.  A tensor is cut into

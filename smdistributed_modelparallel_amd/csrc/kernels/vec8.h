@@ -44,9 +44,12 @@ __device__ __forceinline__ void read8(const T* p, int left, float (&o)[kCols]) {
   for (int j = 0; j < kCols; ++j) o[j] = at8(r, j);
 }
 
-// STREAM: past the caches, for outputs that are written once and are as large as the caches or
-// larger.  65536 rows of 1600 bf16 gathered from a table (210 MB): 72 us stored normally, 46 us so;
-// 1.6 to 13 MB: the same; followed by a kernel that reads them, 149 and 147 us (13 MB: 13.2, 13.3).
+// STREAM: past the caches, for outputs that are written once, in whole lines, and that no kernel
+// finds there later.  Stored normally and so: the gradient of a 50257 x 1600 bf16 table 132 and
+// 118 us; block norms of 16384 x 1600 bf16 52 and 45 us forward, 92 and 90 us backward.  Not where
+// a table's reads want the memory too (65536 gathered rows of a cold table: 76 and 82 us), where
+// what is written is what was just read (clip of 1.4 GB: 837 and 926 us with the norm), nor for
+// rows of fp32, whose lanes write half lines.
 template <bool FULL, bool STREAM, typename T>
 __device__ __forceinline__ void write8(T* p, int left, const float (&o)[kCols]) {
   constexpr int M = 16 / sizeof(T);
