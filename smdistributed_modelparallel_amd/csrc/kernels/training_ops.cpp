@@ -6,6 +6,8 @@
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <algorithm>
 #include <vector>
@@ -138,23 +140,84 @@ void embedding_bwd(at::Tensor dy, at::Tensor ids, c10::optional<at::Tensor> pos,
   check(smpk::embedding_bwd(dt_code(dy, "embedding"), dy.data_ptr(), n, d, t, count, stream()), "embedding_bwd");
 }
 
+// backward() will add the gradient of the leaf `t` to t.grad.  Not so torch.autograd.grad, which returns
+// it, nor a pass that builds a graph, whose sum has to be part of that graph.
+bool accumulates(const at::Tensor& t) {
+  if (at::GradMode::is_enabled()) return false;
+  const auto* info = torch::autograd::get_current_graph_task_exec_info();
+  if (info == nullptr || info->empty()) return true;
+  const auto it = info->find(torch::autograd::impl::try_get_grad_accumulator(t).get());
+  return it != info->end() && it->second.needed_ && !it->second.captures_;
+}
+
 // The gradient of `t` goes straight into its bound slot of the flat buffer: the caller saw the
 // parameter's mark, the slot has to be there still.
 bool bound(const at::Tensor& t, bool marked) {
   if (!marked || !t.defined() || !t.is_leaf()) return false;
   const at::Tensor& g = t.grad();
-  return g.defined() && g.scalar_type() == t.scalar_type() && g.sizes() == t.sizes() && g.is_contiguous();
+  return g.defined() && g.scalar_type() == t.scalar_type() && g.sizes() == t.sizes() && g.is_contiguous() &&
+         accumulates(t);
 }
 
-// Backward passes here launch kernels that autograd does not see: a second derivative is an error.
-variable_list once(variable_list grads, const char* name) {
-  if (!at::GradMode::is_enabled()) return grads;
-  for (auto& g : grads)
-    if (g.defined()) g = g.detach().set_requires_grad(true);  // whatever is built on it reaches the error
-  const auto error = std::make_shared<torch::autograd::DelayedError>(
-      std::string(name) + " cannot be differentiated twice", static_cast<int64_t>(grads.size()));
-  return (*error)(std::move(grads));
+// Autograd takes a leaf's gradient on the stream that was current when the leaf's accumulator was made.
+// If that is the default stream, as where an eager graph of the leaf is alive, no capture can include it:
+// an error here, before autograd tries, which would end the process.
+void check_capture(at::ArrayRef<at::Tensor> inputs, const char* name) {
+  if (stream() == nullptr) return;  // the default stream: never captured
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  TORCH_CHECK(hipStreamIsCapturing(stream(), &status) == hipSuccess, name, ": the stream's capture is invalid");
+  if (status == hipStreamCaptureStatusNone) return;
+  for (const at::Tensor& t : inputs) {
+    if (!t.defined() || !t.is_leaf() || !t.requires_grad()) continue;
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
+    const auto at = accumulator ? accumulator->stream() : std::nullopt;
+    TORCH_CHECK(!at.has_value() || at->id() != 0, name,
+                ": this backward pass is captured while a graph of the same parameters, made on the default stream, is "
+                "alive: drop that graph first (its outputs and losses), or make it on another stream");
+  }
 }
+
+at::Tensor embedding(at::Tensor weight, Opt pos_weight, at::Tensor ids, Opt pos, double scale, int64_t start,
+                     bool foreign_zero, int64_t skip, bool mark_w, bool mark_p);
+
+// The gradients of both tables as functions of dy, for passes that build a graph: linear in dy, so the
+// derivative is a lookup in the tables' second gradients, and that can be differentiated again.
+class EmbeddingGradFunction : public torch::autograd::Function<EmbeddingGradFunction> {
+ public:
+  // {dw, dp}, those of w_shape / p_shape that are not empty
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& dy, const at::Tensor& ids, const Opt& pos,
+                               int64_t period, double scale, int64_t start, int64_t skip,
+                               std::vector<int64_t> w_shape, std::vector<int64_t> p_shape) {
+    ctx->save_for_backward({ids, pos.has_value() ? *pos : at::Tensor()});
+    ctx->saved_data["args"] = std::vector<int64_t>{period, start, skip, !w_shape.empty(), !p_shape.empty()};
+    ctx->saved_data["scale"] = scale;
+    Opt dw, dp;
+    variable_list out;
+    if (!w_shape.empty()) out.push_back(*(dw = at::empty(w_shape, dy.options())));
+    if (!p_shape.empty()) out.push_back(*(dp = at::empty(p_shape, dy.options())));
+    embedding_bwd(dy, ids, pos, period, scale, start, skip, dw, false, dp, false);
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto args = ctx->saved_data["args"].toIntVector();
+    const bool has_w = args[3], has_p = args[4];
+    Opt gp, pos;
+    if (has_p) gp = grads.back();
+    at::Tensor gw = has_w ? grads[0] : at::zeros({1, gp->size(1)}, gp->options());
+    const int64_t d = gw.size(1), skip = args[2];
+    if (has_w && skip >= 0 && skip < gw.size(0))  // the row that takes no gradient passes none on
+      gw = at::cat({gw.narrow(0, 0, skip), at::zeros({1, d}, gw.options()),
+                    gw.narrow(0, skip + 1, gw.size(0) - skip - 1)});
+    const at::Tensor ids = has_p ? saved[0].view({-1, args[0]}) : saved[0];
+    if (has_p && saved[1].defined()) pos = saved[1].view(ids.sizes());
+    variable_list out(9);
+    out[0] = embedding(gw, gp, ids, pos, ctx->saved_data["scale"].toDouble(), args[1], true, has_w ? skip : -1, false,
+                       false).view({-1, d});
+    return out;
+  }
+};
 
 // Autograd's nodes are C++: a short call's time is the host's, and the backward needs no interpreter.
 class EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
@@ -178,9 +241,21 @@ class EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
     const at::Tensor w = ctx->saved_data["weight"].toTensor();
     const bool two = ctx->saved_data.count("pos_weight") != 0;
     const at::Tensor p = two ? ctx->saved_data["pos_weight"].toTensor() : at::Tensor();
+    check_capture({w, p}, "embedding");
     variable_list out(11);
     const at::Tensor dy = grads[0].reshape({-1, w.size(1)}).contiguous();
     Opt dw, dp, pos;
+    if (saved[1].defined()) pos = saved[1];
+    if (at::GradMode::is_enabled() && dy.requires_grad()) {
+      std::vector<int64_t> w_shape, p_shape;
+      if (ctx->needs_input_grad(0)) w_shape = w.sizes().vec();
+      if (two && ctx->needs_input_grad(1)) p_shape = p.sizes().vec();
+      size_t k = 0;
+      const auto g = EmbeddingGradFunction::apply(dy, saved[0], pos, args[0], scale, args[1], args[2], w_shape, p_shape);
+      if (!w_shape.empty()) out[0] = g[k++];
+      if (!p_shape.empty()) out[1] = g[k++];
+      return out;
+    }
     bool add_w = false, add_p = false;
     auto target = [&](const at::Tensor& t, bool marked, Opt& g, bool& add, at::Tensor& result) {
       add = bound(t, marked);
@@ -189,14 +264,13 @@ class EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
     };
     if (ctx->needs_input_grad(0)) target(w, args[3], dw, add_w, out[0]);
     if (two && ctx->needs_input_grad(1)) target(p, args[4], dp, add_p, out[1]);
-    if (saved[1].defined()) pos = saved[1];
     if (add_w && add_p && dw->data_ptr() == dp->data_ptr()) {  // one parameter as both tables: one after the other
       embedding_bwd(dy, saved[0], pos, args[0], scale, args[1], args[2], dw, true, c10::nullopt, false);
       embedding_bwd(dy, saved[0], pos, args[0], scale, args[1], args[2], c10::nullopt, false, dp, true);
     } else {
       embedding_bwd(dy, saved[0], pos, args[0], scale, args[1], args[2], dw, add_w, dp, add_p);
     }
-    return once(std::move(out), "embedding");
+    return out;
   }
 };
 
@@ -377,6 +451,16 @@ std::vector<Opt> block_norm_bwd(Opt dy, Opt ds, Opt x, at::Tensor res, at::Tenso
   return out;
 }
 
+// The backward launches kernels that autograd does not see: a second derivative is an error.
+variable_list once(variable_list grads, const char* name) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (auto& g : grads)
+    if (g.defined()) g = g.detach().set_requires_grad(true);  // whatever is built on it reaches the error
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      std::string(name) + " cannot be differentiated twice", static_cast<int64_t>(grads.size()));
+  return (*error)(std::move(grads));
+}
+
 class BlockNormFunction : public torch::autograd::Function<BlockNormFunction> {
  public:
   static variable_list forward(AutogradContext* ctx, const Opt& x, const at::Tensor& res, const at::Tensor& w,
@@ -403,6 +487,7 @@ class BlockNormFunction : public torch::autograd::Function<BlockNormFunction> {
     const Opt ds = grads.size() > 1 ? opt(grads[1].defined() ? grads[1].contiguous() : grads[1]) : Opt();
     if (!dy.has_value() && !ds.has_value()) return result;
     const auto v = ctx->get_saved_variables();
+    check_capture(v, "block_norm");
     const auto marks = ctx->saved_data["marks"].toIntVector();
     std::vector<bool> need(7, false);
     for (size_t i = 0, edge = 0; i < 7; ++i)  // (autograd counts the tensors that are there)

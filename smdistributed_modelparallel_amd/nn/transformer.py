@@ -258,7 +258,7 @@ _FUSE_EMBEDDING = [os.environ.get("SMP_FUSE_EMBEDDING", "1") != "0"]
 def _plain_lookup(m):
     """The module is nothing but a lookup in a table of this process on the GPU: ops.embedding may
     read its weight without calling it (no hook, option, shard gathering, other stage or checkpoint)."""
-    return (_FUSE_EMBEDDING[0] and type(m) is nn.Embedding and fused_ok(m.weight)
+    return (_FUSE_EMBEDDING[0] and type(m) is nn.Embedding and "forward" not in m.__dict__ and fused_ok(m.weight)
             and m.weight.dtype in (torch.float32, torch.float16, torch.bfloat16) and m.padding_idx is None
             and m.max_norm is None and not m.scale_grad_by_freq and not m.sparse
             and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)

@@ -6,6 +6,7 @@ gradient rows of each token's occurrences in token order and in fp32 -- the same
 run -- and writes the parameters' flat-buffer gradients in place where they are bound
 (`parallel/flat.py`): only the rows that occur are touched then, and no dense gradient exists
 (autograd gets none for them; their post-accumulate hooks still fire).
+A pass that builds a graph of its own (``create_graph``) can be differentiated again.
 CPU tensors use plain torch operations.  torch.autocast changes nothing: both tables and the
 result are of one type.
 """
@@ -38,6 +39,7 @@ def _embedding_torch(ids, weight, padding_idx, scale, vocab_start, position_ids,
 
 
 MAX_TOKENS = 1 << 27
+MAX_ROWS = (1 << 31) - 1
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
@@ -60,6 +62,8 @@ def embedding(ids, weight, padding_idx=None, scale=1.0, vocab_start=None, positi
     (broadcast to ``ids``) or, without them, by the place in the last dimension."""
     if not torch.is_tensor(weight) or weight.dim() != 2 or weight.dtype not in _FLOATS or 0 in weight.shape:
         raise SMPInvalidArgumentError("weight must be a [rows, dim] fp32 / fp16 / bf16 tensor")
+    if max(weight.shape) >= MAX_ROWS:
+        raise SMPInvalidArgumentError(f"tables of fewer than {MAX_ROWS} rows and columns are supported")
     _check_ids("ids", ids, weight.device)
     if ids.numel() > MAX_TOKENS:
         raise SMPInvalidArgumentError(f"{ids.numel()} tokens in one call: at most {MAX_TOKENS} are supported")
@@ -79,7 +83,8 @@ def embedding(ids, weight, padding_idx=None, scale=1.0, vocab_start=None, positi
         if position_ids is not None:
             raise SMPInvalidArgumentError("position_ids need a position_weight")
     else:
-        if position_weight.dim() != 2 or position_weight.shape[1] != weight.shape[1] or 0 in position_weight.shape:
+        if not torch.is_tensor(position_weight) or position_weight.dim() != 2 \
+                or position_weight.shape[1] != weight.shape[1] or not 0 < position_weight.shape[0] < MAX_ROWS:
             raise SMPInvalidArgumentError("position_weight must be [positions, dim] with weight's dim")
         if position_weight.dtype != weight.dtype or position_weight.device != weight.device:
             raise SMPInvalidArgumentError("position_weight must have weight's dtype and device")
@@ -103,8 +108,8 @@ def embedding(ids, weight, padding_idx=None, scale=1.0, vocab_start=None, positi
 
 
 def lookup(ids, weight, padding_idx=None, vocab_start=None):
-    """``embedding`` without scale and positions, for modules: tables of other types (fp64) and
-    empty shards go through plain torch operations."""
-    if weight.dtype in _FLOATS and 0 not in weight.shape:
+    """``embedding`` without scale and positions, for modules: tables of other types (fp64), empty
+    shards, and tables or lists beyond the kernels' sizes go through plain torch operations."""
+    if weight.dtype in _FLOATS and 0 not in weight.shape and ids.numel() <= MAX_TOKENS and weight.shape[0] < MAX_ROWS:
         return embedding(ids, weight, padding_idx, vocab_start=vocab_start)
     return _embedding_torch(ids, weight, padding_idx, 1.0, vocab_start, None, None)

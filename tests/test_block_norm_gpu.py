@@ -282,3 +282,34 @@ def test_autocast_takes_the_residuals_type(device):
     assert torch.equal(y, y2) and torch.equal(s, s2)
     y.sum().backward()
     assert lin.weight.grad.isfinite().all()
+
+
+def test_bound_gradients_stay_out_of_other_passes():
+    from smdistributed_modelparallel_amd.ops.layernorm import block_norm
+
+    x = torch.randn(6, 40, device="cuda").requires_grad_()
+    w = torch.randn(40, device="cuda").requires_grad_()
+    (expect,) = torch.autograd.grad(block_norm(x, x, w)[0].sum(), w)
+    w.grad, w._smp_fused_grad = torch.zeros_like(w), True
+    slot = w.grad
+    (dw,) = torch.autograd.grad(block_norm(x, x, w)[0].sum(), w)
+    assert torch.equal(dw, expect) and slot.eq(0).all()
+    block_norm(x, x, w)[0].sum().backward(inputs=[w])
+    assert w.grad is slot and torch.equal(slot, expect)
+
+
+def test_capture_beside_an_eager_graph_is_refused():
+    """Autograd would take the gradient on the default stream, which a capture cannot include."""
+    from smdistributed_modelparallel_amd.ops.layernorm import block_norm
+
+    x, r = (torch.randn(9, 32, device="cuda") for _ in range(2))
+    w = torch.randn(32, device="cuda").requires_grad_()
+    dy = torch.randn(9, 32, device="cuda")
+    eager, _ = block_norm(x, r, w)
+    (expect,) = torch.autograd.grad(eager, w, dy, retain_graph=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, _ = block_norm(x, r, w)
+        with pytest.raises(RuntimeError, match="alive"):
+            torch.autograd.grad(y, w, dy)
+    assert torch.equal(torch.autograd.grad(eager, w, dy)[0], expect)

@@ -219,14 +219,55 @@ def test_one_parameter_as_both_tables():
     within(w.grad, total, 2 * slack)
 
 
-def test_second_derivatives_are_refused():
+@pytest.mark.parametrize("frozen", [None, "token", "position"])
+@pytest.mark.parametrize("given", [False, True])
+def test_second_derivative(frozen, given):
+    """The gradients are linear in dy: their derivative looks the rows of the second gradients up, but
+    not that of the padding token.  A third pass goes the other way again."""
     from smdistributed_modelparallel_amd.ops.embedding import embedding
 
-    w = torch.randn(6, 16, device="cuda", requires_grad=True)
-    dy = torch.ones(2, 16, device="cuda", requires_grad=True)
-    (dw,) = torch.autograd.grad(embedding(torch.tensor([1, 1], device="cuda"), w), w, dy, create_graph=True)
-    with pytest.raises(RuntimeError, match="twice"):
-        dw.sum().backward()
+    w, p, a, b = (torch.randn(n, 20, device="cuda") for n in (9, 6, 9, 6))
+    ids = torch.tensor([[1, 8, 3, 3], [3, 0, 1, 7]], device="cuda")
+    pos = torch.tensor([[5, 4, 0, 1], [2, 2, 3, 0]], device="cuda") if given else None
+    dy = torch.randn(2, 4, 20, device="cuda", requires_grad=True)
+    leaves = [t.requires_grad_() for t, name in ((w, "token"), (p, "position")) if name != frozen]
+    second = [t.requires_grad_() for t, name in ((a, "token"), (b, "position")) if name != frozen]
+    y = embedding(ids, w, padding_idx=3, scale=0.5, position_ids=pos, position_weight=p)
+    grads = torch.autograd.grad(y, leaves, dy, create_graph=True)
+    assert all(torch.equal(g, e) for g, e in zip(grads, torch.autograd.grad(y, leaves, dy)))
+    (ddy,) = torch.autograd.grad(grads, dy, second, create_graph=True)
+    expect = torch.zeros_like(dy)
+    if frozen != "token":
+        expect = expect + 0.5 * a[ids] * (ids != 3).unsqueeze(-1)
+    if frozen != "position":
+        expect = expect + b[pos if given else torch.arange(4, device="cuda")]
+    assert float((ddy - expect).detach().abs().max()) <= 2.0 ** -23 * float(expect.detach().abs().max())
+    for g, e in zip(torch.autograd.grad(ddy, second, dy.detach()), grads):
+        assert torch.equal(g, e)
+
+
+def test_bound_gradients_stay_out_of_other_passes():
+    """torch.autograd.grad returns the gradient of a bound table, a pass that builds a graph keeps it
+    in that graph, backward(inputs=...) adds it in place."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    w, v = (torch.randn(9, 24, device="cuda").requires_grad_() for _ in range(2))
+    w.grad, w._smp_fused_grad = torch.ones_like(w), True
+    slot = w.grad
+    ids = torch.tensor([4, 4, 1], device="cuda")
+    count = torch.zeros_like(w)
+    count[4], count[1] = 2.0, 1.0
+    (dw,) = torch.autograd.grad(embedding(ids, w).sum(), w)
+    assert torch.equal(dw, count) and slot.eq(1).all()
+    (embedding(ids, w) * embedding(ids, v)).sum().backward(inputs=[v])
+    assert slot.eq(1).all() and v.grad is not None
+    embedding(ids, w).sum().backward(inputs=[w])
+    assert w.grad is slot and torch.equal(slot, 1 + count)
+    dy = torch.ones(3, 24, device="cuda", requires_grad=True)
+    embedding(ids, w).backward(dy, create_graph=True)
+    assert slot.eq(1 + count).all() and torch.equal(w.grad, 1 + 2 * count)
+    (ddy,) = torch.autograd.grad(w.grad.sum(), dy)
+    assert ddy.eq(1).all()
 
 
 def test_table_changed_before_the_backward():
@@ -339,3 +380,28 @@ def test_two_streams_at_once():
         torch.cuda.synchronize()
         for a, b in zip(alone, both):
             assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_capture_beside_an_eager_graph_is_refused():
+    """Autograd would take the gradient on the default stream, which a capture cannot include."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    w = torch.randn(30, 16, device="cuda").requires_grad_()
+    ids = torch.randint(0, 30, (40,), device="cuda")
+    dy = torch.randn(40, 16, device="cuda")
+    eager = embedding(ids, w)
+    (expect,) = torch.autograd.grad(eager, w, dy, retain_graph=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = embedding(ids, w)
+        with pytest.raises(RuntimeError, match="alive"):
+            torch.autograd.grad(y, w, dy)
+    assert torch.equal(torch.autograd.grad(eager, w, dy)[0], expect)
+    del eager, y
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (dw,) = torch.autograd.grad(embedding(ids, w), w, dy)
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dw, expect)

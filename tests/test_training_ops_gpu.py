@@ -123,6 +123,17 @@ def test_lm_head_model_uses_the_fused_lookup(positions, monkeypatch):
     assert hooked and "embedding" not in calls
 
 
+def test_replaced_forward_of_an_embedding_module_is_called():
+    from smdistributed_modelparallel_amd.models import build_gpt
+
+    m = build_gpt("gpt2-tiny", dropout=0.0, num_layers=1).cuda().bfloat16()
+    plain, called = m.word_embedding.forward, []
+    m.word_embedding.forward = lambda ids: called.append(1) or plain(ids)
+    ids = torch.randint(0, 512, (2, 9), device="cuda")
+    m((ids, None, None, None, ids))
+    assert called
+
+
 def test_distributed_embedding_module():
     from smdistributed_modelparallel_amd.nn import DistributedEmbedding
     from smdistributed_modelparallel_amd.ops._ext import track_calls
