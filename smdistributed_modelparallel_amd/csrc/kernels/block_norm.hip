@@ -31,21 +31,36 @@
 namespace smpk {
 namespace {
 
-template <bool FULL>
-__device__ __forceinline__ bool in_row(int j, int left) {
-  return FULL || j < left;
+// How a row splits into vectors: into whole ones; into whole ones of which the last begins before the
+// end of the one before it, whose elements both hold and write -- the same values -- and one counts in
+// the sums over the row; or, in rows of less than one vector, element by element.  40 M bf16 elements in
+// rows of 1601: 69 us forward, 125 us backward; with the last vector element by element 84 and 181 us.
+enum Rows { kWhole, kOverlap, kShort };
+
+// First column of a thread's vector; `left`, at most kCols for the last one, from there to the row's end.
+template <int R>
+__device__ __forceinline__ int column(int vector, int d, int& left) {
+  const int c = vector * kCols;
+  left = d - c;
+  return R == kOverlap && left < kCols ? d - kCols : c;
+}
+
+// Element j counts in sums over the row.
+template <int R>
+__device__ __forceinline__ bool counts(int j, int left) {
+  return R == kWhole || (R == kOverlap ? j + left >= kCols : j < left);
 }
 
 // A vector that may be absent (`other` then) and of either T or fp32.
-template <bool FULL, typename T>
+template <int R, typename T>
 __device__ __forceinline__ void read_opt(const void* p, bool f32, int64_t at, int left, float other, float (&o)[kCols]) {
   if (p == nullptr) {
 #pragma unroll
     for (int j = 0; j < kCols; ++j) o[j] = other;
   } else if (f32) {
-    read8<FULL>(static_cast<const float*>(p) + at, left, o);
+    read8<R != kShort>(static_cast<const float*>(p) + at, left, o);
   } else {
-    read8<FULL>(static_cast<const T*>(p) + at, left, o);
+    read8<R != kShort>(static_cast<const T*>(p) + at, left, o);
   }
 }
 
@@ -94,7 +109,7 @@ struct Team {
 };
 
 // Mean, then the mean square of the differences: values of any offset keep their deviation.
-template <int V, bool FULL, int SUB>
+template <int V, int R, int SUB>
 __device__ __forceinline__ void moments(const float (&v)[V][kCols], const int (&left)[V], int d, float eps, bool rms,
                                         Team<SUB>& team, float& mean, float& rstd) {
   mean = 0.f;
@@ -103,7 +118,7 @@ __device__ __forceinline__ void moments(const float (&v)[V][kCols], const int (&
 #pragma unroll
     for (int k = 0; k < V; ++k)
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) a += v[k][j];  // (zero past the row's end)
+      for (int j = 0; j < kCols; ++j) a += counts<R>(j, left[k]) ? v[k][j] : 0.f;
     team.sum1(a);
     mean = a / d;
   }
@@ -113,7 +128,7 @@ __device__ __forceinline__ void moments(const float (&v)[V][kCols], const int (&
     if (left[k] <= 0) continue;
 #pragma unroll
     for (int j = 0; j < kCols; ++j) {
-      const float c = in_row<FULL>(j, left[k]) ? v[k][j] - mean : 0.f;
+      const float c = counts<R>(j, left[k]) ? v[k][j] - mean : 0.f;
       q = fmaf(c, c, q);
     }
   }
@@ -122,7 +137,7 @@ __device__ __forceinline__ void moments(const float (&v)[V][kCols], const int (&
 }
 
 // threads_of_row threads for a row: SUB, 64 (and blockDim.x / that rows a block), or all of the block
-template <typename T, int V, bool FULL, int SUB>
+template <typename T, int V, int R, int SUB>
 __global__ void __launch_bounds__(1024) block_norm_fwd(BlockNormArgs a, int threads_of_row) {
   __shared__ float smem[64];
   const int team_size = SUB != 0 ? SUB : threads_of_row;
@@ -132,16 +147,15 @@ __global__ void __launch_bounds__(1024) block_norm_fwd(BlockNormArgs a, int thre
   if (SUB != 0) row = row * (blockDim.x / team_size) + tid / team_size;
   if (SUB == 0 && team_size == 64) row = row * (blockDim.x >> 6) + __builtin_amdgcn_readfirstlane(tid >> 6);
   if (row >= a.rows) return;  // (all lanes of their own rows: no barrier or sum follows for them)
-  int left[V];
+  int col[V], left[V];
   float s[V][kCols], h[V][kCols];
   Raw8<T> rs[V], rh[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    const int c = (k * team_size + lane) * kCols;
-    left[k] = a.d - c;
+    const int c = col[k] = column<R>(k * team_size + lane, a.d, left[k]);
     if (left[k] <= 0) continue;
-    if (a.x != nullptr) read8<FULL>(static_cast<const T*>(a.x) + row * a.d + c, left[k], rh[k]);
-    read8<FULL>(static_cast<const T*>(a.res) + row * a.d + c, left[k], rs[k]);
+    if (a.x != nullptr) read8<R != kShort>(static_cast<const T*>(a.x) + row * a.d + c, left[k], rh[k]);
+    read8<R != kShort>(static_cast<const T*>(a.res) + row * a.d + c, left[k], rs[k]);
   }
 #pragma unroll
   for (int k = 0; k < V; ++k)
@@ -152,37 +166,37 @@ __global__ void __launch_bounds__(1024) block_norm_fwd(BlockNormArgs a, int thre
     }
   float mean2 = 0.f, rstd2 = 1.f, mean1, rstd1;
   if (a.x != nullptr) {
-    if (a.pw != nullptr) moments<V, FULL, SUB>(h, left, a.d, a.eps, a.rms, team, mean2, rstd2);
+    if (a.pw != nullptr) moments<V, R, SUB>(h, left, a.d, a.eps, a.rms, team, mean2, rstd2);
     const int64_t gate_row = a.gate != nullptr ? row / a.gate_rows * a.d : 0;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const int c = (k * team_size + lane) * kCols;
+      const int c = col[k];
       if (left[k] <= 0) continue;
       float w[kCols], b[kCols], g[kCols];
-      read_opt<FULL, T>(a.pw, a.w_f32, c, left[k], 1.f, w);
-      read_opt<FULL, T>(a.pb, a.w_f32, c, left[k], 0.f, b);
-      read_opt<FULL, T>(a.gate, a.gate_f32, gate_row + c, left[k], 1.f, g);
+      read_opt<R, T>(a.pw, a.w_f32, c, left[k], 1.f, w);
+      read_opt<R, T>(a.pb, a.w_f32, c, left[k], 0.f, b);
+      read_opt<R, T>(a.gate, a.gate_f32, gate_row + c, left[k], 1.f, g);
 #pragma unroll
       for (int j = 0; j < kCols; ++j) {
         const float v = fmaf((h[k][j] - mean2) * rstd2, w[j], b[j]);
-        s[k][j] = in_row<FULL>(j, left[k]) ? fmaf(a.alpha * g[j], v, s[k][j]) : 0.f;
+        s[k][j] = fmaf(a.alpha * g[j], v, s[k][j]);
       }
-      write8<FULL, true>(static_cast<T*>(a.s) + row * a.d + c, left[k], s[k]);
+      write8<R != kShort, true>(static_cast<T*>(a.s) + row * a.d + c, left[k], s[k]);
     }
   }
-  moments<V, FULL, SUB>(s, left, a.d, a.eps, a.rms, team, mean1, rstd1);
+  moments<V, R, SUB>(s, left, a.d, a.eps, a.rms, team, mean1, rstd1);
   if (lane == 0 && a.stats != nullptr)
     reinterpret_cast<float4*>(a.stats)[row] = make_float4(mean1, rstd1, mean2, rstd2);
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    const int c = (k * team_size + lane) * kCols;
+    const int c = col[k];
     if (left[k] <= 0) continue;
     float w[kCols], b[kCols];
-    read_opt<FULL, T>(a.w, a.w_f32, c, left[k], 1.f, w);
-    read_opt<FULL, T>(a.b, a.w_f32, c, left[k], 0.f, b);
+    read_opt<R, T>(a.w, a.w_f32, c, left[k], 1.f, w);
+    read_opt<R, T>(a.b, a.w_f32, c, left[k], 0.f, b);
 #pragma unroll
     for (int j = 0; j < kCols; ++j) w[j] = fmaf((s[k][j] - mean1) * rstd1, w[j], b[j]);
-    write8<FULL, true>(static_cast<T*>(a.y) + row * a.d + c, left[k], w);
+    write8<R != kShort, true>(static_cast<T*>(a.y) + row * a.d + c, left[k], w);
   }
 }
 
@@ -216,14 +230,14 @@ struct Walk {
 enum { kW1, kB1, kW2, kB2, kG, kSums };
 
 // A whole gate row's gradient, alpha * sum.
-template <typename T, bool FULL>
+template <typename T, int R>
 __device__ __forceinline__ void write_gate(const BlockNormArgs& a, int64_t gate, int c, int left, float (&sum)[kCols]) {
 #pragma unroll
   for (int j = 0; j < kCols; ++j) sum[j] *= a.alpha;
   if (a.gate_f32) {
-    write8<FULL, true>(static_cast<float*>(a.dgate) + gate * a.d + c, left, sum);
+    write8<R != kShort, true>(static_cast<float*>(a.dgate) + gate * a.d + c, left, sum);
   } else {
-    write8<FULL, true>(static_cast<T*>(a.dgate) + gate * a.d + c, left, sum);
+    write8<R != kShort, true>(static_cast<T*>(a.dgate) + gate * a.d + c, left, sum);
   }
 }
 
@@ -234,33 +248,37 @@ struct RowData {
   float4 st;
 };
 
-template <typename T, bool FULL>
+template <typename T, int R>
 __device__ __forceinline__ void load_row(const BlockNormArgs& a, int64_t row, int c, int left, RowData<T>& r) {
   if (left <= 0) return;
   const int64_t at = row * a.d + c;
-  read8<FULL>(static_cast<const T*>(a.res) + at, left, r.res);
-  if (a.x != nullptr) read8<FULL>(static_cast<const T*>(a.x) + at, left, r.x);
-  if (a.dy != nullptr) read8<FULL>(static_cast<const T*>(a.dy) + at, left, r.dy);
-  if (a.ds != nullptr) read8<FULL>(static_cast<const T*>(a.ds) + at, left, r.ds);
+  read8<R != kShort>(static_cast<const T*>(a.res) + at, left, r.res);
+  if (a.x != nullptr) read8<R != kShort>(static_cast<const T*>(a.x) + at, left, r.x);
+  if (a.dy != nullptr) read8<R != kShort>(static_cast<const T*>(a.dy) + at, left, r.dy);
+  if (a.ds != nullptr) read8<R != kShort>(static_cast<const T*>(a.ds) + at, left, r.ds);
 }
 
-template <typename T, bool FULL>
+template <typename T, int R>
 __device__ __forceinline__ void fetch(const BlockNormArgs& a, const Walk& t, int c, int left, RowData<T>& r) {
   if (!t.live || left <= 0) return;
   r.st = reinterpret_cast<const float4*>(a.stats)[t.row];
-  load_row<T, FULL>(a, t.row, c, left, r);
+  load_row<T, R>(a, t.row, c, left, r);
 }
 
 // Rows of up to 6144 elements, one vector a thread, with the column sums in registers.  The weights
 // stay there too, in their own type W (T or fp32): a unit works on many rows.  These registers
 // allow 12 waves a CU.
-template <typename T, typename W, bool FULL, int SUB>
+template <typename T, typename W, int R, int SUB>
 __global__ void __launch_bounds__(768) block_norm_bwd(BlockNormArgs a, int threads_of_row, int iterations) {
+  // past the caches where the stores fill whole lines, or nearly: rows of 1601 bf16 125 us so, 127 us
+  // stored normally, but rows of 101 174 and 152 us, and of 1600 fp32 226 and 211 us
+  constexpr bool kStream = sizeof(T) == 2 && (R == kWhole || SUB == 0);
   extern __shared__ float lds[];  // [64] reductions, then [team_size * kCols] to join the teams' sums
   const int team_size = SUB != 0 ? SUB : threads_of_row;
   const int tid = threadIdx.x, teams = blockDim.x / team_size;
   const int tm = SUB != 0 ? tid / team_size : __builtin_amdgcn_readfirstlane(tid / team_size);
-  const int lane = tid - tm * team_size, c = lane * kCols, left = a.d - c;
+  int left;
+  const int lane = tid - tm * team_size, c = column<R>(lane, a.d, left);
   Team<SUB> team{lds, tm * (team_size / 64), team_size / 64, 0};
   const int unit = blockIdx.x * teams + tm, units = gridDim.x * teams;
   float sum[kSums][kCols];
@@ -275,19 +293,19 @@ __global__ void __launch_bounds__(768) block_norm_bwd(BlockNormArgs a, int threa
     for (int q = 0; q < kSums; ++q) sum[q][j] = 0.f;
   }
   if (left > 0) {
-    read8<FULL>(static_cast<const W*>(a.w) + c, left, w);
-    if (a.pw != nullptr) read8<FULL>(static_cast<const W*>(a.pw) + c, left, pw);
-    if (a.pb != nullptr) read8<FULL>(static_cast<const W*>(a.pb) + c, left, pb);
+    read8<R != kShort>(static_cast<const W*>(a.w) + c, left, w);
+    if (a.pw != nullptr) read8<R != kShort>(static_cast<const W*>(a.pw) + c, left, pw);
+    if (a.pb != nullptr) read8<R != kShort>(static_cast<const W*>(a.pb) + c, left, pb);
   }
   int gate_now = -1;
   RowData<T> r;
   Walk t(a, unit);
-  fetch<T, FULL>(a, t, c, left, r);
+  fetch<T, R>(a, t, c, left, r);
 
   for (int i = 0; i < iterations; ++i) {
     if (a.gate != nullptr && t.live && t.gate != gate_now && left > 0) {
       gate_now = t.gate;
-      read_opt<FULL, T>(a.gate, a.gate_f32, static_cast<int64_t>(t.gate) * a.d + c, left, 1.f, ag);
+      read_opt<R, T>(a.gate, a.gate_f32, static_cast<int64_t>(t.gate) * a.d + c, left, 1.f, ag);
 #pragma unroll
       for (int j = 0; j < kCols; ++j) ag[j] *= a.alpha;
     }
@@ -305,7 +323,7 @@ __global__ void __launch_bounds__(768) block_norm_bwd(BlockNormArgs a, int threa
       if (a.x != nullptr) {
 #pragma unroll
         for (int j = 0; j < kCols; ++j) {
-          n2[j] = in_row<FULL>(j, left) ? (at8(r.x, j) - st.z) * st.w : 0.f;
+          n2[j] = (at8(r.x, j) - st.z) * st.w;
           n1[j] = fmaf(ag[j], fmaf(n2[j], at8(pw, j), at8(pb, j)), n1[j]);
         }
       }
@@ -313,12 +331,13 @@ __global__ void __launch_bounds__(768) block_norm_bwd(BlockNormArgs a, int threa
 #pragma unroll
         for (int j = 0; j < kCols; ++j) {
           const float g = at8(r.dy, j);
-          n1[j] = in_row<FULL>(j, left) ? (n1[j] - st.x) * st.y : 0.f;
+          n1[j] = (n1[j] - st.x) * st.y;
           sum[kW1][j] = fmaf(g, n1[j], sum[kW1][j]);
           sum[kB1][j] += g;
           dy[j] = g * at8(w, j);
-          p += dy[j];
-          q = fmaf(dy[j], n1[j], q);
+          const float own = counts<R>(j, left) ? dy[j] : 0.f;
+          p += own;
+          q = fmaf(own, n1[j], q);
         }
       }
     }
@@ -326,7 +345,7 @@ __global__ void __launch_bounds__(768) block_norm_bwd(BlockNormArgs a, int threa
     const int gate = t.gate;
     const bool last = t.last(a);
     t.next(a, units);
-    if (i + 1 < iterations) fetch<T, FULL>(a, t, c, left, r);
+    if (i + 1 < iterations) fetch<T, R>(a, t, c, left, r);
     if (a.dy != nullptr) {
       team.sum2(p, q);
       p = a.rms ? 0.f : p / a.d;
@@ -338,18 +357,18 @@ __global__ void __launch_bounds__(768) block_norm_bwd(BlockNormArgs a, int threa
 #pragma unroll
         for (int j = 0; j < kCols; ++j) ds[j] = fmaf(st.y, dy[j] - p - n1[j] * q, ds[j]);
       }
-      if (a.dres != nullptr) write8<FULL, true>(static_cast<T*>(a.dres) + at, left, ds);
+      if (a.dres != nullptr) write8<R != kShort, kStream>(static_cast<T*>(a.dres) + at, left, ds);
       if (a.x != nullptr) {
 #pragma unroll
         for (int j = 0; j < kCols; ++j) {
-          const float s = in_row<FULL>(j, left) ? ds[j] : 0.f;
-          sum[kG][j] = fmaf(s, fmaf(n2[j], at8(pw, j), at8(pb, j)), sum[kG][j]);
-          const float dh = s * ag[j];
+          sum[kG][j] = fmaf(ds[j], fmaf(n2[j], at8(pw, j), at8(pb, j)), sum[kG][j]);
+          const float dh = ds[j] * ag[j];
           sum[kW2][j] = fmaf(dh, n2[j], sum[kW2][j]);
           sum[kB2][j] += dh;
           ds[j] = dh * at8(pw, j);  // the gradient of n2; of x itself without a norm
-          u += ds[j];
-          v = fmaf(ds[j], n2[j], v);
+          const float own = counts<R>(j, left) ? ds[j] : 0.f;
+          u += own;
+          v = fmaf(own, n2[j], v);
         }
       }
     }
@@ -364,10 +383,10 @@ __global__ void __launch_bounds__(768) block_norm_bwd(BlockNormArgs a, int threa
       if (a.dx != nullptr) {
 #pragma unroll
         for (int j = 0; j < kCols; ++j) ds[j] = st.w * (ds[j] - u - n2[j] * v);
-        write8<FULL, true>(static_cast<T*>(a.dx) + at, left, ds);
+        write8<R != kShort, kStream>(static_cast<T*>(a.dx) + at, left, ds);
       }
       if (a.gate_direct && last) {
-        write_gate<T, FULL>(a, gate, c, left, sum[kG]);
+        write_gate<T, R>(a, gate, c, left, sum[kG]);
 #pragma unroll
         for (int j = 0; j < kCols; ++j) sum[kG][j] = 0.f;
       }
@@ -378,7 +397,7 @@ __global__ void __launch_bounds__(768) block_norm_bwd(BlockNormArgs a, int threa
 #pragma unroll
   for (int j = 0; j < kCols; ++j) sum[kG][j] *= a.alpha;
   if (a.gate_part != nullptr && left > 0)
-    write8<FULL, false>(a.gate_part + static_cast<int64_t>(unit) * a.d + c, left, sum[kG]);
+    write8<R != kShort, false>(a.gate_part + static_cast<int64_t>(unit) * a.d + c, left, sum[kG]);
 #pragma unroll
   for (int q = 0; q < kSums; ++q) {
     if (a.part[q] == nullptr) continue;
@@ -395,13 +414,13 @@ __global__ void __launch_bounds__(768) block_norm_bwd(BlockNormArgs a, int threa
         for (int j = 0; j < kCols; ++j) sum[q][j] += buf[j * team_size + lane];
       }
     }
-    if (tm == 0 && left > 0) write8<FULL, false>(a.part[q] + static_cast<int64_t>(blockIdx.x) * a.d + c, left, sum[q]);
+    if (tm == 0 && left > 0) write8<R != kShort, false>(a.part[q] + static_cast<int64_t>(blockIdx.x) * a.d + c, left, sum[q]);
   }
 }
 
 // Wider rows, whose elements leave no registers for the column sums: one row a block.  What the
 // column sums need of a row's reductions goes to a.pq.
-template <typename T, int V, bool FULL>
+template <typename T, int V, int R>
 __global__ void __launch_bounds__(1024) block_norm_bwd_rows(BlockNormArgs a) {
   __shared__ float smem[64];
   const int team_size = blockDim.x, lane = threadIdx.x;
@@ -410,17 +429,16 @@ __global__ void __launch_bounds__(1024) block_norm_bwd_rows(BlockNormArgs a) {
   const float4 st = reinterpret_cast<const float4*>(a.stats)[row];
   RowData<T> r[V];  // all loads first
   float n1[V][kCols], n2[V][kCols], dy[V][kCols], ds[V][kCols];
-  int left[V];
+  int col[V], left[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    const int c = (k * team_size + lane) * kCols;
-    left[k] = a.d - c;
-    load_row<T, FULL>(a, row, c, left[k], r[k]);
+    const int c = col[k] = column<R>(k * team_size + lane, a.d, left[k]);
+    load_row<T, R>(a, row, c, left[k], r[k]);
   }
   float p = 0.f, q = 0.f;
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    const int c = (k * team_size + lane) * kCols;
+    const int c = col[k];
     if (left[k] <= 0) continue;
 #pragma unroll
     for (int j = 0; j < kCols; ++j) {
@@ -431,24 +449,25 @@ __global__ void __launch_bounds__(1024) block_norm_bwd_rows(BlockNormArgs a) {
     }
     if (a.x != nullptr) {
       float pw[kCols], pb[kCols], g[kCols];
-      read_opt<FULL, T>(a.pw, a.w_f32, c, left[k], 1.f, pw);
-      read_opt<FULL, T>(a.pb, a.w_f32, c, left[k], 0.f, pb);
-      read_opt<FULL, T>(a.gate, a.gate_f32, gate_row + c, left[k], 1.f, g);
+      read_opt<R, T>(a.pw, a.w_f32, c, left[k], 1.f, pw);
+      read_opt<R, T>(a.pb, a.w_f32, c, left[k], 0.f, pb);
+      read_opt<R, T>(a.gate, a.gate_f32, gate_row + c, left[k], 1.f, g);
 #pragma unroll
       for (int j = 0; j < kCols; ++j) {
-        n2[k][j] = in_row<FULL>(j, left[k]) ? (n2[k][j] - st.z) * st.w : 0.f;
+        n2[k][j] = (n2[k][j] - st.z) * st.w;
         n1[k][j] = fmaf(a.alpha * g[j], fmaf(n2[k][j], pw[j], pb[j]), n1[k][j]);
       }
     }
     if (a.dy != nullptr) {
       float w[kCols];
-      read_opt<FULL, T>(a.w, a.w_f32, c, left[k], 1.f, w);
+      read_opt<R, T>(a.w, a.w_f32, c, left[k], 1.f, w);
 #pragma unroll
       for (int j = 0; j < kCols; ++j) {
-        n1[k][j] = in_row<FULL>(j, left[k]) ? (n1[k][j] - st.x) * st.y : 0.f;
+        n1[k][j] = (n1[k][j] - st.x) * st.y;
         dy[k][j] *= w[j];
-        p += dy[k][j];
-        q = fmaf(dy[k][j], n1[k][j], q);
+        const float own = counts<R>(j, left[k]) ? dy[k][j] : 0.f;
+        p += own;
+        q = fmaf(own, n1[k][j], q);
       }
     }
   }
@@ -461,22 +480,23 @@ __global__ void __launch_bounds__(1024) block_norm_bwd_rows(BlockNormArgs a) {
   float u = 0.f, v = 0.f;
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    const int c = (k * team_size + lane) * kCols;
+    const int c = col[k];
     if (left[k] <= 0) continue;
     if (a.dy != nullptr) {
 #pragma unroll
       for (int j = 0; j < kCols; ++j) ds[k][j] = fmaf(st.y, dy[k][j] - p - n1[k][j] * q, ds[k][j]);
     }
-    if (a.dres != nullptr) write8<FULL, true>(static_cast<T*>(a.dres) + row * a.d + c, left[k], ds[k]);
+    if (a.dres != nullptr) write8<R != kShort, true>(static_cast<T*>(a.dres) + row * a.d + c, left[k], ds[k]);
     if (a.x == nullptr) continue;
     float pw[kCols], g[kCols];
-    read_opt<FULL, T>(a.pw, a.w_f32, c, left[k], 1.f, pw);
-    read_opt<FULL, T>(a.gate, a.gate_f32, gate_row + c, left[k], 1.f, g);
+    read_opt<R, T>(a.pw, a.w_f32, c, left[k], 1.f, pw);
+    read_opt<R, T>(a.gate, a.gate_f32, gate_row + c, left[k], 1.f, g);
 #pragma unroll
     for (int j = 0; j < kCols; ++j) {
-      ds[k][j] = in_row<FULL>(j, left[k]) ? a.alpha * g[j] * ds[k][j] * pw[j] : 0.f;
-      u += ds[k][j];
-      v = fmaf(ds[k][j], n2[k][j], v);
+      ds[k][j] = a.alpha * g[j] * ds[k][j] * pw[j];
+      const float own = counts<R>(j, left[k]) ? ds[k][j] : 0.f;
+      u += own;
+      v = fmaf(own, n2[k][j], v);
     }
   }
   if (a.dx == nullptr) return;
@@ -489,25 +509,26 @@ __global__ void __launch_bounds__(1024) block_norm_bwd_rows(BlockNormArgs a) {
   }
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    const int c = (k * team_size + lane) * kCols;
+    const int c = col[k];
     if (left[k] <= 0) continue;
 #pragma unroll
     for (int j = 0; j < kCols; ++j) ds[k][j] = st.w * (ds[k][j] - u - n2[k][j] * v);
-    write8<FULL, true>(static_cast<T*>(a.dx) + row * a.d + c, left[k], ds[k]);
+    write8<R != kShort, true>(static_cast<T*>(a.dx) + row * a.d + c, left[k], ds[k]);
   }
 }
 
 // The column sums of wide rows: a thread takes 8 columns of a unit's rows and forms n1, n2 and dS
 // again from the rows and their reductions.  blockIdx.y: the unit.
-template <typename T, bool FULL>
+template <typename T, int R>
 __global__ void __launch_bounds__(256) block_norm_bwd_columns(BlockNormArgs a, int iterations) {
-  const int c = (blockIdx.x * 256 + threadIdx.x) * kCols, left = a.d - c;
+  int left;
+  const int c = column<R>(blockIdx.x * 256 + threadIdx.x, a.d, left);
   if (left <= 0) return;
   const int unit = blockIdx.y, units = gridDim.y;
   float w[kCols], pw[kCols], pb[kCols], ag[kCols], sum[kSums][kCols];
-  read_opt<FULL, T>(a.w, a.w_f32, c, left, 1.f, w);
-  read_opt<FULL, T>(a.pw, a.w_f32, c, left, 1.f, pw);
-  read_opt<FULL, T>(a.pb, a.w_f32, c, left, 0.f, pb);
+  read_opt<R, T>(a.w, a.w_f32, c, left, 1.f, w);
+  read_opt<R, T>(a.pw, a.w_f32, c, left, 1.f, pw);
+  read_opt<R, T>(a.pb, a.w_f32, c, left, 0.f, pb);
 #pragma unroll
   for (int j = 0; j < kCols; ++j) {
     ag[j] = a.alpha;
@@ -519,14 +540,14 @@ __global__ void __launch_bounds__(256) block_norm_bwd_columns(BlockNormArgs a, i
   RowData<T> r;
   float2 pq = make_float2(0.f, 0.f);
   auto load = [&] {
-    fetch<T, FULL>(a, t, c, left, r);
+    fetch<T, R>(a, t, c, left, r);
     if (t.live) pq = reinterpret_cast<const float2*>(a.pq)[t.row];
   };
   load();
   for (int i = 0; i < iterations && t.live; ++i) {
     if (a.gate != nullptr && t.gate != gate_now) {
       gate_now = t.gate;
-      read_opt<FULL, T>(a.gate, a.gate_f32, static_cast<int64_t>(t.gate) * a.d + c, left, 1.f, ag);
+      read_opt<R, T>(a.gate, a.gate_f32, static_cast<int64_t>(t.gate) * a.d + c, left, 1.f, ag);
 #pragma unroll
       for (int j = 0; j < kCols; ++j) ag[j] *= a.alpha;
     }
@@ -553,17 +574,17 @@ __global__ void __launch_bounds__(256) block_norm_bwd_columns(BlockNormArgs a, i
       sum[kB2][j] += dh;
     }
     if (a.gate_direct && last) {
-      write_gate<T, FULL>(a, gate, c, left, sum[kG]);
+      write_gate<T, R>(a, gate, c, left, sum[kG]);
 #pragma unroll
       for (int j = 0; j < kCols; ++j) sum[kG][j] = 0.f;
     }
   }
 #pragma unroll
   for (int j = 0; j < kCols; ++j) sum[kG][j] *= a.alpha;
-  if (a.gate_part != nullptr) write8<FULL, false>(a.gate_part + static_cast<int64_t>(unit) * a.d + c, left, sum[kG]);
+  if (a.gate_part != nullptr) write8<R != kShort, false>(a.gate_part + static_cast<int64_t>(unit) * a.d + c, left, sum[kG]);
 #pragma unroll
   for (int q = 0; q < kSums; ++q)
-    if (a.part[q] != nullptr) write8<FULL, false>(a.part[q] + static_cast<int64_t>(unit) * a.d + c, left, sum[q]);
+    if (a.part[q] != nullptr) write8<R != kShort, false>(a.part[q] + static_cast<int64_t>(unit) * a.d + c, left, sum[q]);
 }
 
 // out[g][c] = (or +=) the sum over `split` partial rows; 32 columns x 32 row groups a block
@@ -624,13 +645,15 @@ int block_norm_fwd(int dt, const BlockNormArgs& a, hipStream_t s) {
   const int64_t rows_of_block = wave ? 256 / team : 1, blocks = (a.rows + rows_of_block - 1) / rows_of_block;
   if (blocks > 0x7fffffff) return -3;
   SMPK_DISPATCH(dt, T, {
-    const bool full = a.d % kCols == 0;
-    const auto kernel = sub == 8    ? (full ? block_norm_fwd<T, 1, true, 8> : block_norm_fwd<T, 1, false, 8>)
-                        : sub == 16 ? (full ? block_norm_fwd<T, 1, true, 16> : block_norm_fwd<T, 1, false, 16>)
-                        : sub == 32 ? (full ? block_norm_fwd<T, 1, true, 32> : block_norm_fwd<T, 1, false, 32>)
-                        : v == 1    ? (full ? block_norm_fwd<T, 1, true, 0> : block_norm_fwd<T, 1, false, 0>)
-                        : v == 2    ? (full ? block_norm_fwd<T, 2, true, 0> : block_norm_fwd<T, 2, false, 0>)
-                                    : (full ? block_norm_fwd<T, 4, true, 0> : block_norm_fwd<T, 4, false, 0>);
+    const bool whole = a.d % kCols == 0;
+    const auto kernel =
+        sub == 8    ? (whole ? block_norm_fwd<T, 1, kWhole, 8>
+                             : a.d > kCols ? block_norm_fwd<T, 1, kOverlap, 8> : block_norm_fwd<T, 1, kShort, 8>)
+        : sub == 16 ? (whole ? block_norm_fwd<T, 1, kWhole, 16> : block_norm_fwd<T, 1, kOverlap, 16>)
+        : sub == 32 ? (whole ? block_norm_fwd<T, 1, kWhole, 32> : block_norm_fwd<T, 1, kOverlap, 32>)
+        : v == 1    ? (whole ? block_norm_fwd<T, 1, kWhole, 0> : block_norm_fwd<T, 1, kOverlap, 0>)
+        : v == 2    ? (whole ? block_norm_fwd<T, 2, kWhole, 0> : block_norm_fwd<T, 2, kOverlap, 0>)
+                    : (whole ? block_norm_fwd<T, 4, kWhole, 0> : block_norm_fwd<T, 4, kOverlap, 0>);
     kernel<<<static_cast<unsigned>(blocks), wave ? 256 : team, 0, s>>>(a, team);
   });
   return static_cast<int>(hipGetLastError());
@@ -660,33 +683,36 @@ int block_norm_bwd_plan(int64_t rows, int64_t d, int64_t gate_rows, BlockNormPla
 }
 
 namespace {
-template <typename T, typename W, bool FULL>
+template <typename T, typename W, int R>
 void launch_bwd(const BlockNormArgs& a, const BlockNormPlan& p, hipStream_t s) {
   const int iterations = static_cast<int>(p.iterations);
   if (p.two_pass) {
     const int64_t vectors = (a.d + kCols - 1) / kCols;
     const int v = vectors <= 1024 ? 1 : 2;
-    const auto kernel = v == 1 ? block_norm_bwd_rows<T, 1, FULL> : block_norm_bwd_rows<T, 2, FULL>;
+    const auto kernel = v == 1 ? block_norm_bwd_rows<T, 1, R> : block_norm_bwd_rows<T, 2, R>;
     kernel<<<static_cast<unsigned>(a.rows), static_cast<unsigned>(((vectors + v - 1) / v + 63) / 64 * 64), 0, s>>>(a);
     bool sums = a.gate_direct || a.gate_part != nullptr;
     for (float* q : a.part) sums = sums || q != nullptr;
     if (!sums) return;
     const unsigned columns = static_cast<unsigned>((vectors + 255) / 256);
-    block_norm_bwd_columns<T, FULL><<<dim3(columns, static_cast<unsigned>(p.units)), 256, 0, s>>>(a, iterations);
+    block_norm_bwd_columns<T, R><<<dim3(columns, static_cast<unsigned>(p.units)), 256, 0, s>>>(a, iterations);
     return;
   }
-  const auto kernel = p.team == 8    ? block_norm_bwd<T, W, FULL, 8>
-                      : p.team == 16 ? block_norm_bwd<T, W, FULL, 16>
-                      : p.team == 32 ? block_norm_bwd<T, W, FULL, 32>
-                                     : block_norm_bwd<T, W, FULL, 0>;
+  const auto kernel = p.team == 8    ? block_norm_bwd<T, W, R, 8>
+                      : p.team == 16 ? block_norm_bwd<T, W, R, 16>
+                      : p.team == 32 ? block_norm_bwd<T, W, R, 32>
+                                     : block_norm_bwd<T, W, R, 0>;
   kernel<<<static_cast<unsigned>(p.blocks), p.threads, p.lds, s>>>(a, p.team, iterations);
 }
 template <typename T, typename W>
 void launch_bwd_of(const BlockNormArgs& a, const BlockNormPlan& p, hipStream_t s) {
   if (a.d % kCols == 0) {
-    launch_bwd<T, W, true>(a, p, s);
+    launch_bwd<T, W, kWhole>(a, p, s);
+  } else if (a.d > kCols) {
+    launch_bwd<T, W, kOverlap>(a, p, s);
   } else {
-    launch_bwd<T, W, false>(a, p, s);
+    block_norm_bwd<T, W, kShort, 8><<<static_cast<unsigned>(p.blocks), p.threads, p.lds, s>>>(
+        a, p.team, static_cast<int>(p.iterations));
   }
 }
 }  // namespace

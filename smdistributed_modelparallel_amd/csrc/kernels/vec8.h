@@ -1,9 +1,9 @@
 // Eight consecutive elements of a row in one thread, at any alignment.
 //
 // Rows of odd widths start off 16 bytes.  The hardware loads and stores 16 bytes at any address,
-// so such rows move in the same wide accesses; only a row's last, partial vector goes element by
-// element.  FULL: rows are whole vectors -- no thread branches on `left` (the elements from here to
-// the row's end), and the loads of a batch are issued without a wait between them.
+// so such rows move in the same wide accesses.  FULL: the vector is whole -- no thread branches on
+// `left` (the elements from here to the row's end), and the loads of a batch are issued without a
+// wait between them.  Otherwise a row's last, partial vector goes element by element.
 #pragma once
 #include "common.h"
 
