@@ -95,6 +95,15 @@ def test_long_lists(b, s, rows, dim):
     check(b, s, rows, dim, torch.bfloat16, positions="implicit")
 
 
+@pytest.mark.parametrize("positions", ["none", "implicit", "given"])
+@pytest.mark.parametrize("b,s,rows,dim,dtype", [(4, 5000, 900, 264, torch.bfloat16), (3, 6000, 60000, 264, torch.float32),
+                                                (3, 6000, 2000, 521, torch.float16), (80, 300, 5000, 600, torch.float32),
+                                                (2, 9000, 1100000, 257, torch.bfloat16)])
+def test_long_lists_of_wide_rows(positions, b, s, rows, dim, dtype):
+    """Position sums and zeros that run beside the sort of the tokens."""
+    check(b, s, rows, dim, dtype, positions=positions, padding=5)
+
+
 @pytest.mark.parametrize("positions", ["implicit", "given"])
 @pytest.mark.parametrize("dtype,dim", [(torch.float32, 36), (torch.bfloat16, 1600), (torch.float16, 37)])
 def test_positions_and_scale(positions, dtype, dim):
