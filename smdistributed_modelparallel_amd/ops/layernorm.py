@@ -186,8 +186,8 @@ def _block_norm_hip(x, residual, weight, bias, post_weight, post_bias, gate, gat
 
 
 def _gate_matrix(gate, shape):
-    """The gate as [groups, d] where each row serves a run of consecutive rows of the input, and
-    the length of that run.  Gates that broadcast otherwise are expanded, in fp32: autograd sums
+    """The gate as rows of d elements, each for a run of consecutive rows of the input, and the
+    length of that run.  Gates that broadcast otherwise are expanded, in fp32: autograd sums
     their gradient back, and its terms must not be rounded before they are added."""
     d = shape[-1]
     if gate.shape == (d,):
@@ -201,7 +201,7 @@ def _gate_matrix(gate, shape):
     if any(n != 1 for n in lead[k:]):
         gate, k = gate.float().expand(*shape), len(shape) - 1
     groups = math.prod(shape[:k])
-    return gate.reshape(groups, d), math.prod(shape[:-1]) // max(groups, 1)
+    return gate, math.prod(shape[:-1]) // max(groups, 1)
 
 
 def _norm_torch(v, weight, bias, eps, rms):
