@@ -308,16 +308,18 @@ class DistributedOptimizer(torch.optim.Optimizer):
         ranges = [self._grad_range(d) for d in self.domains if not (once and d.key == "default")]
         # fp64 over the ranks too: no finite gradient overflows the sum of squares
         acc = mt.grad_power(ranges, norm_type, scale=1.0 / self.loss_scale).to(dev)
-        op = dist.ReduceOp.SUM if norm_type == 2 else dist.ReduceOp.MAX
+        total, op = acc, dist.ReduceOp.SUM
+        if norm_type != 2:  # as whole numbers, in the same order: a maximum of floats may lose a rank's NaN
+            total, op = acc.abs().view(torch.int64), dist.ReduceOp.MAX
         if state.sdp is not None:
             # every replica holds identical reduced shards: the norm spans one shard group
             if state.pgs.shard is not None:
-                dist.all_reduce(acc, op=op, group=state.pgs.shard)
+                dist.all_reduce(total, op=op, group=state.pgs.shard)
         elif state.cfg.shard_optimizer_state and core.dp_size() > 1:
-            dist.all_reduce(acc, op=op, group=state.pgs.world)
+            dist.all_reduce(total, op=op, group=state.pgs.world)
         elif core.mp_size() > 1:
-            dist.all_reduce(acc, op=op, group=state.pgs.mp)
-        norm = (acc.sqrt() if norm_type == 2 else acc).float()
+            dist.all_reduce(total, op=op, group=state.pgs.mp)
+        norm = (total.sqrt() if norm_type == 2 else total.view(torch.float64)).float()
         coef = torch.clamp(max_norm / (norm + 1e-6), max=1.0)
         self._clip_coef = coef
         return norm

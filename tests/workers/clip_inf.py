@@ -47,6 +47,14 @@ def main():
         full = dict(ref.named_parameters())
         for n, p in model.local_named_parameters():
             assert torch.allclose(p, full[n], rtol=1e-5, atol=1e-7), n
+    # a NaN of one stage reaches all of them
+    for bad in range(2):
+        opt.zero_grad()
+        train(model, x)
+        if smp.pp_rank() == bad:
+            next(p for _, p in model.local_named_parameters()).grad[0] = math.nan
+        assert math.isnan(float(opt.clip_master_grads(1.0, math.inf))), bad
+        opt._clip_coef = None
     try:
         opt.clip_master_grads(1.0, 1)
     except ValueError:
