@@ -554,7 +554,7 @@ void check_disjoint(const std::vector<at::Tensor>& in, const std::vector<at::Ten
     if (in[i].numel() == 0) continue;
     const auto a = extent(in[i]), b = extent(out[i]);
     r.push_back({b.first, b.second, true});
-    if (a != b) r.push_back({a.first, a.second, false});
+    if (a != b || in[i].scalar_type() != out[i].scalar_type()) r.push_back({a.first, a.second, false});
   }
   std::sort(r.begin(), r.end(), [](const Range& x, const Range& y) { return x.s < y.s; });
   uintptr_t end = 0, write_end = 0;

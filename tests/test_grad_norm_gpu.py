@@ -133,6 +133,17 @@ def test_shared_memory_is_refused():
     assert x.eq(1).all()
 
 
+def test_one_memory_as_two_types_is_refused():
+    from smdistributed_modelparallel_amd.backend.exceptions import SMPInvalidArgumentError
+    from smdistributed_modelparallel_amd.ops.multi_tensor import clip_grad_norm_
+
+    for device in ("cpu", "cuda"):
+        x = torch.ones(100, device=device, dtype=torch.float16)
+        with pytest.raises(SMPInvalidArgumentError):
+            clip_grad_norm_([x], 100.0, out=[x.view(torch.bfloat16)])
+        assert x.eq(1).all()
+
+
 def test_parameters_of_a_model():
     from smdistributed_modelparallel_amd.optimizers import clip_grad_norm_
 
