@@ -268,6 +268,11 @@ struct EmbeddingGrad {
   float* part;
   uint8_t* marks;
 };
+// The same for short lists into small tables, without workspaces: all tables have to be allowed.
+// bytes: of a dense gradient that is written, 0 for one that is added to.
+bool embedding_bwd_short(int64_t n, int64_t d, int64_t rows, int64_t bytes);
+int embedding_bwd_of_short(int dt, const void* dy, int64_t n, int64_t d, const EmbeddingGrad* tables, int count,
+                           hipStream_t s);
 // Up to two tables at once; their gradients must not share memory.
 int embedding_bwd(int dt, const void* dy, int64_t n, int64_t d, const EmbeddingGrad* tables, int count, hipStream_t s);
 

@@ -100,6 +100,12 @@ void embedding_bwd(at::Tensor dy, at::Tensor ids, c10::optional<at::Tensor> pos,
   int count = 0;
   int64_t bytes = 0;
   int64_t at[2][5];  // keys, tokens, counts, part, marks in the workspace
+  bool brief = true;
+  for (int i = 0; i < 2; ++i) {
+    const auto& g = i == 0 ? dw : dp;
+    if (!g.has_value()) continue;
+    brief = brief && smpk::embedding_bwd_short(n, d, g->size(0), (i == 0 ? dw_accumulate : dp_accumulate) ? 0 : g->nbytes());
+  }
   for (int i = 0; i < 2; ++i) {
     const auto& g = i == 0 ? dw : dp;
     if (!g.has_value()) continue;
@@ -116,6 +122,10 @@ void embedding_bwd(at::Tensor dy, at::Tensor ids, c10::optional<at::Tensor> pos,
     e.skip = i == 0 ? skip : -1;
     e.dw = g->data_ptr();
     e.accumulate = i == 0 ? dw_accumulate : dp_accumulate;
+    if (brief) {
+      ++count;
+      continue;
+    }
     e.plan = smpk::embedding_bwd_plan(n, d, rows, sequence ? std::max<int64_t>(n / period, 1) : 0);
     const bool sort = !sequence && n > 0;
     const int64_t lists = e.plan.one_launch ? 4 * n : 8 * n;
@@ -128,6 +138,10 @@ void embedding_bwd(at::Tensor dy, at::Tensor ids, c10::optional<at::Tensor> pos,
     ++count;
   }
   if (count == 0) return;
+  if (brief) {
+    check(smpk::embedding_bwd_of_short(dt_code(dy, "embedding"), dy.data_ptr(), n, d, t, count, stream()), "embedding_bwd");
+    return;
+  }
   auto ws = at::empty({bytes}, dy.options().dtype(at::kByte));
   uint8_t* const base = ws.data_ptr<uint8_t>();
   for (int i = 0; i < count; ++i) {

@@ -95,6 +95,16 @@ def test_long_lists(b, s, rows, dim):
     check(b, s, rows, dim, torch.bfloat16, positions="implicit")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("positions", ["none", "implicit", "given"])
+@pytest.mark.parametrize("b,s,rows,dim", [(2, 256, 1, 8), (1, 512, 3, 512), (1, 513, 3, 16), (16, 1, 30000, 1027), (2, 65, 2500, 520),
+                                          (3, 100, 1048576, 12), (3, 99, 1048577, 12), (1, 15, 1000, 16384), (7, 64, 5, 585),
+                                          (7, 64, 5, 586), (1, 1, 2, 1)])
+def test_short_lists(b, s, rows, dim, positions, dtype):
+    """At the limits of the kernel for short lists and just beyond them; few rows of many tokens."""
+    check(b, s, rows, dim, dtype, positions=positions, padding=rows - 1 if rows > 1 else None, scale=0.5)
+
+
 @pytest.mark.parametrize("positions", ["none", "implicit", "given"])
 @pytest.mark.parametrize("b,s,rows,dim,dtype", [(4, 5000, 900, 264, torch.bfloat16), (3, 6000, 60000, 264, torch.float32),
                                                 (3, 6000, 2000, 521, torch.float16), (80, 300, 5000, 600, torch.float32),
