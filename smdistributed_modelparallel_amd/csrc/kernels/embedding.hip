@@ -34,13 +34,22 @@ constexpr int kPerThread = 4;  // vectors of a thread, all loads in flight toget
 
 // Vectors of the output in order, kT * kPerThread of them a block: all lanes are busy at any width.
 // Threads past the end and tokens without a row load row 0 and drop it: no branch separates the
-// loads.
+// loads.  slice: an XCD (every kXcds-th block) takes `slice` blocks of each sequence, the same
+// positions of all of them (or nearly: in whole blocks), so that its L2 holds their rows.  32 x 1000 tokens of 1600
+// bf16: 33 us, and 43 us with the blocks in order; 32 x 2048, whose sequences are multiples of kXcds
+// blocks in any case: 84 us both.
+constexpr uint32_t kXcds = 8;
 template <typename T, bool FULL>
 __global__ void __launch_bounds__(kT) emb_fwd(IndexList ids, const T* __restrict__ w, int64_t w_stride, float scale,
                                               int foreign_zero, IndexList pos, const T* __restrict__ p,
                                               int64_t p_stride, T* __restrict__ y, int n, int d, uint32_t per_row,
-                                              uint32_t reciprocal) {
-  const int64_t v0 = static_cast<int64_t>(blockIdx.x) * (kT * kPerThread);
+                                              uint32_t reciprocal, uint32_t slice) {
+  uint32_t block = blockIdx.x;
+  if (slice != 0 && block < gridDim.x / (kXcds * slice) * (kXcds * slice)) {
+    const uint32_t k = block / kXcds, sequence = k / slice;
+    block = (sequence * kXcds + block % kXcds) * slice + (k - sequence * slice);
+  }
+  const int64_t v0 = static_cast<int64_t>(block) * (kT * kPerThread);
   const int t0 = static_cast<int>(v0 / per_row);
   const uint32_t r0 = static_cast<uint32_t>(v0 - static_cast<int64_t>(t0) * per_row);
   int t[kPerThread], c[kPerThread];
@@ -806,12 +815,15 @@ int embedding_fwd(int dt, const IndexList& ids, const void* w, int64_t w_stride,
   const int64_t blocks = (n * per_row + kT * kPerThread - 1) / (kT * kPerThread);
   if (blocks > 0x7fffffff || n > 0x7fffffff - kT * kPerThread) return -3;
   const uint32_t reciprocal = per_row == 1 ? 0xffffffffu : static_cast<uint32_t>((1ull << 32) / per_row);
+  uint32_t slice = 0;
+  if (p != nullptr && pos.ids == nullptr)
+    slice = static_cast<uint32_t>((pos.period * per_row + kXcds * kT * kPerThread / 2) / (kXcds * kT * kPerThread));
   SMPK_DISPATCH(dt, T, {
     const auto kernel = d % kCols == 0 ? emb_fwd<T, true> : emb_fwd<T, false>;
     kernel<<<static_cast<unsigned>(blocks), kT, 0, s>>>(ids, static_cast<const T*>(w), w_stride, scale, foreign_zero, pos,
                                                        static_cast<const T*>(p), p_stride, static_cast<T*>(y),
                                                        static_cast<int>(n), static_cast<int>(d),
-                                                       static_cast<uint32_t>(per_row), reciprocal);
+                                                       static_cast<uint32_t>(per_row), reciprocal, slice);
   });
   return static_cast<int>(hipGetLastError());
 }
