@@ -22,8 +22,8 @@
 // barrier, and the rows of a CU's waves overlap freely.  Wider rows, and all wider rows of the
 // backward, belong to a team of waves.
 //
-// Measured, bf16: 16384 x 1600 with a gate, forward 45 us (4.7 TB/s), backward 70 us (4.5 TB/s);
-// 16384 x 4096 root-mean-square with fp32 weights, 105 us and 160 us (5.0 TB/s); a copy of 1 GiB
+// Measured, bf16: 16384 x 1600 with a gate, forward 45 us (4.7 TB/s), backward 65 us (4.8 TB/s);
+// 16384 x 4096 root-mean-square with fp32 weights, 105 us and 168 us (4.8 TB/s); a copy of 1 GiB
 // reaches 5.1 TB/s.
 #include "kernels.h"
 #include "vec8.h"
@@ -587,12 +587,14 @@ __global__ void __launch_bounds__(256) block_norm_bwd_columns(BlockNormArgs a, i
     if (a.part[q] != nullptr) write8<R != kShort, false>(a.part[q] + static_cast<int64_t>(unit) * a.d + c, left, sum[q]);
 }
 
-// out[g][c] = (or +=) the sum over `split` partial rows; 32 columns x 32 row groups a block
+// out[g][c] = (or +=) the sum over `split` partial rows; 32 columns x 32 row groups a block.  9 us for two
+// vectors of 256 partial rows and 16 gate rows of 4096.
 __global__ void __launch_bounds__(1024) block_norm_join(BlockNormJoin l, int d) {
   __shared__ float buf[32][33];
-  const BlockNormJoin::Item& it = l.item[blockIdx.y];
-  const int64_t g = blockIdx.z;
-  if (g >= it.groups) return;
+  int64_t g = blockIdx.y;
+  int i = 0;
+  while (g >= l.item[i].groups) g -= l.item[i++].groups;  // (the grid has one y for each group of each item)
+  const BlockNormJoin::Item& it = l.item[i];
   const int x = threadIdx.x & 31, r = threadIdx.x >> 5, c = blockIdx.x * 32 + x;
   float v = 0.f;
   if (c < d) {
@@ -732,10 +734,10 @@ int block_norm_bwd(int dt, const BlockNormArgs& a, const BlockNormPlan& p, hipSt
 
 int block_norm_join(const BlockNormJoin& l, int d, hipStream_t s) {
   if (l.count <= 0) return 0;
-  int64_t groups = 1;
-  for (int i = 0; i < l.count; ++i) groups = l.item[i].groups > groups ? l.item[i].groups : groups;
+  int64_t groups = 0;
+  for (int i = 0; i < l.count; ++i) groups += l.item[i].groups;
   if (groups > 65535) return -3;
-  block_norm_join<<<dim3((d + 31) / 32, l.count, static_cast<unsigned>(groups)), 1024, 0, s>>>(l, d);
+  block_norm_join<<<dim3((d + 31) / 32, static_cast<unsigned>(groups)), 1024, 0, s>>>(l, d);
   return static_cast<int>(hipGetLastError());
 }
 
