@@ -329,14 +329,15 @@ def test_offsets_past_32_bits():
     assert dw[-1].eq(1).all() and dw[300_000].eq(4).all() and float(dw.sum(dtype=torch.float64)) == 5 * dim
 
 
-def test_graph_replays():
+@pytest.mark.parametrize("b", [3, 50, 200])
+def test_graph_replays(b):
     """Forward and backward captured: every replay on new ids gives what the eager call gives."""
     from smdistributed_modelparallel_amd.ops.embedding import embedding
 
     w = torch.randn(900, 64, device="cuda").requires_grad_()
     p = torch.randn(130, 64, device="cuda").requires_grad_()
-    ids = torch.randint(0, 900, (50, 128), device="cuda")
-    dy = torch.randn(50, 128, 64, device="cuda")
+    ids = torch.randint(0, 900, (b, 128), device="cuda")
+    dy = torch.randn(b, 128, 64, device="cuda")
 
     def step():
         y = embedding(ids, w, position_weight=p, scale=0.5, padding_idx=7)
@@ -351,7 +352,7 @@ def test_graph_replays():
     with torch.cuda.graph(graph):
         out = step()
     for k in range(3):
-        ids.copy_(torch.randint(0, 900 >> (4 * k), (50, 128), device="cuda"))
+        ids.copy_(torch.randint(0, 900 >> (4 * k), (b, 128), device="cuda"))
         dy.normal_()
         graph.replay()
         torch.cuda.synchronize()
