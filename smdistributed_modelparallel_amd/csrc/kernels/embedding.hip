@@ -836,8 +836,12 @@ bool embedding_bwd_short(int64_t n, int64_t d, int64_t rows, int64_t bytes) {
 }
 
 EmbeddingPlan embedding_bwd_plan(int64_t n, int64_t d, int64_t rows, int64_t batch) {
-  const bool sorted = batch > 0 || n <= 0;
   EmbeddingPlan p{};
+  if (n <= 0) {  // nothing to order, to add up or to join: rows are cleared at most
+    p.one_launch = 1;
+    p.chunk = 16;
+    return p;
+  }
   int bits = 1;
   while ((rows >> bits) != 0) ++bits;  // the keys 0 .. rows
   p.range = static_cast<int>((rows + kRangeBlocks - 1) / kRangeBlocks);
@@ -864,8 +868,8 @@ EmbeddingPlan embedding_bwd_plan(int64_t n, int64_t d, int64_t rows, int64_t bat
   // (narrow rows share their blocks' lanes: the same time at 16, of many more blocks)
   while (d > 32 * kCols && c < 64 && n / (c * 2) >= 1024) c *= 2;
   // positions of up to 64 sequences: whole runs in a chunk, which leave nothing to join
-  p.join = !(sorted && batch <= 64);
-  if (!p.join && batch > 0) c = c < batch ? batch : c / batch * batch;
+  p.join = !(batch > 0 && batch <= 64);
+  if (!p.join) c = c < batch ? batch : c / batch * batch;
   p.chunk = static_cast<int>(c);
   p.chunks = (n + c - 1) / c;
   return p;

@@ -425,3 +425,26 @@ def test_capture_beside_an_eager_graph_is_refused():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(dw, expect)
+
+
+@pytest.mark.parametrize("rows", [262144, 262145, 300000, 1100000])
+@pytest.mark.parametrize("shape", [(0,), (3, 0), (0, 4)])
+def test_no_tokens_of_large_tables(rows, shape):
+    """An empty batch of a table of any size: dense gradients are zeros, bound ones stay as they are."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    ids = torch.empty(shape, dtype=torch.long, device="cuda")
+    for positions in (None, "implicit", "given"):
+        w, p = (torch.randn(rows, 9, device="cuda", requires_grad=True) for _ in range(2))
+        kw = {} if positions is None else {"position_weight": p}
+        if positions == "given":
+            kw["position_ids"] = ids
+        leaves = [w] if positions is None else [w, p]
+        y = embedding(ids, w, padding_idx=rows - 1, **kw)
+        assert y.shape == shape + (9,)
+        for g, t in zip(torch.autograd.grad(y, leaves, torch.empty_like(y), retain_graph=True), leaves):
+            assert g.shape == t.shape and not g.any()
+        for t in leaves:
+            t.grad, t._smp_fused_grad = torch.ones_like(t), True
+        embedding(ids, w, **kw).backward(torch.empty_like(y))
+        assert all(t.grad.eq(1).all() for t in leaves)
