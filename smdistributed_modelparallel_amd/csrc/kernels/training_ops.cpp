@@ -335,7 +335,7 @@ smpk::BlockNormArgs block_args(const Opt& x, const at::Tensor& res, const at::Te
   TORCH_CHECK(vec(w) && vec(b) && vec(pw) && vec(pb), "block_norm: weights and biases must be alike");
   if (gate.has_value()) {
     TORCH_CHECK(gate->device() == res.device() && gate->is_contiguous() && gate_rows >= 1 &&
-                    gate->numel() == rows / gate_rows * d && rows % gate_rows == 0 &&
+                    (rows == 0 || (gate->numel() == rows / gate_rows * d && rows % gate_rows == 0)) &&
                     (gate->scalar_type() == res.scalar_type() || gate->scalar_type() == at::kFloat),
                 "block_norm: bad gate");
   }

@@ -191,7 +191,7 @@ def _gate_matrix(gate, shape):
     their gradient back, and its terms must not be rounded before they are added."""
     d = shape[-1]
     if gate.shape == (d,):
-        return gate, math.prod(shape[:-1])
+        return gate, max(math.prod(shape[:-1]), 1)
     if gate.shape[-1:] != (d,):
         gate = gate.float().expand(*gate.shape[:-1], d)
     lead = (1,) * (len(shape) - gate.dim()) + tuple(gate.shape[:-1])
@@ -201,7 +201,7 @@ def _gate_matrix(gate, shape):
     if any(n != 1 for n in lead[k:]):
         gate, k = gate.float().expand(*shape), len(shape) - 1
     groups = math.prod(shape[:k])
-    return gate, math.prod(shape[:-1]) // max(groups, 1)
+    return gate, max(math.prod(shape[:-1]) // max(groups, 1), 1)  # (an input without rows has runs too)
 
 
 def _norm_torch(v, weight, bias, eps, rms):

@@ -313,3 +313,41 @@ def test_capture_beside_an_eager_graph_is_refused():
         with pytest.raises(RuntimeError, match="alive"):
             torch.autograd.grad(y, w, dy)
     assert torch.equal(torch.autograd.grad(eager, w, dy)[0], expect)
+
+
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("gate", ["none", "scalar", "channel", "sample", "places", "rows", "full"])
+@pytest.mark.parametrize("shape", [(0, 3, 8), (2, 0, 8), (0, 0, 8), (0, 3, 7000)])
+def test_no_rows_with_a_gate(shape, gate, post):
+    t = inputs(shape, torch.bfloat16, torch.float32, False, post, gate, gdtype=torch.float32)
+    leaf = {k: None if v is None else v.clone().requires_grad_() for k, v in t.items()}
+    with torch.no_grad():
+        assert all(o.shape == shape for o in call(leaf, 0.5, 1e-5, False))
+    y, s = call(leaf, 0.5, 1e-5, False)
+    assert y.shape == s.shape == shape and y.dtype == s.dtype == torch.bfloat16
+    names = [k for k, v in leaf.items() if v is not None]
+    for k, g in zip(names, torch.autograd.grad([y, s], [leaf[k] for k in names], [torch.empty_like(y)] * 2)):
+        assert g.shape == leaf[k].shape and g.dtype == leaf[k].dtype and not g.any(), k
+
+
+def test_no_rows_of_a_module_with_a_gate():
+    from smdistributed_modelparallel_amd.nn import FusedBlockNorm
+
+    m = FusedBlockNorm(24, gate=0.5).cuda()
+    for p in m.parameters():
+        p.grad, p._smp_fused_grad = torch.ones_like(p), True
+    x = torch.empty(0, 5, 24, device="cuda", requires_grad=True)
+    y, s = m(x, x)
+    (y.sum() + s.sum()).backward()
+    assert x.grad.shape == x.shape and all(p.grad.eq(1).all() for p in m.parameters())
+
+
+def test_one_row_of_a_flat_gate():
+    """Rows without leading dimensions."""
+    check((1, 1, 40), torch.float32, gate="channel")
+    t = {k: None if v is None else v.view(40) for k, v in
+         inputs((1, 1, 40), torch.float32, torch.float32, False, True, "full").items()}
+    y, s = call(t, 0.5, 1e-5, False)
+    want, slack = ref.exact(t, 0.5, 1e-5, False), ref.slack(t, 0.5, 1e-5, False)
+    within("y", y, want["y"], slack["y"])
+    within("s", s, want["s"], slack["s"])
