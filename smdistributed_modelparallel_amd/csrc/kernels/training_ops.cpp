@@ -164,10 +164,18 @@ bool accumulates(const at::Tensor& t) {
   return it != info->end() && it->second.needed_ && !it->second.captures_;
 }
 
+// Something other than the sum into t.grad wants the gradient of the leaf `t`: a hook of the tensor
+// or of its accumulator, which may change it before it is added.
+bool hooked(const at::Tensor& t) {
+  if (!torch::autograd::impl::hooks(t).empty()) return true;
+  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
+  return accumulator && !(accumulator->pre_hooks().empty() && accumulator->post_hooks().empty());
+}
+
 // The gradient of `t` goes straight into its bound slot of the flat buffer: the caller saw the
 // parameter's mark, the slot has to be there still.
 bool bound(const at::Tensor& t, bool marked) {
-  if (!marked || !t.defined() || !t.is_leaf()) return false;
+  if (!marked || !t.defined() || !t.is_leaf() || hooked(t)) return false;
   const at::Tensor& g = t.grad();
   return g.defined() && g.scalar_type() == t.scalar_type() && g.sizes() == t.sizes() && g.is_contiguous() &&
          accumulates(t);

@@ -5,7 +5,8 @@ into the tables' dtype, in one kernel (`csrc/kernels/embedding.hip`).  The backw
 gradient rows of each token's occurrences in token order and in fp32 -- the same bits on every
 run -- and writes the parameters' flat-buffer gradients in place where they are bound
 (`parallel/flat.py`): only the rows that occur are touched then, and no dense gradient exists
-(autograd gets none for them; their post-accumulate hooks still fire).
+(autograd gets none for them; their post-accumulate hooks still fire).  A parameter with other hooks
+takes its gradient through autograd: they see it, and may change it, before it is added.
 A pass that builds a graph of its own (``create_graph``) can be differentiated again.
 CPU tensors use plain torch operations.  torch.autocast changes nothing: both tables and the
 result are of one type.

@@ -351,3 +351,18 @@ def test_one_row_of_a_flat_gate():
     want, slack = ref.exact(t, 0.5, 1e-5, False), ref.slack(t, 0.5, 1e-5, False)
     within("y", y, want["y"], slack["y"])
     within("s", s, want["s"], slack["s"])
+
+
+def test_hooks_of_bound_parameters_get_their_gradients():
+    t = inputs((3, 50, 72), torch.float32, torch.float32, False, True, "channel")
+    names = ("weight", "bias", "post_weight", "post_bias", "gate")
+    u = {k: torch.nn.Parameter(v) if k in names else v for k, v in t.items()}
+    dy, ds = (torch.randn(3, 50, 72, device="cuda") for _ in range(2))
+    expect = dict(zip(names, torch.autograd.grad(call(u, 0.5, 1e-5, False), [u[k] for k in names], [dy, ds])))
+    seen = {}
+    for k in names:
+        u[k].grad, u[k]._smp_fused_grad = torch.zeros_like(u[k]), True
+        u[k].register_hook(lambda g, k=k: seen.update({k: g.clone()}) or 3 * g)
+    torch.autograd.backward(call(u, 0.5, 1e-5, False), [dy, ds])
+    for k in names:
+        assert torch.equal(seen[k], expect[k]) and torch.equal(u[k].grad, 3 * expect[k]), k

@@ -448,3 +448,34 @@ def test_no_tokens_of_large_tables(rows, shape):
             t.grad, t._smp_fused_grad = torch.ones_like(t), True
         embedding(ids, w, **kw).backward(torch.empty_like(y))
         assert all(t.grad.eq(1).all() for t in leaves)
+
+
+@pytest.mark.parametrize("of", ["tensor", "accumulator"])
+def test_hooks_of_a_bound_table_get_its_gradient(of):
+    """A tensor hook may change the gradient before it is added (rows masked here); a hook of the
+    accumulator sees it."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    g = torch.Generator(device="cuda").manual_seed(2)
+    w, p = (torch.nn.Parameter(torch.randn(n, 24, generator=g, device="cuda")) for n in (9, 6))
+    ids = torch.tensor([[4, 4, 1, 8], [0, 4, 2, 2]], device="cuda")
+    dy = torch.randn(2, 4, 24, generator=g, device="cuda")
+    expect = torch.autograd.grad(embedding(ids, w, scale=2.0, position_weight=p), [w, p], dy)
+    for t in (w, p):
+        t.grad, t._smp_fused_grad = torch.ones_like(t), True
+    slots = [w.grad, p.grad]
+    mask = (torch.arange(9, device="cuda") % 2 == 0).float().unsqueeze(1)
+    seen = []
+    if of == "tensor":
+        handle = w.register_hook(lambda g: seen.append(g.clone()) or g * mask)
+    else:
+        accumulator = w.expand_as(w).grad_fn.next_functions[0][0]
+        handle = accumulator.register_hook(lambda _, grads: seen.append(grads[0].clone()) and None)
+    embedding(ids, w, scale=2.0, position_weight=p).backward(dy)
+    assert w.grad is slots[0] and p.grad is slots[1]
+    assert len(seen) == 1 and torch.equal(seen[0], expect[0])
+    assert torch.equal(w.grad, 1 + expect[0] * (mask if of == "tensor" else 1))
+    assert float((p.grad - 1 - expect[1]).abs().max()) <= 2 * U32 * float(1 + expect[1].abs().max())
+    handle.remove()
+    embedding(ids, w, scale=2.0, position_weight=p).backward(dy)
+    assert len(seen) == 1 and w.grad is slots[0]
