@@ -172,10 +172,19 @@ bool hooked(const at::Tensor& t) {
   return accumulator && !(accumulator->pre_hooks().empty() && accumulator->post_hooks().empty());
 }
 
+// The sum into t.grad belongs on the stream that was current when the accumulator of the leaf `t` was made,
+// and autograd makes the caller wait for that stream alone.  A node of another stream returns its gradient,
+// which autograd brings there.
+bool here(const at::Tensor& t) {
+  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
+  const auto of_leaf = accumulator ? accumulator->stream() : std::nullopt;
+  return !of_leaf.has_value() || of_leaf->id() == at::hip::getCurrentHIPStream(t.device().index()).id();
+}
+
 // The gradient of `t` goes straight into its bound slot of the flat buffer: the caller saw the
 // parameter's mark, the slot has to be there still.
 bool bound(const at::Tensor& t, bool marked) {
-  if (!marked || !t.defined() || !t.is_leaf() || hooked(t)) return false;
+  if (!marked || !t.defined() || !t.is_leaf() || hooked(t) || !here(t)) return false;
   const at::Tensor& g = t.grad();
   return g.defined() && g.scalar_type() == t.scalar_type() && g.sizes() == t.sizes() && g.is_contiguous() &&
          accumulates(t);

@@ -146,3 +146,87 @@ def test_distributed_embedding_module():
     y.sum().backward()
     assert torch.equal(m.weight.grad[:, 0], torch.bincount(ids.flatten(), minlength=40).float() * (torch.arange(40, device="cuda") != 3))
     assert m.double()(ids).dtype == torch.float64
+
+
+def _bound(*tensors):
+    out = [torch.nn.Parameter(t.clone()) for t in tensors]
+    for t in out:
+        t.grad, t._smp_fused_grad = torch.zeros_like(t), True
+    return out
+
+
+def test_bound_gradients_of_two_streams():
+    """One bound parameter used on two streams of one graph gets the sum of both uses, also where the
+    caller reads it without waiting for either stream itself."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+    from smdistributed_modelparallel_amd.ops.layernorm import block_norm
+
+    torch.manual_seed(0)
+    table, scale = torch.randn(6000, 520, device="cuda"), torch.randn(520, device="cuda")
+    ids = [torch.randint(0, 6000, (40000,), device="cuda") for _ in range(2)]
+    x = [torch.randn(40000, 520, device="cuda") for _ in range(2)]
+    dy = [torch.randn(40000, 520, device="cuda") for _ in range(2)]
+    alone = []
+    for k in range(2):
+        w, v = table.clone().requires_grad_(), scale.clone().requires_grad_()
+        outs = [embedding(ids[k], w), block_norm(x[k], x[k], v)[0]]
+        alone.append(torch.autograd.grad(outs, [w, v], [dy[k], dy[k]]))
+        del outs
+    main, streams = torch.cuda.current_stream(), [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        w, v = _bound(table, scale)
+        outs = []
+        for k, s in enumerate(streams):
+            s.wait_stream(main)
+            with torch.cuda.stream(s):
+                outs += [embedding(ids[k], w), block_norm(x[k], x[k], v)[0]]
+        for s in streams:
+            main.wait_stream(s)
+        slots = [w.grad, v.grad]
+        torch.autograd.backward(outs, [dy[0], dy[0], dy[1], dy[1]])
+        got = [w.grad.clone(), v.grad.clone()]  # (on the caller's stream)
+        assert w.grad is slots[0] and v.grad is slots[1]
+        for g, a, b in zip(got, *alone):  # one rounding of the sum, in one order or the other
+            assert float((g.double() - (a.double() + b.double())).abs().max()) <= 2.0 ** -23 * float((a.abs() + b.abs()).max())
+        del outs
+
+
+def test_bound_gradients_with_an_accumulator_of_another_stream():
+    """The leaf's accumulator was made on another stream than the pass runs on, and is alive."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    torch.manual_seed(1)
+    ids, dy = torch.randint(0, 6000, (40000,), device="cuda"), torch.randn(40000, 520, device="cuda")
+    (w,) = _bound(torch.randn(6000, 520, device="cuda"))
+    (expect,) = torch.autograd.grad(embedding(ids, w), w, dy)
+    keep = w.expand_as(w)  # (its graph holds the accumulator, made on the default stream)
+    main, side = torch.cuda.current_stream(), torch.cuda.Stream()
+    for k in range(3):
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            y = embedding(ids, w)
+        main.wait_stream(side)
+        y.backward(dy)
+        assert torch.equal(w.grad, (k + 1) * expect) or k == 2  # (1 and 2 times are exact)
+        del y
+    assert float((w.grad - 3 * expect).abs().max()) <= 2.0 ** -23 * float(w.grad.abs().max())
+    assert keep.requires_grad
+
+
+@pytest.mark.parametrize("side", [False, True])
+def test_bound_gradients_need_no_dense_one(side):
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    (w,) = _bound(torch.randn(50000, 520, device="cuda"))
+    w.register_post_accumulate_grad_hook(lambda t: None)
+    ids = torch.randint(0, 50000, (600,), device="cuda")
+    dy = torch.ones(600, 520, device="cuda")
+    stream = torch.cuda.Stream() if side else torch.cuda.current_stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        embedding(ids, w).backward(dy)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before < w.nbytes / 4
+    assert torch.equal(w.grad[:, 0], torch.bincount(ids, minlength=50000).float())
