@@ -230,3 +230,28 @@ def test_bound_gradients_need_no_dense_one(side):
     torch.cuda.synchronize()
     assert torch.cuda.max_memory_allocated() - before < w.nbytes / 4
     assert torch.equal(w.grad[:, 0], torch.bincount(ids, minlength=50000).float())
+
+
+@pytest.mark.parametrize("late", [False, True])
+def test_caller_waits_for_bound_gradients(late):
+    """The pass runs on another stream than the caller's, which is busy; the caller reads at once."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+    from smdistributed_modelparallel_amd.ops.layernorm import block_norm
+
+    torch.manual_seed(2)
+    w, v = _bound(torch.randn(3000, 136, device="cuda"), torch.randn(136, device="cuda"))
+    ids, x = torch.randint(0, 3000, (2000,), device="cuda"), torch.randn(2000, 136, device="cuda")
+    dy = torch.randn(2000, 136, device="cuda")
+    outs = [embedding(ids, w), block_norm(x, x, v)[0]]
+    expect = torch.autograd.grad(outs, [w, v], [dy, dy])
+    del outs
+    keep = [t.expand_as(t) for t in (w, v)] if late else None
+    main, side = torch.cuda.current_stream(), torch.cuda.Stream()
+    side.wait_stream(main)
+    with torch.cuda.stream(side):
+        outs = [embedding(ids, w), block_norm(x, x, v)[0]]
+        torch.cuda._sleep(100_000_000)
+    torch.autograd.backward(outs, [dy, dy])
+    got = [w.grad.clone(), v.grad.clone()]
+    assert all(torch.equal(a, b) for a, b in zip(got, expect))
+    assert keep is None or len(keep) == 2
