@@ -4,10 +4,12 @@
 
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <vector>
@@ -37,6 +39,23 @@ int dt_code(const at::Tensor& t, const char* name) {
 hipStream_t stream() { return at::hip::getCurrentHIPStream().stream(); }
 
 void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " launch failed with code ", rc); }
+
+// A tensor that is its memory and nothing else, as the kernels take it.  Not so: dual numbers, the
+// tensors of function transforms (vmap, torch.func) and of classes that dispatch operations themselves
+// (fake or distributed ones), lazily negated and zero tensors.
+bool plain(const at::Tensor& t) {
+  using Key = c10::DispatchKey;
+  static const c10::DispatchKeySet other({Key::Python, Key::Batched, Key::FuncTorchBatched, Key::FuncTorchGradWrapper,
+                                          Key::BatchedNestedTensor, Key::Functionalize, Key::Conjugate, Key::Negative,
+                                          Key::ZeroTensor});
+  return !t.key_set().has_any(other) && !t.is_nested() && !t._fw_grad(/*level=*/0).defined();
+}
+
+// No trace, mode or function transform is active, which would have to know of the launch.
+bool unobserved() {
+  return !torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::any_modes_set() &&
+         !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode);
+}
 
 // ------------------------------------------------------------------- embedding
 smpk::IndexList index_list(const c10::optional<at::Tensor>& ids, int64_t n, int64_t start, int64_t rows,
@@ -250,6 +269,17 @@ class EmbeddingGradFunction : public torch::autograd::Function<EmbeddingGradFunc
   }
 };
 
+// Both gradients by torch's operations, which see to duals, batches and graphs of a dy that is not plain:
+// added up in fp32 and rounded once.
+at::Tensor table_gradient(const at::Tensor& dy, const at::Tensor& ids, at::IntArrayRef shape, double scale, int64_t start,
+                          int64_t skip) {
+  const at::Tensor row = ids.to(at::kLong) - start;
+  const at::Tensor other = (row < 0).logical_or(row >= shape[0]).logical_or(row == (skip < 0 ? shape[0] : skip));
+  const at::Tensor sum = at::zeros(shape, ids.options().dtype(at::kFloat))
+                             .index_add(0, row.masked_fill(other, 0), dy.to(at::kFloat).masked_fill(other.unsqueeze(1), 0));
+  return (sum * scale).to(dy.scalar_type());
+}
+
 // Autograd's nodes are C++: a short call's time is the host's, and the backward needs no interpreter.
 class EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
  public:
@@ -274,6 +304,13 @@ class EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
     const at::Tensor p = two ? ctx->saved_data["pos_weight"].toTensor() : at::Tensor();
     check_capture({w, p}, "embedding");
     variable_list out(11);
+    if (!plain(grads[0])) {
+      const at::Tensor dy = grads[0].reshape({-1, w.size(1)});
+      const at::Tensor at = saved[1].defined() ? saved[1] : at::arange(dy.size(0), saved[0].options()).remainder(args[0]);
+      if (ctx->needs_input_grad(0)) out[0] = table_gradient(dy, saved[0], w.sizes(), scale, args[1], args[2]);
+      if (two && ctx->needs_input_grad(1)) out[1] = table_gradient(dy, at, p.sizes(), 1.0, 0, -1);
+      return out;
+    }
     const at::Tensor dy = grads[0].reshape({-1, w.size(1)}).contiguous();
     Opt dw, dp, pos;
     if (saved[1].defined()) pos = saved[1];
@@ -325,6 +362,15 @@ at::Tensor embedding(at::Tensor weight, Opt pos_weight, at::Tensor ids, Opt pos,
   if (!grad) return embedding_fwd(flat, weight, scale, start, foreign_zero, pos, pos_weight, period).view(shape);
   return EmbeddingFunction::apply(weight, pos_weight, flat, pos, period, scale, start, foreign_zero, skip, mark_w, mark_p)
       .view(shape);
+}
+
+// None where the kernels do not take the call: the caller has the same in torch's operations
+Opt embedding_call(at::Tensor weight, Opt pos_weight, at::Tensor ids, Opt pos, double scale, int64_t start,
+                   bool foreign_zero, int64_t skip, bool mark_w, bool mark_p) {
+  bool take = unobserved() && plain(weight) && plain(ids);
+  for (const Opt* t : {&pos_weight, &pos}) take = take && (!t->has_value() || plain(**t));
+  if (!take) return c10::nullopt;
+  return embedding(weight, pos_weight, ids, pos, scale, start, foreign_zero, skip, mark_w, mark_p);
 }
 
 // ------------------------------------------------------------------ block norm
@@ -517,6 +563,9 @@ class BlockNormFunction : public torch::autograd::Function<BlockNormFunction> {
     const Opt dy = opt(grads[0].defined() ? grads[0].contiguous() : grads[0]);
     const Opt ds = grads.size() > 1 ? opt(grads[1].defined() ? grads[1].contiguous() : grads[1]) : Opt();
     if (!dy.has_value() && !ds.has_value()) return result;
+    TORCH_CHECK((!dy.has_value() || plain(*dy)) && (!ds.has_value() || plain(*ds)),
+                "block_norm: the gradient of an output must be a plain tensor, not a dual, batched or otherwise wrapped "
+                "one (calls made inside a function transform or on dual numbers take such gradients)");
     const auto v = ctx->get_saved_variables();
     check_capture(v, "block_norm");
     const auto marks = ctx->saved_data["marks"].toIntVector();
@@ -543,10 +592,13 @@ class BlockNormFunction : public torch::autograd::Function<BlockNormFunction> {
 };
 
 // {y, s} (y alone without x), differentiable in all tensors; marks: which of w, b, pw, pb, gate are
-// parameters bound to the flat gradient buffer
-variable_list block_norm(Opt x, at::Tensor res, at::Tensor w, Opt b, Opt pw, Opt pb, Opt gate, int64_t gate_rows,
+// parameters bound to the flat gradient buffer.  None where the kernels do not take the call, as above.
+c10::optional<variable_list> block_norm(Opt x, at::Tensor res, at::Tensor w, Opt b, Opt pw, Opt pb, Opt gate, int64_t gate_rows,
                          double alpha, double eps, bool rms, std::vector<int64_t> marks) {
   TORCH_CHECK(marks.size() == 5, "block_norm: bad lists");
+  bool take = unobserved() && plain(res) && plain(w);
+  for (const Opt* t : {&x, &b, &pw, &pb, &gate}) take = take && (!t->has_value() || plain(**t));
+  if (!take) return c10::nullopt;
   auto dense = [](Opt& t) {
     if (t.has_value()) t = t->contiguous();
   };
@@ -696,7 +748,7 @@ void register_training_ops(py::module_& m) {
         py::arg("marks"));
   m.def("grad_norm", &grad_norm, py::arg("grads"), py::arg("inf"), py::arg("scale"), py::arg("out") = py::none(),
         py::arg("max_norm") = 0.0);
-  m.def("embedding", &embedding, py::arg("weight"), py::arg("pos_weight"), py::arg("ids"), py::arg("pos"),
+  m.def("embedding", &embedding_call, py::arg("weight"), py::arg("pos_weight"), py::arg("ids"), py::arg("pos"),
         py::arg("scale"), py::arg("start"), py::arg("foreign_zero"), py::arg("skip"), py::arg("mark_w"),
         py::arg("mark_p"));
 }

@@ -8,7 +8,9 @@ run -- and writes the parameters' flat-buffer gradients in place where they are 
 (autograd gets none for them; their post-accumulate hooks still fire).  A parameter with other hooks
 takes its gradient through autograd: they see it, and may change it, before it is added.
 A pass that builds a graph of its own (``create_graph``) can be differentiated again.
-CPU tensors use plain torch operations.  torch.autocast changes nothing: both tables and the
+CPU tensors use plain torch operations, and so do calls whose launch would go unnoticed: on dual
+numbers (forward-mode derivatives), inside function transforms (``torch.vmap``, ``torch.func``), under
+``torch.jit.trace`` or a dispatch mode, and of tensor classes that dispatch operations themselves.  torch.autocast changes nothing: both tables and the
 result are of one type.
 """
 import math
@@ -19,23 +21,33 @@ from ..backend.exceptions import SMPInvalidArgumentError
 from ._ext import ext
 
 
-def _embedding_torch(ids, weight, padding_idx, scale, vocab_start, position_ids, position_weight):
-    rows = weight.shape[0]
-    if vocab_start is None:
-        y = torch.nn.functional.embedding(ids, weight, padding_idx)
+def _rows_torch(ids, table, padding_idx, fill):
+    """Rows of a table; `fill` where an id is none of its rows."""
+    rows = table.shape[0]
+    outside = (ids < 0) | (ids >= rows)
+    if padding_idx is not None and not 0 <= padding_idx < rows:
+        padding_idx = None
+    return torch.nn.functional.embedding(ids.clamp(0, rows - 1), table, padding_idx).masked_fill(outside.unsqueeze(-1), fill)
+
+
+def _embedding_torch(ids, weight, padding_idx, scale, vocab_start, position_ids, position_weight, nan_outside=False):
+    """In torch's operations.  nan_outside: ids outside a whole table give NaN, as by the kernels,
+    instead of torch's own error."""
+    if vocab_start is not None:
+        pad = None if padding_idx is None else padding_idx - vocab_start
+        y = _rows_torch(ids - vocab_start, weight, pad, 0.0)
+    elif nan_outside:
+        y = _rows_torch(ids, weight, padding_idx, math.nan)
     else:
-        local = ids - vocab_start
-        outside = (local < 0) | (local >= rows)
-        pad = None
-        if padding_idx is not None and vocab_start <= padding_idx < vocab_start + rows:
-            pad = padding_idx - vocab_start
-        y = torch.nn.functional.embedding(local.clamp(0, rows - 1), weight, pad)
-        y = y.masked_fill(outside.unsqueeze(-1), 0.0)
+        y = torch.nn.functional.embedding(ids, weight, padding_idx)
     if position_weight is None:
         return y if scale == 1.0 else (y.float() * scale).to(weight.dtype)
     if position_ids is None:
         position_ids = torch.arange(ids.shape[-1], device=ids.device).expand(ids.shape)
-    p = torch.nn.functional.embedding(position_ids, position_weight)
+    if nan_outside:
+        p = _rows_torch(position_ids, position_weight, None, math.nan)
+    else:
+        p = torch.nn.functional.embedding(position_ids, position_weight)
     return (y.float() * scale + p.float()).to(weight.dtype)
 
 
@@ -101,11 +113,13 @@ def embedding(ids, weight, padding_idx=None, scale=1.0, vocab_start=None, positi
                                           f"{position_weight.shape[0]} rows")
     if weight.is_cuda:
         start = vocab_start or 0
-        return ext().embedding(weight, position_weight, ids, position_ids, scale, start, vocab_start is not None,
-                               -1 if padding_idx is None else padding_idx - start,
-                               getattr(weight, "_smp_fused_grad", False),
-                               getattr(position_weight, "_smp_fused_grad", False))
-    return _embedding_torch(ids, weight, padding_idx, scale, vocab_start, position_ids, position_weight)
+        y = ext().embedding(weight, position_weight, ids, position_ids, scale, start, vocab_start is not None,
+                            -1 if padding_idx is None else padding_idx - start,
+                            getattr(weight, "_smp_fused_grad", False),
+                            getattr(position_weight, "_smp_fused_grad", False))
+        if y is not None:
+            return y
+    return _embedding_torch(ids, weight, padding_idx, scale, vocab_start, position_ids, position_weight, weight.is_cuda)
 
 
 def lookup(ids, weight, padding_idx=None, vocab_start=None):

@@ -180,7 +180,9 @@ MAX_BLOCK_NORM_ROWS = 1 << 30
 
 def _block_norm_hip(x, residual, weight, bias, post_weight, post_bias, gate, gate_rows, alpha, eps, rms):
     """[y, s] by the kernels (x None: [y], the norm of residual); parameters bound to the flat
-    gradient buffer take their gradients there in place, unless they have hooks that want them."""
+    gradient buffer take their gradients there in place, unless they have hooks that want them.
+    None where the kernels do not take the call: dual numbers, function transforms, traces, dispatch
+    modes, tensor classes that dispatch operations themselves."""
     marks = [int(getattr(t, "_smp_fused_grad", False)) for t in (weight, bias, post_weight, post_bias, gate)]
     return ext().block_norm(x, residual, weight, bias, post_weight, post_bias, gate, gate_rows, alpha, eps, rms, marks)
 
@@ -209,6 +211,12 @@ def _norm_torch(v, weight, bias, eps, rms):
         v = v - v.mean(-1, keepdim=True)
     v = v * torch.rsqrt((v * v).mean(-1, keepdim=True) + eps) * weight.float()
     return v if bias is None else v + bias.float()
+
+
+def _block_norm_torch(x, residual, weight, bias, post_weight, post_bias, gate, alpha, eps, rms):
+    h = x.float() if post_weight is None else _norm_torch(x.float(), post_weight, post_bias, eps, rms)
+    s = residual.float() + alpha * (h if gate is None else gate.float() * h)
+    return _norm_torch(s, weight, bias, eps, rms).to(x.dtype), s.to(x.dtype)
 
 
 def _check_norm(name, rows, weight, bias, dtype):
@@ -264,15 +272,13 @@ def block_norm(x, residual, weight, bias=None, post_weight=None, post_bias=None,
         lead = x.dim() - gate.dim()
         if lead < 0 or any(n not in (1, m) for n, m in zip(gate.shape, x.shape[lead:])):
             raise SMPInvalidArgumentError(f"gate {tuple(gate.shape)} does not broadcast to {tuple(x.shape)}")
-    if not x.is_cuda:
-        h = x.float() if post_weight is None else _norm_torch(x.float(), post_weight, post_bias, eps, rms)
-        s = residual.float() + residual_scale * (h if gate is None else gate.float() * h)
-        return _norm_torch(s, weight, bias, eps, rms).to(x.dtype), s.to(x.dtype)
-    run = 1
-    if gate is not None:
-        gate, run = _gate_matrix(gate if gate.dim() else gate.reshape(1), x.shape)
-    y, s = _block_norm_hip(x, residual, weight, bias, post_weight, post_bias, gate, run, residual_scale, eps, bool(rms))
-    return y, s
+    out = None
+    if x.is_cuda:
+        rows, run = (gate, 1) if gate is None else _gate_matrix(gate if gate.dim() else gate.reshape(1), x.shape)
+        out = _block_norm_hip(x, residual, weight, bias, post_weight, post_bias, rows, run, residual_scale, eps, bool(rms))
+    if out is None:
+        out = _block_norm_torch(x, residual, weight, bias, post_weight, post_bias, gate, residual_scale, eps, rms)
+    return tuple(out)
 
 
 def rms_norm(x, weight, eps=1e-5):
@@ -283,6 +289,5 @@ def rms_norm(x, weight, eps=1e-5):
     eps = float(eps)
     if not (math.isfinite(eps) and eps >= 0.0):
         raise SMPInvalidArgumentError(f"bad eps {eps}")
-    if not x.is_cuda:
-        return _norm_torch(x.float(), weight, None, eps, True).to(x.dtype)
-    return _block_norm_hip(None, x, weight, None, None, None, None, 1, 1.0, eps, True)[0]
+    out = _block_norm_hip(None, x, weight, None, None, None, None, 1, 1.0, eps, True) if x.is_cuda else None
+    return _norm_torch(x.float(), weight, None, eps, True).to(x.dtype) if out is None else out[0]
