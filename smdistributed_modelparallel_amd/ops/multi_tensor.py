@@ -306,6 +306,15 @@ def grad_power(tensors, norm_type=2.0, scale=1.0):
 
 
 @torch.no_grad()
+def flat_power(ranges, norm_type=2.0, scale=1.0):
+    """``grad_power`` of an optimizer's flat gradients: on the CPU of any floating type."""
+    if not ranges or _on_gpu(ranges):
+        return grad_power(ranges, norm_type, scale)
+    ranges, inf, scale = _norm_args(ranges, norm_type, scale)
+    return _grad_power_cpu(ranges, inf, scale)
+
+
+@torch.no_grad()
 def grad_norm(tensors, norm_type=2.0, scale=1.0):
     """L2 (or, ``norm_type=inf``, largest-value) norm of all elements of a list of tensors, times
     ``scale``: a fp32 scalar tensor, the same bits on every run, no host synchronisation.  The

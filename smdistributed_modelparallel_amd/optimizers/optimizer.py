@@ -307,7 +307,7 @@ class DistributedOptimizer(torch.optim.Optimizer):
         once = core.tp_size() > 1 and core.tp_rank() != 0 and not state.cfg.shard_optimizer_state
         ranges = [self._grad_range(d) for d in self.domains if not (once and d.key == "default")]
         # fp64 over the ranks too: no finite gradient overflows the sum of squares
-        acc = mt.grad_power(ranges, norm_type, scale=1.0 / self.loss_scale).to(dev)
+        acc = mt.flat_power(ranges, norm_type, scale=1.0 / self.loss_scale).to(dev)
         total, op = acc, dist.ReduceOp.SUM
         if norm_type != 2:  # as whole numbers, in the same order: a maximum of floats may lose a rank's NaN
             total, op = acc.abs().view(torch.int64), dist.ReduceOp.MAX

@@ -98,3 +98,9 @@ def test_clip_master_grads_by_largest_value_over_stages():
     from tests.dist_utils import run_workers
 
     assert all("OK clip" in o for o in run_workers("clip_inf", 2, timeout=120))
+
+
+def test_clip_master_grads_of_a_model_in_64_bits():
+    from tests.dist_utils import run_workers
+
+    assert all("OK clip" in o for o in run_workers("clip_fp64", 2, timeout=120))
