@@ -250,10 +250,12 @@ def block_norm(x, residual, weight, bias=None, post_weight=None, post_bias=None,
     [dim] have their dtype or are fp32.  ``gate`` (that dtype or fp32) broadcasts to ``x``: one
     vector, one for each sample ([batch, 1, dim]), or one value for each element; None is 1.
     All arithmetic is fp32, and the second norm is taken of ``s`` before it is rounded.  Under
-    torch.autocast, where a block's output and the residual differ in type, the residual's holds."""
+    torch.autocast, where a block's output and the residual differ in type, the residual's holds for
+    the output and for a 16-bit gate; a fp32 gate stays."""
     if torch.is_tensor(x) and torch.is_tensor(residual) and torch.is_autocast_enabled(x.device.type):
         x = x.to(residual.dtype)
-        gate = gate.to(residual.dtype) if torch.is_tensor(gate) else gate
+        if torch.is_tensor(gate) and gate.dtype != torch.float32:  # (fp32 gates go with rows of any type)
+            gate = gate.to(residual.dtype)
     _check_rows(x, "x")
     if not torch.is_tensor(residual) or residual.shape != x.shape or residual.dtype != x.dtype \
             or residual.device != x.device:

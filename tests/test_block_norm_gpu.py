@@ -366,3 +366,23 @@ def test_hooks_of_bound_parameters_get_their_gradients():
     torch.autograd.backward(call(u, 0.5, 1e-5, False), [dy, ds])
     for k in names:
         assert torch.equal(seen[k], expect[k]) and torch.equal(u[k].grad, 3 * expect[k]), k
+
+
+@pytest.mark.parametrize("device", ["cpu", "cuda"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_autocast_keeps_a_fp32_gate(device, dtype):
+    """Beside 16-bit rows the gate and its gradient have the same bits with and without autocast."""
+    from smdistributed_modelparallel_amd.ops.layernorm import block_norm
+
+    g = torch.Generator().manual_seed(4)
+    x, r = (torch.randn(4, 3, 48, generator=g).to(device, dtype) for _ in range(2))
+    w, dy, ds = torch.randn(48, generator=g).to(device), *(torch.randn(4, 3, 48, generator=g).to(device, dtype) for _ in range(2))
+    for shape in ((48,), (4, 1, 48), (4, 3, 48)):
+        gate = torch.randn(shape, generator=g).to(device).requires_grad_()
+        plain = block_norm(x, r, w, gate=gate)
+        plain += torch.autograd.grad(plain, gate, [dy, ds])
+        with torch.autocast(device, dtype=torch.bfloat16):
+            cast = block_norm(x, r, w, gate=gate)
+        cast += torch.autograd.grad(cast, gate, [dy, ds])
+        assert cast[2].dtype == torch.float32
+        assert all(torch.equal(a, b) for a, b in zip(plain, cast))
