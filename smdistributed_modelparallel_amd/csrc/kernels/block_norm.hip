@@ -146,6 +146,7 @@ __global__ void __launch_bounds__(1024) block_norm_fwd(BlockNormArgs a, int thre
   int64_t row = blockIdx.x;
   if (SUB != 0) row = row * (blockDim.x / team_size) + tid / team_size;
   if (SUB == 0 && team_size == 64) row = row * (blockDim.x >> 6) + __builtin_amdgcn_readfirstlane(tid >> 6);
+  row += a.first_row;
   if (row >= a.rows) return;  // (all lanes of their own rows: no barrier or sum follows for them)
   int col[V], left[V];
   float s[V][kCols], h[V][kCols];
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(1024) block_norm_bwd_rows(BlockNormArgs a) {
   __shared__ float smem[64];
   const int team_size = blockDim.x, lane = threadIdx.x;
   Team<0> team{smem, 0, team_size / 64, 0};
-  const int64_t row = blockIdx.x, gate_row = a.gate != nullptr ? row / a.gate_rows * a.d : 0;
+  const int64_t row = a.first_row + blockIdx.x, gate_row = a.gate != nullptr ? row / a.gate_rows * a.d : 0;
   const float4 st = reinterpret_cast<const float4*>(a.stats)[row];
   RowData<T> r[V];  // all loads first
   float n1[V][kCols], n2[V][kCols], dy[V][kCols], ds[V][kCols];
@@ -634,6 +635,17 @@ constexpr int64_t kMaxSummed = 6144;
 // Threads of a row of up to 32 vectors: lanes of one wave, which takes several rows then.
 int sub_of(int64_t vectors) { return vectors <= 8 ? 8 : vectors <= 16 ? 16 : vectors <= 32 ? 32 : 0; }
 
+// Rows in launches of at most 2^28 threads: a grid has to stay below 2^32, and a launch of that size
+// takes 100 us or more.  launch(arguments, blocks)
+template <typename F>
+void in_parts(BlockNormArgs a, int64_t rows_of_block, int64_t threads, const F& launch) {
+  const int64_t most = (1ll << 28) / threads;
+  for (; a.first_row < a.rows; a.first_row += most * rows_of_block) {
+    const int64_t blocks = (a.rows - a.first_row + rows_of_block - 1) / rows_of_block;
+    launch(a, static_cast<unsigned>(blocks < most ? blocks : most));
+  }
+}
+
 }  // namespace
 
 int block_norm_fwd(int dt, const BlockNormArgs& a, hipStream_t s) {
@@ -644,8 +656,7 @@ int block_norm_fwd(int dt, const BlockNormArgs& a, hipStream_t s) {
   const int sub = sub_of(vectors);
   const int v = vectors <= 64 ? 1 : vectors <= 128 ? 2 : wave ? 4 : vectors <= 1024 ? 1 : 2;
   const int team = sub ? sub : wave ? 64 : static_cast<int>(((vectors + v - 1) / v + 63) / 64 * 64);
-  const int64_t rows_of_block = wave ? 256 / team : 1, blocks = (a.rows + rows_of_block - 1) / rows_of_block;
-  if (blocks > 0x7fffffff) return -3;
+  const int threads = wave ? 256 : team;
   SMPK_DISPATCH(dt, T, {
     const bool whole = a.d % kCols == 0;
     const auto kernel =
@@ -656,7 +667,8 @@ int block_norm_fwd(int dt, const BlockNormArgs& a, hipStream_t s) {
         : v == 1    ? (whole ? block_norm_fwd<T, 1, kWhole, 0> : block_norm_fwd<T, 1, kOverlap, 0>)
         : v == 2    ? (whole ? block_norm_fwd<T, 2, kWhole, 0> : block_norm_fwd<T, 2, kOverlap, 0>)
                     : (whole ? block_norm_fwd<T, 4, kWhole, 0> : block_norm_fwd<T, 4, kOverlap, 0>);
-    kernel<<<static_cast<unsigned>(blocks), wave ? 256 : team, 0, s>>>(a, team);
+    in_parts(a, wave ? 256 / team : 1, threads,
+             [&](const BlockNormArgs& part, unsigned blocks) { kernel<<<blocks, threads, 0, s>>>(part, team); });
   });
   return static_cast<int>(hipGetLastError());
 }
@@ -692,7 +704,8 @@ void launch_bwd(const BlockNormArgs& a, const BlockNormPlan& p, hipStream_t s) {
     const int64_t vectors = (a.d + kCols - 1) / kCols;
     const int v = vectors <= 1024 ? 1 : 2;
     const auto kernel = v == 1 ? block_norm_bwd_rows<T, 1, R> : block_norm_bwd_rows<T, 2, R>;
-    kernel<<<static_cast<unsigned>(a.rows), static_cast<unsigned>(((vectors + v - 1) / v + 63) / 64 * 64), 0, s>>>(a);
+    const unsigned threads = static_cast<unsigned>(((vectors + v - 1) / v + 63) / 64 * 64);
+    in_parts(a, 1, threads, [&](const BlockNormArgs& part, unsigned blocks) { kernel<<<blocks, threads, 0, s>>>(part); });
     bool sums = a.gate_direct || a.gate_part != nullptr;
     for (float* q : a.part) sums = sums || q != nullptr;
     if (!sums) return;

@@ -311,6 +311,7 @@ struct BlockNormArgs {
   const void *x = nullptr, *res = nullptr, *w = nullptr, *b = nullptr, *pw = nullptr, *pb = nullptr, *gate = nullptr;
   int w_f32 = 0, gate_f32 = 0, rms = 0;
   int64_t rows = 0, gate_rows = 1, groups = 0;  // groups: rows / gate_rows
+  int64_t first_row = 0;  // of a launch that takes some of the rows
   int d = 0;
   float alpha = 1.f, eps = 0.f;
   float* stats = nullptr;  // [rows][4]: mean, 1 / deviation of s, then of x

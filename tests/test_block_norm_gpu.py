@@ -386,3 +386,25 @@ def test_autocast_keeps_a_fp32_gate(device, dtype):
         cast += torch.autograd.grad(cast, gate, [dy, ds])
         assert cast[2].dtype == torch.float32
         assert all(torch.equal(a, b) for a, b in zip(plain, cast))
+
+
+@pytest.mark.parametrize("rows,d", [((1 << 29) + 11, 1), ((1 << 25) + 5, 66), (700_000, 6145)])
+def test_more_rows_than_one_launch_takes(rows, d):
+    """A row's results have the same bits whatever rows the call has beside it."""
+    from smdistributed_modelparallel_amd.ops.layernorm import block_norm
+
+    g = torch.Generator(device="cuda").manual_seed(5)
+    w, pw = (torch.rand(d, generator=g, device="cuda") + 0.5 for _ in range(2))
+    x = torch.empty(rows, d, device="cuda", dtype=torch.float16).normal_(generator=g)
+    threads = 8 if d == 1 else 16 if d == 66 else 832
+    most = (1 << 28) // threads  # rows of a launch
+    places = sorted({0, rows - 40, *(k * most - 20 for k in range(1, rows // most + 1))})
+    assert len(places) > 2
+    x.requires_grad_()
+    y, s = block_norm(x, x, w, post_weight=pw, rms=True)
+    (dx,) = torch.autograd.grad(y, x, y.detach())
+    for at in places:
+        part = x.detach()[at:at + 40].clone().requires_grad_()
+        py, ps = block_norm(part, part, w, post_weight=pw, rms=True)
+        assert torch.equal(y[at:at + 40], py) and torch.equal(s[at:at + 40], ps)
+        assert torch.equal(dx[at:at + 40], torch.autograd.grad(py, part, py.detach())[0])
