@@ -18,6 +18,7 @@ namespace smpk {
 namespace {
 
 constexpr int kT = 256;
+constexpr int64_t kMostBlocks = (1ll << 32) / kT;  // a grid's threads stay below 2^32
 // Longest list that is ordered in one launch: 8192 ids of a vocabulary of 12608 take 14 us so, and
 // 19 us in one block's registers; 65536 ids of 50257 take 80 us, and 28 us in radix passes.
 constexpr int64_t kRangeTokens = 16384;
@@ -391,7 +392,7 @@ __device__ __forceinline__ void write_row(T* p, int left, float (&sum)[kCols], f
 }
 
 // What a launch has to do for one table: blocks [first, first + blocks) add up its tokens, then
-// [clear, clear + clears) clear rows.
+// [clear, clear + clears) clear rows, `windows` of them in all.
 struct Work {
   Sorted l;
   void* dw;
@@ -399,7 +400,7 @@ struct Work {
   const uint8_t* marks;
   float scale;
   int accumulate, chunk;
-  int64_t first, blocks, clear, clears;
+  int64_t first, blocks, clear, clears, windows;
   int stream;  // zeros past the caches
 };
 
@@ -439,22 +440,25 @@ __device__ __forceinline__ void zero_rows(uint64_t rows, T* at, int64_t left, in
   }
 }
 
-// A dense gradient: 16 rows x 512 columns a block, of which the rows without a token are cleared
-// (marks null: the rows from `period` on).
+// A dense gradient: windows of 16 rows x 512 columns, of which the rows without a token are cleared
+// (marks null: the rows from `period` on).  One window a block in tables of up to kClears of them.
+constexpr int64_t kClears = 1 << 21;
 template <bool FULL, typename T>
 __device__ __forceinline__ void clear_rows(const Work& wk, int64_t block, int slabs, T* dw, int d) {
   const Sorted& l = wk.l;
   const int lane = threadIdx.x & 63;
-  const int64_t window = block / slabs, r0 = window * kZeroRows, mine = r0 + lane;
-  const int c = static_cast<int>(block - window * slabs) * 64 * kCols;
-  const bool empty = lane < kZeroRows && mine < l.rows &&
-                     (l.n == 0 || (wk.marks != nullptr ? wk.marks[mine] == 0 : mine >= l.period));
-  const uint64_t rows = __ballot(empty);  // the same in all waves
-  T* const at = dw + r0 * d + c;
-  if (wk.stream) {  // (two loops: the compiler would make one store of two that differ in this alone)
-    zero_rows<FULL, true>(rows, at, d - c, d);
-  } else {
-    zero_rows<FULL, false>(rows, at, d - c, d);
+  for (; block < wk.windows; block += wk.clears) {
+    const int64_t window = block / slabs, r0 = window * kZeroRows, mine = r0 + lane;
+    const int c = static_cast<int>(block - window * slabs) * 64 * kCols;
+    const bool empty = lane < kZeroRows && mine < l.rows &&
+                       (l.n == 0 || (wk.marks != nullptr ? wk.marks[mine] == 0 : mine >= l.period));
+    const uint64_t rows = __ballot(empty);  // the same in all waves
+    T* const at = dw + r0 * d + c;
+    if (wk.stream) {  // (two loops: the compiler would make one store of two that differ in this alone)
+      zero_rows<FULL, true>(rows, at, d - c, d);
+    } else {
+      zero_rows<FULL, false>(rows, at, d - c, d);
+    }
   }
 }
 
@@ -813,7 +817,7 @@ int embedding_fwd(int dt, const IndexList& ids, const void* w, int64_t w_stride,
   if (n <= 0 || d <= 0) return 0;
   const int64_t per_row = (d + kCols - 1) / kCols;
   const int64_t blocks = (n * per_row + kT * kPerThread - 1) / (kT * kPerThread);
-  if (blocks > 0x7fffffff || n > 0x7fffffff - kT * kPerThread) return -3;
+  if (blocks >= kMostBlocks || n > 0x7fffffff - kT * kPerThread) return -3;
   const uint32_t reciprocal = per_row == 1 ? 0xffffffffu : static_cast<uint32_t>((1ull << 32) / per_row);
   uint32_t slice = 0;
   if (p != nullptr && pos.ids == nullptr)
@@ -944,7 +948,8 @@ int embedding_bwd(int dt, const void* dy, int64_t n, int64_t d, const EmbeddingG
   }
   for (int i = 0; i < count; ++i) {
     w[i].clear = grid;
-    w[i].clears = tables[i].accumulate ? 0 : (w[i].l.rows + kZeroRows - 1) / kZeroRows * slabs;
+    w[i].windows = tables[i].accumulate ? 0 : (w[i].l.rows + kZeroRows - 1) / kZeroRows * slabs;
+    w[i].clears = w[i].windows < kClears ? w[i].windows : kClears;
     grid += w[i].clears;
   }
   if (count == 1) {
@@ -952,7 +957,7 @@ int embedding_bwd(int dt, const void* dy, int64_t n, int64_t d, const EmbeddingG
     w[1].first = w[1].clear = grid;
     w[1].blocks = 0;
   }
-  if (grid > 0x7fffffff || join_slabs > 65535) return -3;
+  if (grid >= kMostBlocks || join_slabs > 65535) return -3;
   if (grid == 0) return 0;
   SMPK_DISPATCH(dt, T, {
     if (wide) {

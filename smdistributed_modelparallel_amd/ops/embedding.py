@@ -53,7 +53,13 @@ def _embedding_torch(ids, weight, padding_idx, scale, vocab_start, position_ids,
 
 MAX_TOKENS = 1 << 27
 MAX_ROWS = (1 << 31) - 1
+MAX_COLUMNS = 1 << 24
+MAX_VECTORS = ((1 << 24) - 1) * 1024  # of 8 elements, in the output: what one launch writes
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _sizes_ok(ids, weight):
+    return ids.numel() <= MAX_TOKENS and ids.numel() * ((weight.shape[1] + 7) // 8) <= MAX_VECTORS
 
 
 def _check_ids(name, t, device):
@@ -75,11 +81,12 @@ def embedding(ids, weight, padding_idx=None, scale=1.0, vocab_start=None, positi
     (broadcast to ``ids``) or, without them, by the place in the last dimension."""
     if not torch.is_tensor(weight) or weight.dim() != 2 or weight.dtype not in _FLOATS or 0 in weight.shape:
         raise SMPInvalidArgumentError("weight must be a [rows, dim] fp32 / fp16 / bf16 tensor")
-    if max(weight.shape) >= MAX_ROWS:
-        raise SMPInvalidArgumentError(f"tables of fewer than {MAX_ROWS} rows and columns are supported")
+    if weight.shape[0] >= MAX_ROWS or weight.shape[1] > MAX_COLUMNS:
+        raise SMPInvalidArgumentError(f"tables of fewer than {MAX_ROWS} rows, of at most {MAX_COLUMNS} columns, are supported")
     _check_ids("ids", ids, weight.device)
-    if ids.numel() > MAX_TOKENS:
-        raise SMPInvalidArgumentError(f"{ids.numel()} tokens in one call: at most {MAX_TOKENS} are supported")
+    if not _sizes_ok(ids, weight):
+        raise SMPInvalidArgumentError(f"{ids.numel()} tokens of {weight.shape[1]} in one call: at most {MAX_TOKENS} tokens and "
+                                      f"{8 * MAX_VECTORS} elements are supported")
     rows = weight.shape[0]
     scale = float(scale)
     if not math.isfinite(scale):
@@ -125,6 +132,7 @@ def embedding(ids, weight, padding_idx=None, scale=1.0, vocab_start=None, positi
 def lookup(ids, weight, padding_idx=None, vocab_start=None):
     """``embedding`` without scale and positions, for modules: tables of other types (fp64), empty
     shards, and tables or lists beyond the kernels' sizes go through plain torch operations."""
-    if weight.dtype in _FLOATS and 0 not in weight.shape and ids.numel() <= MAX_TOKENS and weight.shape[0] < MAX_ROWS:
+    if weight.dtype in _FLOATS and 0 not in weight.shape and weight.shape[0] < MAX_ROWS \
+            and weight.shape[1] <= MAX_COLUMNS and _sizes_ok(ids, weight):
         return embedding(ids, weight, padding_idx, vocab_start=vocab_start)
     return _embedding_torch(ids, weight, padding_idx, 1.0, vocab_start, None, None)

@@ -89,3 +89,11 @@ _I = torch.zeros(2, 3, dtype=torch.long)
 def test_refusals(args, kwargs):
     with pytest.raises(SMPInvalidArgumentError):
         embedding(*args, **kwargs)
+
+
+@pytest.mark.parametrize("n,rows,dim", [(1, 2, (1 << 24) + 1), (1, (1 << 31) - 1, 1), ((1 << 27) + 1, 2, 1), (1 << 27, 2, 1024),
+                                        (16384, 2, 8388608)])
+def test_sizes_beyond_a_launch_are_refused(n, rows, dim):
+    """Expanded tensors: one element of memory each."""
+    with pytest.raises(SMPInvalidArgumentError):
+        embedding(torch.zeros(1, dtype=torch.long).expand(n), torch.zeros(1, 1).expand(rows, dim))

@@ -479,3 +479,33 @@ def test_hooks_of_a_bound_table_get_its_gradient(of):
     handle.remove()
     embedding(ids, w, scale=2.0, position_weight=p).backward(dy)
     assert len(seen) == 1 and w.grad is slots[0]
+
+
+@pytest.mark.parametrize("n", [0, 900])
+@pytest.mark.parametrize("rows,dim", [((1 << 25) + 37, 8), ((1 << 28) + 100, 1), ((1 << 25) + 4, 33), (40_000, 600_000)])
+def test_gradients_of_very_large_tables(rows, dim, n):
+    """More rows to clear than one launch has blocks for."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    w = torch.ones(rows, dim, device="cuda", dtype=torch.float16).requires_grad_()
+    ids = torch.randint(0, rows, (n,), device="cuda")
+    ids[:2], ids[2:3] = rows - 1, 0
+    y = embedding(ids, w)
+    assert y.eq(1).all()
+    (dw,) = torch.autograd.grad(y, w, y.detach())
+    assert torch.equal(dw[:, 0], torch.bincount(ids, minlength=rows).half())
+    filled = sum(int(part.count_nonzero()) for part in dw.split(max((1 << 28) // dim, 1)))
+    assert torch.equal(dw[:, 0], dw[:, -1]) and filled == ids.unique().numel() * dim
+
+
+def test_most_tokens():
+    """The longest list: the radix sort of 2^27 tokens."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    n, rows = 1 << 27, 30000
+    w = torch.randn(rows, 1, device="cuda").requires_grad_()
+    ids = torch.randint(0, rows, (n,), device="cuda", dtype=torch.int32)
+    y = embedding(ids, w)
+    assert torch.equal(y[:, 0], w.detach()[:, 0][ids.long()])
+    (dw,) = torch.autograd.grad(y, w, torch.ones_like(y))
+    assert torch.equal(dw[:, 0], torch.bincount(ids, minlength=rows).float())
