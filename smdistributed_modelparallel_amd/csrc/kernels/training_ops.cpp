@@ -77,8 +77,11 @@ void check_table_dims(const at::Tensor& w) {
   TORCH_CHECK(w.is_cuda() && w.dim() == 2, "embedding: a table must be a GPU matrix");
 }
 
+// Elements of a row one after the other (of one element: whatever its stride says).
+bool rows_dense(const at::Tensor& w) { return w.stride(1) == 1 || w.size(1) == 1; }
+
 void check_table(const at::Tensor& w) {
-  TORCH_CHECK(w.is_cuda() && w.dim() == 2 && w.stride(1) == 1 && w.size(1) < (1ll << 31), "embedding: bad table");
+  TORCH_CHECK(w.is_cuda() && w.dim() == 2 && rows_dense(w) && w.size(1) < (1ll << 31), "embedding: bad table");
 }
 
 // n tokens: ids (or, for the positions, none: t % period) into w [rows, d], rows dense along d
@@ -346,16 +349,16 @@ class EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
 at::Tensor embedding(at::Tensor weight, Opt pos_weight, at::Tensor ids, Opt pos, double scale, int64_t start,
                      bool foreign_zero, int64_t skip, bool mark_w, bool mark_p) {
   check_table_dims(weight);
-  auto rows_dense = [](const at::Tensor& t) { return t.stride(1) == 1 ? t : t.contiguous(); };
+  auto dense = [](const at::Tensor& t) { return rows_dense(t) ? t : t.contiguous(); };
   auto shape = ids.sizes().vec();
   shape.push_back(weight.size(1));
   const int64_t period = pos_weight.has_value() && !pos.has_value() ? std::max<int64_t>(ids.size(-1), 1) : 1;
   const at::Tensor flat = ids.reshape({-1}).contiguous();
   if (pos.has_value()) pos = pos->reshape({-1}).contiguous();
-  weight = rows_dense(weight);
+  weight = dense(weight);
   if (pos_weight.has_value()) {
     check_table_dims(*pos_weight);
-    pos_weight = rows_dense(*pos_weight);
+    pos_weight = dense(*pos_weight);
   }
   const bool grad = at::GradMode::is_enabled() &&
                     (weight.requires_grad() || (pos_weight.has_value() && pos_weight->requires_grad()));

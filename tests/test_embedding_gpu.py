@@ -509,3 +509,21 @@ def test_most_tokens():
     assert torch.equal(y[:, 0], w.detach()[:, 0][ids.long()])
     (dw,) = torch.autograd.grad(y, w, torch.ones_like(y))
     assert torch.equal(dw[:, 0], torch.bincount(ids, minlength=rows).float())
+
+
+def test_tables_of_one_column():
+    """Their last stride may be anything; so may the first one of tables of one row."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+
+    ids = torch.tensor([3, 0, 3, 9], device="cuda")
+    base = torch.randn(10, 10, device="cuda")
+    for w in (torch.randn(1, 10, device="cuda").t(), base[2:3].t(), base[:, 2:3], base[:1, :1].expand(10, 1)):
+        for p in (None, torch.randn(1, 4, device="cuda").t()):
+            w = w.detach().requires_grad_()
+            y = embedding(ids, w, position_weight=p)
+            assert torch.equal(y, w.detach()[ids] + (0.0 if p is None else p))
+            (dw,) = torch.autograd.grad(y, w, torch.ones_like(y))
+            assert dw[:, 0].tolist() == [1, 0, 0, 2, 0, 0, 0, 0, 0, 1]
+    row = base[:, 4:5].t()
+    y = embedding(torch.zeros(3, dtype=torch.long, device="cuda"), row)
+    assert torch.equal(y, row.expand(3, 10))
