@@ -671,12 +671,13 @@ std::vector<at::Tensor> grad_norm(std::vector<at::Tensor> grads, bool inf, doubl
   }
   for (size_t i = 0; i < grads.size(); ++i) {
     at::Tensor& t = grads[i];
-    TORCH_CHECK_VALUE(t.defined() && t.layout() == at::kStrided && is_float(t), "tensor ", i, " is none of them");
+    TORCH_CHECK_VALUE(t.defined() && t.layout() == at::kStrided && is_float(t) && plain(t), "tensor ", i,
+                      " is none of them (or no plain tensor)");
     TORCH_CHECK_VALUE(t.device() == device, "tensor ", i, " is on ", t.device(), ", not on ", device);
     total += t.numel();
     if (out.has_value()) {
       at::Tensor& o = dest[i];
-      TORCH_CHECK_VALUE(o.defined() && o.layout() == at::kStrided && is_float(o) && o.device() == device &&
+      TORCH_CHECK_VALUE(o.defined() && o.layout() == at::kStrided && is_float(o) && plain(o) && o.device() == device &&
                             o.sizes() == t.sizes(),
                         "output ", i, " differs from its gradient in shape or device, or is none of them");
       for (int64_t k = 0; k < o.dim(); ++k)

@@ -249,7 +249,7 @@ def _grad_norm_hip(tensors, inf, scale, out=None, max_norm=0.0):
     try:
         return ext().grad_norm(tensors, inf, scale, out, max_norm)
     except (TypeError, ValueError) as e:
-        raise SMPInvalidArgumentError(f"gradients must be strided fp32 / fp16 / bf16 tensors of one device: {e}") from None
+        raise SMPInvalidArgumentError(f"gradients must be plain strided fp32 / fp16 / bf16 tensors of one device: {e}") from None
 
 
 def _on_gpu(tensors):

@@ -200,3 +200,26 @@ def test_block_norm_refuses_gradients_that_are_no_plain_tensors():
     with pytest.raises(RuntimeError, match="plain tensor"):
         torch.autograd.grad(y, x, dy.expand(2, *dy.shape), is_grads_batched=True, retain_graph=True)
     assert torch.autograd.grad(y, x, dy)[0].isfinite().all()
+
+
+def test_gradient_norm_refuses_tensors_that_are_not_their_memory():
+    """Fake, dual, batched and lazily negated tensors: nothing is read or written."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from smdistributed_modelparallel_amd.backend.exceptions import SMPInvalidArgumentError
+    from smdistributed_modelparallel_amd.ops.multi_tensor import clip_grad_norm_, grad_norm, grad_power
+
+    x = torch.ones(40, device="cuda")
+    with FakeTensorMode():
+        fake = torch.empty(40, device="cuda")
+    negated = torch._neg_view(x)
+    with fwd.dual_level():
+        for bad in (fake, negated, fwd.make_dual(x.clone(), x)):
+            for call in (grad_norm, grad_power, lambda ts: clip_grad_norm_(ts, 1.0)):
+                with pytest.raises(SMPInvalidArgumentError):
+                    call([x, bad])
+            with pytest.raises(SMPInvalidArgumentError):
+                clip_grad_norm_([x], 1.0, out=[bad])
+    with pytest.raises(SMPInvalidArgumentError):
+        torch.vmap(lambda t: grad_norm([t]))(x.view(4, 10))
+    assert x.eq(1).all()
