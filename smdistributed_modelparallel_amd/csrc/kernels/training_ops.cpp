@@ -331,7 +331,11 @@ class EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
     auto target = [&](const at::Tensor& t, bool marked, Opt& g, bool& add, at::Tensor& result) {
       add = bound(t, marked);
       g = add ? t.grad() : at::empty(t.sizes(), t.options());
-      if (!add) result = *g;
+      if (add) {
+        torch::autograd::impl::bump_version(*g);
+      } else {
+        result = *g;
+      }
     };
     if (ctx->needs_input_grad(0)) target(w, args[3], dw, add_w, out[0]);
     if (two && ctx->needs_input_grad(1)) target(p, args[4], dp, add_p, out[1]);
@@ -582,7 +586,9 @@ class BlockNormFunction : public torch::autograd::Function<BlockNormFunction> {
       if (i == 4 && t.numel() != t.size(-1)) continue;  // a gate with many rows may be written without a partial sum
       bool again = false;  // a parameter used twice is added to in place only once
       for (size_t k = 0; k < i; ++k) again = again || (into[k].has_value() && into[k]->is_same(t.grad()));
-      if (!again) into[i] = t.grad();
+      if (again) continue;
+      into[i] = t.grad();
+      torch::autograd::impl::bump_version(*into[i]);
     }
     const auto out = block_norm_bwd(dy, ds, opt(v[0]), v[1], v[2], opt(v[3]), opt(v[4]), opt(v[5]), opt(v[6]),
                                     ctx->saved_data["gate_rows"].toInt(), ctx->saved_data["alpha"].toDouble(),
@@ -738,8 +744,13 @@ std::vector<at::Tensor> grad_norm(std::vector<at::Tensor> grads, bool inf, doubl
     if (!each)
       for (auto l = lists.rbegin(); l != lists.rend(); ++l)
         check(smpk::grad_scale(*l, size, factor, stream()), "grad_scale");
-    for (size_t i = 0; i < dest.size(); ++i)
-      if (!dest[i].is_same((*out)[i])) (*out)[i].copy_(dest[i]);
+    for (size_t i = 0; i < dest.size(); ++i) {
+      if (dest[i].is_same((*out)[i])) {
+        torch::autograd::impl::bump_version(dest[i]);  // a graph that holds it may not use it any more
+      } else {
+        (*out)[i].copy_(dest[i]);
+      }
+    }
   }
   return {power, norm};
 }

@@ -255,3 +255,36 @@ def test_caller_waits_for_bound_gradients(late):
     got = [w.grad.clone(), v.grad.clone()]
     assert all(torch.equal(a, b) for a, b in zip(got, expect))
     assert keep is None or len(keep) == 2
+
+
+def test_writes_in_place_are_seen_by_graphs():
+    """What autograd saved before a clip, or before a bound gradient grew, it refuses to use after it."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+    from smdistributed_modelparallel_amd.ops.layernorm import block_norm
+    from smdistributed_modelparallel_amd.ops.multi_tensor import clip_grad_norm_
+
+    x = torch.randn(8, 16, device="cuda", requires_grad=True)
+
+    def clip(g):
+        clip_grad_norm_([g], 0.1)
+
+    def clip_into(g):
+        clip_grad_norm_([torch.ones_like(g)], 0.1, out=[g])
+
+    def lookup(g):
+        w = torch.nn.Parameter(torch.randn(8, 16, device="cuda"))
+        w.grad, w._smp_fused_grad = g, True
+        embedding(torch.tensor([1, 2], device="cuda"), w).sum().backward()
+        assert w.grad is g
+
+    def norm(g):
+        w = torch.nn.Parameter(torch.randn(16, device="cuda"))
+        w.grad, w._smp_fused_grad = g[0], True
+        block_norm(x.detach(), x.detach(), w)[0].sum().backward()
+
+    for write in (clip, clip_into, lookup, norm):
+        g = torch.randn(8, 16, device="cuda")
+        loss = (x * g).sum()
+        write(g)
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
