@@ -10,7 +10,7 @@ takes its gradient through autograd: they see it, and may change it, before it i
 A pass that builds a graph of its own (``create_graph``) can be differentiated again.
 CPU tensors use plain torch operations, and so do calls whose launch would go unnoticed: on dual
 numbers (forward-mode derivatives), inside function transforms (``torch.vmap``, ``torch.func``), under
-``torch.jit.trace`` or a dispatch mode, and of tensor classes that dispatch operations themselves.  torch.autocast changes nothing: both tables and the
+``torch.compile``, ``torch.jit.trace`` or a dispatch mode, and of tensor classes that dispatch operations themselves.  torch.autocast changes nothing: both tables and the
 result are of one type.
 """
 import math
@@ -118,7 +118,7 @@ def embedding(ids, weight, padding_idx=None, scale=1.0, vocab_start=None, positi
         elif ids.dim() == 0 or ids.shape[-1] > position_weight.shape[0]:
             raise SMPInvalidArgumentError(f"ids {tuple(ids.shape)} need position_ids: the position table has "
                                           f"{position_weight.shape[0]} rows")
-    if weight.is_cuda:
+    if weight.is_cuda and not torch.compiler.is_compiling():
         start = vocab_start or 0
         y = ext().embedding(weight, position_weight, ids, position_ids, scale, start, vocab_start is not None,
                             -1 if padding_idx is None else padding_idx - start,

@@ -181,8 +181,10 @@ MAX_BLOCK_NORM_ROWS = 1 << 30
 def _block_norm_hip(x, residual, weight, bias, post_weight, post_bias, gate, gate_rows, alpha, eps, rms):
     """[y, s] by the kernels (x None: [y], the norm of residual); parameters bound to the flat
     gradient buffer take their gradients there in place, unless they have hooks that want them.
-    None where the kernels do not take the call: dual numbers, function transforms, traces, dispatch
-    modes, tensor classes that dispatch operations themselves."""
+    None where the kernels do not take the call: dual numbers, function transforms, torch.compile,
+    traces, dispatch modes, tensor classes that dispatch operations themselves."""
+    if torch.compiler.is_compiling():
+        return None
     marks = [int(getattr(t, "_smp_fused_grad", False)) for t in (weight, bias, post_weight, post_bias, gate)]
     return ext().block_norm(x, residual, weight, bias, post_weight, post_bias, gate, gate_rows, alpha, eps, rms, marks)
 

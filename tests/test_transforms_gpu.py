@@ -1,5 +1,5 @@
 """embedding and block_norm where a kernel's launch alone would lose something: dual numbers,
-function transforms, traces, dispatch modes.
+function transforms, compiled functions, traces, dispatch modes.
 
 The embedding is linear in its tables, so its results are held to the formula: one rounding of fp32
 (2^-24) for the product and one for the sum, taken twice.  block_norm's tangents are held to the
@@ -223,3 +223,25 @@ def test_gradient_norm_refuses_tensors_that_are_not_their_memory():
     with pytest.raises(SMPInvalidArgumentError):
         torch.vmap(lambda t: grad_norm([t]))(x.view(4, 10))
     assert x.eq(1).all()
+
+
+def test_compiled_in_one_graph():
+    """torch.compile sees torch's operations, in values and gradients."""
+    from smdistributed_modelparallel_amd.nn import DistributedEmbedding
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+    from smdistributed_modelparallel_amd.ops.layernorm import block_norm, rms_norm
+
+    w, p, _, _, ids = tables()
+    m, v = DistributedEmbedding(9, 24, padding_idx=3).cuda(), torch.randn(24, device="cuda")
+    w.requires_grad_()
+
+    def f(ids):
+        x = embedding(ids, w, scale=0.5, position_weight=p) + m(ids)
+        return (*block_norm(x, 2 * x, v, gate=v), rms_norm(x, v))
+
+    got, want = torch.compile(f, backend="eager", fullgraph=True)(ids), f(ids)
+    for a, b in zip(got, want):
+        near(a, b, 2.0 ** -14)
+    dy = [torch.randn_like(o) for o in want]
+    for a, b in zip(torch.autograd.grad(got, [w, m.weight], dy), torch.autograd.grad(want, [w, m.weight], dy)):
+        near(a, b, 2.0 ** -14)
