@@ -6,6 +6,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/variable.h>
@@ -43,13 +44,16 @@ void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " launch faile
 // A tensor that is its memory and nothing else, as the kernels take it.  Not so: dual numbers, the
 // tensors of function transforms (vmap, torch.func) and of classes that dispatch operations themselves
 // (fake or distributed ones), lazily negated and zero tensors.
-bool plain(const at::Tensor& t) {
+bool plain(const at::Tensor& t, bool duals) {
   using Key = c10::DispatchKey;
   static const c10::DispatchKeySet other({Key::Python, Key::Batched, Key::FuncTorchBatched, Key::FuncTorchGradWrapper,
                                           Key::BatchedNestedTensor, Key::Functionalize, Key::Conjugate, Key::Negative,
                                           Key::ZeroTensor});
-  return !t.key_set().has_any(other) && !t.is_nested() && !t._fw_grad(/*level=*/0).defined();
+  return !t.key_set().has_any(other) && !t.is_nested() && !(duals && t._fw_grad(/*level=*/0).defined());
 }
+
+// There may be dual numbers: asked once a call, a tensor's own tangent takes a lock.
+bool duals_live() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
 
 // No trace, mode or function transform is active, which would have to know of the launch.
 bool unobserved() {
@@ -307,7 +311,7 @@ class EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
     const at::Tensor p = two ? ctx->saved_data["pos_weight"].toTensor() : at::Tensor();
     check_capture({w, p}, "embedding");
     variable_list out(11);
-    if (!plain(grads[0])) {
+    if (!plain(grads[0], duals_live())) {
       const at::Tensor dy = grads[0].reshape({-1, w.size(1)});
       const at::Tensor at = saved[1].defined() ? saved[1] : at::arange(dy.size(0), saved[0].options()).remainder(args[0]);
       if (ctx->needs_input_grad(0)) out[0] = table_gradient(dy, saved[0], w.sizes(), scale, args[1], args[2]);
@@ -374,8 +378,9 @@ at::Tensor embedding(at::Tensor weight, Opt pos_weight, at::Tensor ids, Opt pos,
 // None where the kernels do not take the call: the caller has the same in torch's operations
 Opt embedding_call(at::Tensor weight, Opt pos_weight, at::Tensor ids, Opt pos, double scale, int64_t start,
                    bool foreign_zero, int64_t skip, bool mark_w, bool mark_p) {
-  bool take = unobserved() && plain(weight) && plain(ids);
-  for (const Opt* t : {&pos_weight, &pos}) take = take && (!t->has_value() || plain(**t));
+  const bool duals = duals_live();
+  bool take = unobserved() && plain(weight, duals) && plain(ids, duals);
+  for (const Opt* t : {&pos_weight, &pos}) take = take && (!t->has_value() || plain(**t, duals));
   if (!take) return c10::nullopt;
   return embedding(weight, pos_weight, ids, pos, scale, start, foreign_zero, skip, mark_w, mark_p);
 }
@@ -570,7 +575,8 @@ class BlockNormFunction : public torch::autograd::Function<BlockNormFunction> {
     const Opt dy = opt(grads[0].defined() ? grads[0].contiguous() : grads[0]);
     const Opt ds = grads.size() > 1 ? opt(grads[1].defined() ? grads[1].contiguous() : grads[1]) : Opt();
     if (!dy.has_value() && !ds.has_value()) return result;
-    TORCH_CHECK((!dy.has_value() || plain(*dy)) && (!ds.has_value() || plain(*ds)),
+    const bool duals = duals_live();
+    TORCH_CHECK((!dy.has_value() || plain(*dy, duals)) && (!ds.has_value() || plain(*ds, duals)),
                 "block_norm: the gradient of an output must be a plain tensor, not a dual, batched or otherwise wrapped "
                 "one (calls made inside a function transform or on dual numbers take such gradients)");
     const auto v = ctx->get_saved_variables();
@@ -605,8 +611,9 @@ class BlockNormFunction : public torch::autograd::Function<BlockNormFunction> {
 c10::optional<variable_list> block_norm(Opt x, at::Tensor res, at::Tensor w, Opt b, Opt pw, Opt pb, Opt gate, int64_t gate_rows,
                          double alpha, double eps, bool rms, std::vector<int64_t> marks) {
   TORCH_CHECK(marks.size() == 5, "block_norm: bad lists");
-  bool take = unobserved() && plain(res) && plain(w);
-  for (const Opt* t : {&x, &b, &pw, &pb, &gate}) take = take && (!t->has_value() || plain(**t));
+  const bool duals = duals_live();
+  bool take = unobserved() && plain(res, duals) && plain(w, duals);
+  for (const Opt* t : {&x, &b, &pw, &pb, &gate}) take = take && (!t->has_value() || plain(**t, duals));
   if (!take) return c10::nullopt;
   auto dense = [](Opt& t) {
     if (t.has_value()) t = t->contiguous();
@@ -669,6 +676,7 @@ std::vector<at::Tensor> grad_norm(std::vector<at::Tensor> grads, bool inf, doubl
   TORCH_CHECK_VALUE(!grads.empty() && grads[0].defined() && grads[0].is_cuda(), "no GPU tensors");
   const at::Device device = grads[0].device();
   const c10::DeviceGuard guard(device);
+  const bool duals = duals_live();
   int64_t total = 0;
   std::vector<at::Tensor> dest;
   if (out.has_value()) {
@@ -677,14 +685,14 @@ std::vector<at::Tensor> grad_norm(std::vector<at::Tensor> grads, bool inf, doubl
   }
   for (size_t i = 0; i < grads.size(); ++i) {
     at::Tensor& t = grads[i];
-    TORCH_CHECK_VALUE(t.defined() && t.layout() == at::kStrided && is_float(t) && plain(t), "tensor ", i,
+    TORCH_CHECK_VALUE(t.defined() && t.layout() == at::kStrided && is_float(t) && plain(t, duals), "tensor ", i,
                       " is none of them (or no plain tensor)");
     TORCH_CHECK_VALUE(t.device() == device, "tensor ", i, " is on ", t.device(), ", not on ", device);
     total += t.numel();
     if (out.has_value()) {
       at::Tensor& o = dest[i];
-      TORCH_CHECK_VALUE(o.defined() && o.layout() == at::kStrided && is_float(o) && plain(o) && o.device() == device &&
-                            o.sizes() == t.sizes(),
+      TORCH_CHECK_VALUE(o.is_same(t) || (o.defined() && o.layout() == at::kStrided && is_float(o) && plain(o, duals) &&
+                                         o.device() == device && o.sizes() == t.sizes()),
                         "output ", i, " differs from its gradient in shape or device, or is none of them");
       for (int64_t k = 0; k < o.dim(); ++k)
         TORCH_CHECK_VALUE(o.stride(k) != 0 || o.size(k) <= 1, "output ", i, " is expanded: it cannot be written");

@@ -10,8 +10,8 @@ takes its gradient through autograd: they see it, and may change it, before it i
 A pass that builds a graph of its own (``create_graph``) can be differentiated again.
 CPU tensors use plain torch operations, and so do calls whose launch would go unnoticed: on dual
 numbers (forward-mode derivatives), inside function transforms (``torch.vmap``, ``torch.func``), under
-``torch.compile``, ``torch.jit.trace`` or a dispatch mode, and of tensor classes that dispatch operations themselves.  torch.autocast changes nothing: both tables and the
-result are of one type.
+``torch.compile``, ``torch.jit.trace`` or a dispatch mode, and of tensor classes that dispatch
+operations themselves.  torch.autocast changes nothing: both tables and the result are of one type.
 """
 import math
 
@@ -27,7 +27,8 @@ def _rows_torch(ids, table, padding_idx, fill):
     outside = (ids < 0) | (ids >= rows)
     if padding_idx is not None and not 0 <= padding_idx < rows:
         padding_idx = None
-    return torch.nn.functional.embedding(ids.clamp(0, rows - 1), table, padding_idx).masked_fill(outside.unsqueeze(-1), fill)
+    y = torch.nn.functional.embedding(ids.clamp(0, rows - 1), table, padding_idx)
+    return y.masked_fill(outside.unsqueeze(-1), fill)
 
 
 def _embedding_torch(ids, weight, padding_idx, scale, vocab_start, position_ids, position_weight, nan_outside=False):
@@ -58,8 +59,12 @@ MAX_VECTORS = ((1 << 24) - 1) * 1024  # of 8 elements, in the output: what one l
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
-def _sizes_ok(ids, weight):
-    return ids.numel() <= MAX_TOKENS and ids.numel() * ((weight.shape[1] + 7) // 8) <= MAX_VECTORS
+def _table_ok(rows, dim):
+    return rows < MAX_ROWS and dim <= MAX_COLUMNS
+
+
+def _list_ok(n, dim):
+    return n <= MAX_TOKENS and n * ((dim + 7) // 8) <= MAX_VECTORS
 
 
 def _check_ids(name, t, device):
@@ -81,13 +86,14 @@ def embedding(ids, weight, padding_idx=None, scale=1.0, vocab_start=None, positi
     (broadcast to ``ids``) or, without them, by the place in the last dimension."""
     if not torch.is_tensor(weight) or weight.dim() != 2 or weight.dtype not in _FLOATS or 0 in weight.shape:
         raise SMPInvalidArgumentError("weight must be a [rows, dim] fp32 / fp16 / bf16 tensor")
-    if weight.shape[0] >= MAX_ROWS or weight.shape[1] > MAX_COLUMNS:
-        raise SMPInvalidArgumentError(f"tables of fewer than {MAX_ROWS} rows, of at most {MAX_COLUMNS} columns, are supported")
     _check_ids("ids", ids, weight.device)
-    if not _sizes_ok(ids, weight):
-        raise SMPInvalidArgumentError(f"{ids.numel()} tokens of {weight.shape[1]} in one call: at most {MAX_TOKENS} tokens and "
-                                      f"{8 * MAX_VECTORS} elements are supported")
-    rows = weight.shape[0]
+    rows, dim = weight.shape
+    if not _table_ok(rows, dim):
+        raise SMPInvalidArgumentError(f"tables of fewer than {MAX_ROWS} rows, of at most {MAX_COLUMNS} columns, are supported")
+    n = ids.numel()
+    if not _list_ok(n, dim):
+        raise SMPInvalidArgumentError(f"{n} tokens of {dim} in one call: at most {MAX_TOKENS} tokens and {8 * MAX_VECTORS} "
+                                      f"elements are supported")
     scale = float(scale)
     if not math.isfinite(scale):
         raise SMPInvalidArgumentError(f"scale must be finite, got {scale}")
@@ -132,7 +138,6 @@ def embedding(ids, weight, padding_idx=None, scale=1.0, vocab_start=None, positi
 def lookup(ids, weight, padding_idx=None, vocab_start=None):
     """``embedding`` without scale and positions, for modules: tables of other types (fp64), empty
     shards, and tables or lists beyond the kernels' sizes go through plain torch operations."""
-    if weight.dtype in _FLOATS and 0 not in weight.shape and weight.shape[0] < MAX_ROWS \
-            and weight.shape[1] <= MAX_COLUMNS and _sizes_ok(ids, weight):
+    if weight.dtype in _FLOATS and 0 not in weight.shape and _table_ok(*weight.shape) and _list_ok(ids.numel(), weight.shape[1]):
         return embedding(ids, weight, padding_idx, vocab_start=vocab_start)
     return _embedding_torch(ids, weight, padding_idx, 1.0, vocab_start, None, None)
