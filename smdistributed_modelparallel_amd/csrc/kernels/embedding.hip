@@ -8,8 +8,9 @@
 // brought into the order of their rows first (bound by latency: 27 us for 65536 tokens), then every
 // row of dy is read once and every row of dW written once (bound by HBM).
 //
-// Measured, 65536 tokens, 50257 x 1600 bf16, with a table of 2048 positions: forward 73 us; sums and
-// zeros of both tables 117 us (580 MB, 5.0 TB/s); joins 9 us.  One block for each row of the table,
+// Measured, 65536 tokens, 50257 x 1600 bf16, with a table of 2048 positions: forward 73 us after other work,
+// 65 us of a table that was read just before; sums and zeros of both tables 118 us (580 MB, 4.9 TB/s); joins
+// 9 us.  One block for each row of the table,
 // which looked for its tokens in all ids, took 3400 us.
 #include "kernels.h"
 #include "vec8.h"
@@ -19,8 +20,9 @@ namespace {
 
 constexpr int kT = 256;
 constexpr int64_t kMostBlocks = (1ll << 32) / kT;  // a grid's threads stay below 2^32
-// Longest list that is ordered in one launch: 8192 ids of a vocabulary of 12608 take 14 us so, and
-// 19 us in one block's registers; 65536 ids of 50257 take 80 us, and 28 us in radix passes.
+// Longest list that is ordered in one launch.  The whole gradient of lists of a vocabulary of 50257, 8 bf16
+// columns, so and by radix passes: 8192 tokens 40 and 51 us, 16384 51 and 57 us, 24576 59 us both, 65536 93
+// and 58 us.
 constexpr int64_t kRangeTokens = 16384;
 constexpr int64_t kRangeBlocks = 256;  // blocks of that launch: one for each CU
 
@@ -37,8 +39,8 @@ constexpr int kPerThread = 4;  // vectors of a thread, all loads in flight toget
 // Threads past the end and tokens without a row load row 0 and drop it: no branch separates the
 // loads.  slice: an XCD (every kXcds-th block) takes `slice` blocks of each sequence, the same
 // positions of all of them (or nearly: in whole blocks), so that its L2 holds their rows.  32 x 1000 tokens of 1600
-// bf16: 33 us, and 43 us with the blocks in order; 32 x 2048, whose sequences are multiples of kXcds
-// blocks in any case: 84 us both.
+// bf16: 30 us, and 40 us with the blocks in order; 32 x 2048, whose sequences are multiples of kXcds
+// blocks in any case: 65 us both; 64 x 512, whose are not quite: 32 and 28 us.
 constexpr uint32_t kXcds = 8;
 template <typename T, bool FULL>
 __global__ void __launch_bounds__(kT) emb_fwd(IndexList ids, const T* __restrict__ w, int64_t w_stride, float scale,
@@ -124,7 +126,9 @@ __global__ void __launch_bounds__(kT) emb_fwd(IndexList ids, const T* __restrict
 // consecutive run of the items, each wave a consecutive part of it; the waves count their digits,
 // the counts become the places of each wave's items, and the wave walks over its items once more,
 // 64 at a time, in order.  No place depends on the order in which anything runs.  65536 tokens:
-// 8.5 us to count and 4.8 us to place, each pass; both are the latency of few blocks.
+// 5.0 us to count and 8.7 us to place, each pass; both are the latency of few blocks.  Every block reads the
+// counts of all: 256 blocks up to 2 M tokens, more above.  Gradient of 8 bf16 columns: 2^22 tokens 0.58 ms,
+// 2^24 2.2 ms, 2^27 39 ms.
 constexpr int kWaves = 16;
 constexpr int kSortThreads = kWaves * 64;
 constexpr int kMaxBits = 10;
@@ -406,7 +410,9 @@ struct Work {
 
 constexpr int kZeroRows = 16;
 // Cleared rows of a table that the caches hold (256 MB, of which the reads need a part) go through
-// them: 62 MB 15.7 us against 21.7 us past them; 155 MB 35.2 us against 28.9 us.
+// them: 62 MB of fp32 15.7 us against 21.7 us past them; 155 MB of fp16 35.2 us against 28.9 us.  Of bf16
+// tables alone, replayed, the zeros past the caches are ahead earlier: 64 MB 25 and 22 us for the whole
+// gradient, 96 MB 30 and 26 us, 128 MB 36 and 30 us.
 constexpr int64_t kCached = 96ll << 20;
 
 // 512 columns of the rows of a bit mask, every fourth of them for this wave, become zero; `at`: the

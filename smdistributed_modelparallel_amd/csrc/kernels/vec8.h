@@ -46,10 +46,11 @@ __device__ __forceinline__ void read8(const T* p, int left, float (&o)[kCols]) {
 
 // STREAM: past the caches, for outputs that are written once, in whole lines, and that no kernel
 // finds there later.  Stored normally and so: the gradient of a 50257 x 1600 bf16 table 132 and
-// 118 us; block norms of 16384 x 1600 bf16 52 and 45 us forward, 92 and 90 us backward.  Not where
-// a table's reads want the memory too (65536 gathered rows of a cold table: 76 and 82 us), where
-// what is written is what was just read (clip of 1.4 GB: 837 and 926 us with the norm), nor for
-// rows of fp32, whose lanes write half lines.
+// 118 us; block norms of 16384 rows forward, 1600 bf16 44 and 43 us, 4096 bf16 107 and 94 us, 1600 fp32 91 and
+// 70 us, backward, 1600 bf16 82 and 72 us.  Not where a table's reads want the memory too (65536 gathered
+// rows of a cold table: 76 and 82 us; 65 and 52 us of one that was read just before), where what is written is
+// what was just read (clip of 1.4 GB: 837 and 926 us with the norm), nor for rows of fp32 in the backward,
+// whose lanes write half lines.
 template <bool FULL, bool STREAM, typename T>
 __device__ __forceinline__ void write8(T* p, int left, const float (&o)[kCols]) {
   constexpr int M = 16 / sizeof(T);

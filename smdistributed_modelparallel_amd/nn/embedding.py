@@ -7,6 +7,9 @@
   ids are masked, and the partial lookups are summed with a reduce-scatter (own batch) or
   all-reduce (``_output_full_batch``, used by the vocab-parallel LM head).
 Uneven splits follow ``get_local_channels``.
+
+Nothing waits for the token ids on the GPU: one that is no row of the (whole) vocabulary gives a row
+of NaN there and takes no gradient (in a vocabulary shard, zeros); on the CPU it is an IndexError.
 """
 import torch
 import torch.nn as nn

@@ -960,7 +960,9 @@ class DistributedTransformerLMHead(DistributedModule):
 
     def _embed(self, input_ids, position_ids, default_positions):
         """Token embeddings plus position embeddings: one kernel for both tables where their modules
-        are plain lookups of this process (same bits as the two lookups and their sum)."""
+        are plain lookups of this process (same bits as the two lookups and their sum).  An id or
+        position outside its table gives a row of NaN then, where the modules' lookups stop the
+        program by a device assertion."""
         word = self.word_embedding
         pos = self.position_embedding if self.use_positional_embedding else None
         if _plain_lookup(word) and (pos is None or (_plain_lookup(pos) and pos.weight.dtype == word.weight.dtype)):

@@ -247,7 +247,9 @@ def block_norm(x, residual, weight, bias=None, post_weight=None, post_bias=None,
         s = residual + residual_scale * gate * h
         y = norm(s; weight, bias)
 
-    -> ``(y, s)``, in one kernel each way.  ``norm`` is LayerNorm or, with ``rms``, the
+    -> ``(y, s)``, in one kernel each way (two backward for rows above 6144).  Without a gate and a
+    norm after the block it is ``add_layer_norm`` without dropout, and keeps x and the residual for
+    the backward, where that keeps their sum.  ``norm`` is LayerNorm or, with ``rms``, the
     root-mean-square norm.  ``x`` and ``residual`` [..., dim] are alike; the weights and biases
     [dim] have their dtype or are fp32.  ``gate`` (that dtype or fp32) broadcasts to ``x``: one
     vector, one for each sample ([batch, 1, dim]), or one value for each element; None is 1.
