@@ -313,9 +313,10 @@ class EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
     variable_list out(11);
     if (!plain(grads[0], duals_live())) {
       const at::Tensor dy = grads[0].reshape({-1, w.size(1)});
-      const at::Tensor at = saved[1].defined() ? saved[1] : at::arange(dy.size(0), saved[0].options()).remainder(args[0]);
+      const at::Tensor place =
+          saved[1].defined() ? saved[1] : at::arange(dy.size(0), saved[0].options()).remainder(args[0]);
       if (ctx->needs_input_grad(0)) out[0] = table_gradient(dy, saved[0], w.sizes(), scale, args[1], args[2]);
-      if (two && ctx->needs_input_grad(1)) out[1] = table_gradient(dy, at, p.sizes(), 1.0, 0, -1);
+      if (two && ctx->needs_input_grad(1)) out[1] = table_gradient(dy, place, p.sizes(), 1.0, 0, -1);
       return out;
     }
     const at::Tensor dy = grads[0].reshape({-1, w.size(1)}).contiguous();
@@ -753,8 +754,8 @@ std::vector<at::Tensor> grad_norm(std::vector<at::Tensor> grads, bool inf, doubl
       for (auto l = lists.rbegin(); l != lists.rend(); ++l)
         check(smpk::grad_scale(*l, size, factor, stream()), "grad_scale");
     for (size_t i = 0; i < dest.size(); ++i) {
-      if (dest[i].is_same((*out)[i])) {
-        torch::autograd::impl::bump_version(dest[i]);  // a graph that holds it may not use it any more
+      if (dest[i].is_same((*out)[i])) {  // a graph that holds it may not use it any more
+        if (!dest[i].is_inference()) torch::autograd::impl::bump_version(dest[i]);
       } else {
         (*out)[i].copy_(dest[i]);
       }

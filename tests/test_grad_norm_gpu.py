@@ -178,3 +178,14 @@ def test_same_bits_and_graph_replays():
         got = [norm.clone()] + [o.clone() for o in out]
         eager = [clip_grad_norm_(ts, 3.0, out=out)] + out
         assert all(torch.equal(a, b) for a, b in zip(got, eager))
+
+
+def test_inference_tensors():
+    """They have no versions to count."""
+    from smdistributed_modelparallel_amd.ops.multi_tensor import clip_grad_norm_
+
+    with torch.inference_mode():
+        x = torch.ones(16, device="cuda")
+        assert float(clip_grad_norm_([x], 2.0)) == 4.0
+    assert float(clip_grad_norm_([x], 1.0)) == pytest.approx(2.0, rel=1e-6)
+    assert float(x.sum()) == pytest.approx(4.0, rel=1e-6)
