@@ -288,3 +288,37 @@ def test_writes_in_place_are_seen_by_graphs():
         write(g)
         with pytest.raises(RuntimeError, match="inplace"):
             loss.backward()
+
+
+def test_captured_bound_gradients():
+    """A captured backward adds to bound gradients at every replay what the eager one adds."""
+    from smdistributed_modelparallel_amd.ops.embedding import embedding
+    from smdistributed_modelparallel_amd.ops.layernorm import block_norm
+
+    torch.manual_seed(4)
+    table, place, scale = (torch.randn(n, device="cuda") for n in ((700, 136), (60, 136), (136,)))
+    ids, dy = torch.randint(0, 700, (20, 50), device="cuda"), torch.randn(20, 50, 136, device="cuda")
+
+    def step(w, p, v):
+        x = embedding(ids, w, position_weight=p, padding_idx=3)
+        y, s = block_norm(x, x, v, gate=v)
+        torch.autograd.backward([y, s], [dy, dy])
+
+    captured, eager = _bound(table, place, scale), _bound(table, place, scale)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*captured)
+    torch.cuda.current_stream().wait_stream(side)
+    for t in captured:
+        t.grad.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(*captured)
+    for k in range(3):
+        ids.copy_(torch.randint(0, 700 >> (3 * k), (20, 50), device="cuda"))
+        dy.normal_()
+        graph.replay()
+        step(*eager)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a.grad, b.grad) for a, b in zip(captured, eager))
